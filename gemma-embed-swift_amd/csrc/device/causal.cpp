@@ -1,0 +1,260 @@
+// Per-op entries of causal models' attention (ge_op_attention_causal, ge_op_attention_prefix): checks,
+// the plan of a call's work, and its launches.
+//
+// A call's rows are tiled per base: a sequence against its own keys, and, over a shared prefix, either
+// a run of neighbouring sequences whose rows all see the whole prefix (their rows stack up, so the
+// prefix is read once per tile of rows and not once per sequence) or one sequence that does not. Each
+// tile's visible keys are split until the launch fills the GPU; rows that end in more than one part are
+// joined by a second launch.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <vector>
+
+#include "causal.hpp"
+#include "runtime_internal.hpp"
+
+namespace ge {
+namespace {
+
+// Split tiles: keys an item takes at least (a split costs its rows' partial results and a share of the
+// joining launch), and the workgroups a launch is split up to.
+constexpr int64_t kSplitMinKeys = 256, kSplitGroups = 512;
+constexpr int64_t kMaxRows = int64_t(1) << 30, kMaxStride = int64_t(1) << 24;
+
+struct Tile {
+    uint32_t row0, n_rows, part;
+    int64_t lo, hi;  // visible keys of its rows
+    uint32_t splits;
+};
+
+struct Base {
+    uint32_t q_token, key0, source;
+    int64_t tokens, keys, shift;
+    bool direct;  // its rows have no other part
+    std::vector<Tile> tiles;
+};
+
+struct Plan {
+    std::vector<CausalItem> items;
+    std::vector<CausalJoin> joins;
+    size_t part_rows = 0;
+    int kinds = 0;
+};
+
+Base make_base(uint32_t q_token, int64_t tokens, uint32_t source, uint32_t key0, int64_t keys, int64_t shift, int group,
+               int window, int wide, bool direct) {
+    Base b{q_token, key0, source, tokens, keys, shift, direct, {}};
+    const int64_t rows = tokens * group;
+    for (int64_t r = 0; r < rows; r += wide) {
+        const int64_t n = std::min<int64_t>(wide, rows - r), i0 = r / group, i1 = (r + n - 1) / group;
+        Tile t{uint32_t(r), uint32_t(n), 0, 0, 0, 0};
+        t.lo = window ? std::max<int64_t>(0, i0 + shift - window + 1) : 0;
+        t.hi = std::min(keys, i1 + shift + 1);
+        if (t.hi <= t.lo) t.lo = t.hi = 0;
+        b.tiles.push_back(t);
+    }
+    return b;
+}
+
+Plan make_plan(const ge_attention_shape& s, const ge_attention_seq* seqs, int n_seqs, int64_t prefix_len) {
+    const int group = s.heads / s.kv_heads, wide = causal_wide_rows(s.head_dim);
+    std::vector<Base> bases;
+    struct Use {
+        int own = -1, prefix = -1;
+        int64_t prefix_row = 0;  // the sequence's first row in its prefix base
+    };
+    std::vector<Use> use(size_t(n_seqs), Use{});
+    for (int i = 0; i < n_seqs; i++) {
+        const ge_attention_seq& q = seqs[i];
+        if (!q.q_len || (prefix_len && !q.kv_len)) continue;
+        use[size_t(i)].own = int(bases.size());
+        bases.push_back(make_base(q.q_start, q.q_len, 0, q.kv_start, q.kv_len, int64_t(q.kv_len) - q.q_len, group, s.window,
+                                  wide, prefix_len == 0));
+    }
+    for (int i = 0; prefix_len && i < n_seqs;) {
+        if (!seqs[i].q_len) {
+            i++;
+            continue;
+        }
+        // every row of such a sequence sees the whole prefix, wherever it stands
+        auto whole = [&](const ge_attention_seq& q) { return s.window == 0 && int64_t(q.q_len) <= int64_t(q.kv_len) + 1; };
+        int64_t tokens = seqs[i].q_len, shift = prefix_len + seqs[i].kv_len - int64_t(seqs[i].q_len);
+        bool alone = seqs[i].kv_len == 0;
+        int j = i + 1;
+        use[size_t(i)].prefix = int(bases.size());
+        if (whole(seqs[i])) {
+            shift = kMaxRows;
+            for (; j < n_seqs && whole(seqs[j]) && seqs[j].q_start == seqs[i].q_start + uint64_t(tokens); j++) {
+                use[size_t(j)].prefix = int(bases.size());
+                use[size_t(j)].prefix_row = tokens * group;
+                tokens += seqs[j].q_len;
+                alone = alone && seqs[j].kv_len == 0;
+            }
+        }
+        bases.push_back(make_base(seqs[i].q_start, tokens, 1, 0, prefix_len, shift, group, s.window, wide, alone));
+        i = j;
+    }
+
+    int64_t keys = 0;
+    for (const Base& b : bases)
+        for (const Tile& t : b.tiles) keys += t.hi - t.lo;
+    const int64_t limit =
+        (std::max(kSplitMinKeys, (keys * s.kv_heads + kSplitGroups - 1) / kSplitGroups) + 63) / 64 * 64;
+    Plan p;
+    for (Base& b : bases)
+        for (Tile& t : b.tiles) {
+            const int64_t n = t.hi - t.lo, splits = (n + limit - 1) / limit;
+            // 64-key steps keep the parts' blocks whole
+            const int64_t step = splits ? (n + splits * 64 - 1) / (splits * 64) * 64 : 0;
+            const bool narrow = t.n_rows <= uint32_t(kCausalNarrowRows), direct = b.direct && splits <= 1;
+            t.part = uint32_t(p.part_rows);
+            for (int64_t k = t.lo; k < t.hi || (direct && t.splits == 0); k += step) {
+                p.items.push_back(CausalItem{b.q_token, t.row0, t.n_rows, b.key0, uint32_t(k), uint32_t(std::min(k + step, t.hi)),
+                                             int32_t(b.shift), direct ? kDirect : uint32_t(p.part_rows), b.source, narrow});
+                p.kinds |= narrow ? 2 : 1;
+                t.splits++;
+                if (direct) break;
+                p.part_rows += t.n_rows;
+            }
+            if (p.part_rows >= kDirect) fail(GE_ERR_INVALID, "attention: the call's rows and keys are too many for one call");
+        }
+    // The longest items first, so the last ones to start are short.
+    std::stable_sort(p.items.begin(), p.items.end(), [](const CausalItem& a, const CausalItem& b) {
+        return (a.k_hi - a.k_lo) * (a.narrow ? 1 : 4) > (b.k_hi - b.k_lo) * (b.narrow ? 1 : 4);
+    });
+
+    for (int i = 0; i < n_seqs; i++) {
+        const Use& u = use[size_t(i)];
+        const Base* const side[2] = {u.own >= 0 ? &bases[size_t(u.own)] : nullptr,
+                                     u.prefix >= 0 ? &bases[size_t(u.prefix)] : nullptr};
+        const int64_t first[2] = {0, u.prefix_row}, rows = int64_t(seqs[i].q_len) * group;
+        for (int64_t r = 0; r < rows;) {
+            CausalJoin j{seqs[i].q_start, uint32_t(r), 0, {}, {}, {}};
+            int64_t end = rows;
+            bool written = false;
+            for (int k = 0; k < 2; k++) {
+                if (!side[k]) continue;
+                const int64_t at = first[k] + r;
+                const Tile& t = side[k]->tiles[size_t(at / wide)];
+                j.part[k] = t.part + uint32_t(at - t.row0);
+                j.stride[k] = t.n_rows;
+                j.splits[k] = t.splits;
+                end = std::min(end, int64_t(t.row0) + t.n_rows - first[k]);
+                written = written || (side[k]->direct && t.splits <= 1);
+            }
+            j.n_rows = uint32_t(end - r);
+            if (!written) p.joins.push_back(j);
+            r = end;
+        }
+    }
+    return p;
+}
+
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+void check_stride(const char* what, int64_t& stride, int64_t width) {
+    if (stride == 0) stride = width;
+    if (stride < width || stride % 8 || stride > kMaxStride)
+        fail(GE_ERR_INVALID, "attention: %s row stride %lld (a multiple of 8 from %lld to %lld elements, or 0)", what,
+             static_cast<long long>(stride), static_cast<long long>(width), static_cast<long long>(kMaxStride));
+}
+
+void attend(ge_ctx* c, const ge_attention_shape* shape, const void* q, const void* prefix_k, const void* prefix_v,
+            int64_t prefix_len, const void* k, const void* v, const ge_attention_seq* seqs, int n_seqs, void* out) {
+    if (!shape) fail(GE_ERR_INVALID, "attention: null shape");
+    ge_attention_shape s = *shape;
+    if (s.type != GE_TYPE_F16 && s.type != GE_TYPE_BF16) fail(GE_ERR_INVALID, "attention: type %d is neither F16 nor BF16", s.type);
+    if (!causal_head_dim_ok(s.head_dim)) fail(GE_ERR_INVALID, "attention: head dim %d (64, 128, 256 or 512)", s.head_dim);
+    if (s.heads <= 0 || s.kv_heads <= 0 || s.heads % s.kv_heads || s.heads > 4096)
+        fail(GE_ERR_INVALID, "attention: %d query heads over %d KV heads (a multiple, up to 4096)", s.heads, s.kv_heads);
+    if (s.q_rows < 0 || s.kv_rows < 0 || prefix_len < 0 || s.q_rows >= kMaxRows || s.kv_rows >= kMaxRows ||
+        prefix_len >= kMaxRows || s.window < 0 || s.window >= kMaxRows || n_seqs < 0)
+        fail(GE_ERR_INVALID, "attention: rows, prefix, window and sequences from 0 to under 2^30");
+    if (int64_t(s.q_rows) * (s.heads / s.kv_heads) >= kMaxRows)
+        fail(GE_ERR_INVALID, "attention: %d rows of %d query heads a KV head pass 2^30", s.q_rows, s.heads / s.kv_heads);
+    if (!std::isfinite(s.scale)) fail(GE_ERR_INVALID, "attention: scale is not finite");
+    const int64_t kv_width = int64_t(s.kv_heads) * s.head_dim, q_width = int64_t(s.heads) * s.head_dim;
+    check_stride("q", s.q_stride, q_width);
+    check_stride("k", s.k_stride, kv_width);
+    check_stride("v", s.v_stride, kv_width);
+    check_stride("out", s.out_stride, q_width);
+    if (n_seqs == 0) return;
+    if (!seqs) fail(GE_ERR_INVALID, "attention: null sequences");
+    uint64_t q_end = 0, kv_end = 0;
+    for (int i = 0; i < n_seqs; i++) {
+        const ge_attention_seq& e = seqs[i];
+        if (e.q_start < q_end && e.q_len) fail(GE_ERR_INVALID, "attention: sequence %d's query rows start before the last one's end", i);
+        if (uint64_t(e.q_start) + e.q_len > uint64_t(s.q_rows) || uint64_t(e.kv_start) + e.kv_len > uint64_t(s.kv_rows))
+            fail(GE_ERR_INVALID, "attention: sequence %d: query rows [%u, +%u) of %d, key rows [%u, +%u) of %d", i, e.q_start,
+                 e.q_len, s.q_rows, e.kv_start, e.kv_len, s.kv_rows);
+        if (e.q_len) q_end = uint64_t(e.q_start) + e.q_len;
+        if (e.q_len && e.kv_len) kv_end = 1;
+    }
+    if (q_end == 0) return;
+    if (!q || !out || (kv_end && (!k || !v)) || (prefix_len && (!prefix_k || !prefix_v)))
+        fail(GE_ERR_INVALID, "attention: q, out, and k and v of every key row");
+    if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(out) || !aligned(prefix_k) || !aligned(prefix_v))
+        fail(GE_ERR_INVALID, "attention: buffers are 16-byte aligned");
+
+    const Plan p = make_plan(s, seqs, n_seqs, prefix_len);
+    if (p.items.size() * uint64_t(s.kv_heads) > kCausalMaxGroups || p.joins.size() * uint64_t(s.kv_heads) > kCausalMaxGroups)
+        fail(GE_ERR_INVALID, "attention: the call's rows and keys are too many for one call");
+    OpTemps temps(c);
+    const size_t item_bytes = (p.items.size() * sizeof(CausalItem) + 255) / 256 * 256;
+    unsigned char* const lists = op_lists(c, item_bytes + p.joins.size() * sizeof(CausalJoin));
+    std::copy(p.items.begin(), p.items.end(), reinterpret_cast<CausalItem*>(lists));
+    std::copy(p.joins.begin(), p.joins.end(), reinterpret_cast<CausalJoin*>(lists + item_bytes));
+    const size_t o_at = temps.reserve(p.part_rows * size_t(kv_width) * 4);
+    const size_t ml_at = temps.reserve(p.part_rows * size_t(s.kv_heads) * 8);
+    unsigned char* const base = p.part_rows ? temps.base() : nullptr;
+
+    CausalArgs a{};
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k);
+    a.v = static_cast<const uint16_t*>(v);
+    a.prefix_k = static_cast<const uint16_t*>(prefix_k);
+    a.prefix_v = static_cast<const uint16_t*>(prefix_v);
+    a.out = static_cast<uint16_t*>(out);
+    a.items = reinterpret_cast<const CausalItem*>(lists);
+    a.joins = reinterpret_cast<const CausalJoin*>(lists + item_bytes);
+    a.part_o = reinterpret_cast<float*>(base + o_at);
+    a.part_ml = reinterpret_cast<float2*>(base + ml_at);
+    a.q_stride = s.q_stride;
+    a.k_stride = s.k_stride;
+    a.v_stride = s.v_stride;
+    a.out_stride = s.out_stride;
+    a.part_rows = p.part_rows;
+    a.n_items = int(p.items.size());
+    a.n_joins = int(p.joins.size());
+    a.group = s.heads / s.kv_heads;
+    a.kv_heads = s.kv_heads;
+    a.window = s.window;
+    // a hidden key's -inf times this stays -inf, also at scale 0
+    a.c = std::min(std::max(std::fabs(s.scale) * 1.4426950408889634f, FLT_MIN), FLT_MAX);
+    a.q_flip = s.scale < 0.0f ? 0x80008000u : 0u;
+    launch(c, "attention_causal", [&] { return launch_causal(c->stream, a, s.head_dim, s.type == GE_TYPE_BF16, p.kinds); });
+    if (a.n_joins)
+        launch(c, "attention_join", [&] { return launch_causal_join(c->stream, a, s.head_dim, s.type == GE_TYPE_BF16); });
+    hip_check(hipStreamSynchronize(c->stream), "hipStreamSynchronize");
+}
+
+}  // namespace
+}  // namespace ge
+
+extern "C" {
+
+int ge_op_attention_causal(ge_ctx* c, const ge_attention_shape* shape, const void* q, const void* k, const void* v,
+                           const ge_attention_seq* seqs, int32_t n_seqs, void* out) {
+    return ge::guarded(c, [&] { ge::attend(c, shape, q, nullptr, nullptr, 0, k, v, seqs, n_seqs, out); });
+}
+
+int ge_op_attention_prefix(ge_ctx* c, const ge_attention_shape* shape, const void* q, const void* prefix_k,
+                           const void* prefix_v, int32_t prefix_len, const void* k, const void* v,
+                           const ge_attention_seq* seqs, int32_t n_seqs, void* out) {
+    return ge::guarded(c, [&] { ge::attend(c, shape, q, prefix_k, prefix_v, prefix_len, k, v, seqs, n_seqs, out); });
+}
+
+}  // extern "C"

@@ -1,0 +1,659 @@
+// Attention of causal models: packed prompts and cached keys, and a batch over a shared prefix
+// (gfx950). Every query row i of a sequence sees the keys j <= i + shift and, with a window,
+// j > i + shift - window:
+//   o_i = sum_j exp(scale q_i.k_j) v_j / sum_j exp(scale q_i.k_j),   0 where it sees no key.
+//
+// Rows. The G = heads / kv_heads query heads of a KV head score against the same keys, so the kernels
+// work on stacked rows: row r of a KV head is token r / G of the item's sequence, query head
+// kvh G + r % G. Of a batch over a shared prefix the rows of all its sequences stack up too.
+//
+// One wave holds 32 rows for the whole kernel and streams key blocks past them on
+// v_mfma_f32_32x32x16 (twice the rate of the 16x16x32 form here):
+//   S^T = K Q^T: A = 32 keys x 16 dims from LDS, B = the rows' fragments in registers. Lane l's 16
+//     accumulators are the keys 8 (e / 4) + 4 (l / 32) + e % 4 of row l % 32, so a row's softmax
+//     needs one exchange between two lanes.
+//   O^T += V^T P^T: the same accumulators, rounded to the inputs' type, are the B operand of the
+//     16-key steps when V^T's keys are taken in that order; V^T comes from V's rows in LDS by the
+//     transposing LDS read (4 keys x 16 dims a read of 16 lanes), so no transposed copy of V exists.
+// The running maximum moves only when a score passes it by 2^8 (in log2), as in attention.hip; P is
+// taken 2^6 higher, which uses fp16's range up to 2^14 and keeps keys of 2^-30 of the maximum.
+#include "causal.hpp"
+#include "common.hpp"
+
+namespace ge {
+namespace {
+
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+// The two input types: the matrix instruction, two floats rounded to nearest even and packed, and
+// the bits whose sum with a value's magnitude reaches its sign bit iff its exponent is all ones.
+struct F16 {
+    static __device__ __forceinline__ float16_t mfma(u32x4 a, u32x4 b, float16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        return __builtin_bit_cast(uint32_t, half2_t{_Float16(x), _Float16(y)});
+    }
+    static __device__ __forceinline__ float value(uint16_t x) { return h2f(x); }
+    static constexpr uint32_t kNonFinite = 0x04000400u;
+};
+struct BF16 {
+    static __device__ __forceinline__ float16_t mfma(u32x4 a, u32x4 b, float16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        return __builtin_bit_cast(uint32_t, bf16x2_t{__bf16(x), __bf16(y)});
+    }
+    static __device__ __forceinline__ float value(uint16_t x) { return __uint_as_float(uint32_t(x) << 16); }
+    static constexpr uint32_t kNonFinite = 0x00800080u;
+};
+
+constexpr float kRaise = 6.0f;       // P = 2^(score - maximum + kRaise)
+constexpr float kLazy = 8.0f;        // the maximum moves when a score passes it by this much (log2)
+constexpr int kNoWindow = -(1 << 30);
+
+// Max and sum over lanes l and l ^ 32 (the two halves of a row's keys).
+__device__ __forceinline__ float max_over_halves(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float sum_over_halves(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+__device__ __forceinline__ u32x2 lds_read_transposed(const unsigned char* p) {
+    return __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)p));
+}
+
+// A block of BK keys of one KV head in LDS: K, then V, each in 1 KB chunks of 8 keys x 64 dims (one
+// buffer_load ... lds each, eight whole 128-byte lines), chunk (panel, key / 8) at
+// (panel BK / 8 + key / 8) KB:
+//   K: key k's 16-byte piece c of the panel at 128 (k % 8) + 16 (c ^ (k / 2) % 8): the 16 keys a
+//     fragment read takes at a time fall on 16 different 16-byte columns of the 64 banks.
+//   V: 128-byte tiles of 4 keys x 16 dims, the source of one transposing read.
+template <int HD, int BK>
+struct KvBlock {
+    static constexpr int kBytes = BK * HD * 2, kChunks = kBytes / 1024;
+
+    // This lane's byte offsets into a chunk's rows of K and V. parity: of the chunk's key / 8.
+    static __device__ __forceinline__ uint32_t k_lane(int lane, int parity, uint32_t row_bytes) {
+        const int piece = (lane & 7) ^ (parity * 4 + (lane >> 4));
+        return uint32_t(lane >> 3) * row_bytes + uint32_t(piece * 16);
+    }
+    static __device__ __forceinline__ uint32_t v_lane(int lane, uint32_t row_bytes) {
+        const int tile = lane >> 3, key = (tile >> 2) * 4 + ((lane & 7) >> 1), dim = (tile & 3) * 16 + (lane & 1) * 8;
+        return uint32_t(key) * row_bytes + uint32_t(dim * 2);
+    }
+    // Chunk c of a block whose rows start at r's base; rows past r's size read as zeros.
+    static __device__ __forceinline__ void copy(__amdgpu_buffer_rsrc_t r, unsigned char* block, int c, uint32_t lane_off,
+                                                uint32_t row_bytes) {
+        const int panel = c / (BK / 8), k8 = c % (BK / 8);
+        lds_copy16(r, block + c * 1024, lane_off + uint32_t(k8 * 8) * row_bytes + uint32_t(panel * 128), 0);
+    }
+    // Rows [key, key + rows) of a tensor whose row 0 is at base, for the head at element offset `at`.
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const uint16_t* base, size_t key, int64_t stride, int at,
+                                                                     int rows) {
+        return buffer_rsrc(base + key * size_t(stride) + at, uint32_t((rows - 1) * stride + HD) * 2u);
+    }
+};
+
+// Waves that hold the same 32 rows, each with its share of the head's dims in its accumulators: at head
+// dim 512 the queries (128 registers) and all accumulators (256) do not fit beside the rest, so two
+// waves both compute the scores and take half of the product each.
+template <int HD>
+constexpr int kDimWaves = HD > 256 ? 2 : 1;
+// Fragments read ahead of their products (more spill at head dim 256).
+template <int HD>
+constexpr int kFragmentsAhead = HD > 128 ? 2 : 4;
+
+// 32 rows of one KV head: queries in registers, accumulators (of the dims' share `part`), running
+// maximum and sum.
+template <typename T, int HD>
+struct Rows {
+    static constexpr int KS = HD / 16, DT = HD / 32 / kDimWaves<HD>;
+    u32x4 q[KS];
+    float16_t o[DT];
+    float m, l;
+    int hi, lo;            // the last and first key this lane's row sees
+    int hi_all, hi_any;    // the last key the wave's first row sees (so all do), and its last row
+    int lo_all, lo_any;    // the first key the wave's last row sees (so all do), and its first row
+    int d0;                // the first 32-dim tile of this wave's accumulators
+
+    // Stacked rows [r0, r0 + n) of the item (n >= 1 rows of this wave; lanes past them repeat the last).
+    __device__ __forceinline__ void init(const CausalArgs& a, const CausalItem& it, int kvh, int r0, int n, int dims, int lane) {
+        const uint32_t r = uint32_t(r0) + uint32_t(min(lane & 31, n - 1)), g = uint32_t(a.group);
+        const uint32_t i = r / g, head = uint32_t(kvh) * g + r % g;
+        const uint16_t* p = a.q + (size_t(it.q_token) + i) * size_t(a.q_stride) + size_t(head) * HD + (lane >> 5) * 8;
+#pragma unroll
+        for (int s = 0; s < KS; s++) q[s] = *reinterpret_cast<const u32x4*>(p + s * 16) ^ a.q_flip;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] = float16_t{};
+        m = -INFINITY;
+        l = 0.0f;
+        d0 = dims * DT;
+        const int last = int(it.k_hi) - 1, first = a.window ? it.shift - a.window + 1 : kNoWindow;
+        const int i0 = int(uint32_t(r0) / g), i1 = int(uint32_t(r0 + n - 1) / g);
+        hi = min(int(i) + it.shift, last);
+        lo = int(i) + first;
+        hi_all = min(i0 + it.shift, last);
+        hi_any = min(i1 + it.shift, last);
+        lo_all = i1 + first;
+        lo_any = i0 + first;
+    }
+
+    // One block of BK keys from index kb on, in LDS at K and V.
+    template <int BK>
+    struct Block {
+        static constexpr int KT = BK / 32, kAhead = kFragmentsAhead<HD>;
+        float16_t s[KT];
+
+        __device__ __forceinline__ void scores(const Rows& w, const unsigned char* K, int lane) {
+            const int key = lane & 31, f = (key >> 1) & 7;
+            const unsigned char* at[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) at[c] = K + key * 128 + (((2 * c + (lane >> 5)) ^ f) * 16);
+            // fragments read kAhead steps before their product; the barriers keep the scheduler from
+            // reading all of them first, which spills
+            u32x4 ring[kAhead];
+            auto read = [&](int i) {
+                const int t = i / KS, k = i % KS;
+                ring[i % kAhead] = *reinterpret_cast<const u32x4*>(at[k & 3] + (k >> 2) * (BK * 128) + t * 4096);
+            };
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) read(i);
+#pragma unroll
+            for (int i = 0; i < KT * KS; i++) {
+                const int t = i / KS, k = i % KS;
+                if (k == 0) s[t] = float16_t{};
+                __builtin_amdgcn_sched_barrier(0);
+                s[t] = T::mfma(ring[i % kAhead], w.q[k], s[t]);
+                if (i + kAhead < KT * KS) read(i + kAhead);
+            }
+        }
+
+        __device__ __forceinline__ bool sees_all(const Rows& w, int kb) const {
+            return kb + BK - 1 <= w.hi_all && kb >= w.lo_all;
+        }
+
+        // Hidden keys to -inf, the running maximum, and P.
+        __device__ __forceinline__ void softmax(Rows& w, int kb, float c, int lane, u32x4 (&p)[2 * KT]) {
+            if (!sees_all(w, kb)) {
+                const int k0 = kb + (lane >> 5) * 4;
+#pragma unroll
+                for (int t = 0; t < KT; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int key = k0 + 32 * t + 8 * (e >> 2) + (e & 3);
+                        s[t][e] = key <= w.hi && key >= w.lo ? s[t][e] : -INFINITY;
+                    }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) top = fmaxf(top, s[t][e]);
+            if (__builtin_amdgcn_ballot_w64(top * c > w.m + kLazy)) {
+                // a row's own scores decide, so its bits do not depend on the wave's other rows
+                const float block = max_over_halves(top) * c, m_new = block > w.m + kLazy ? block : w.m;
+                const float fade = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w.m - m_new);
+                w.l *= fade;
+#pragma unroll
+                for (int d = 0; d < DT; d++) w.o[d] *= fade;
+                w.m = m_new;
+            }
+            const float ref = w.m == -INFINITY ? 0.0f : kRaise - w.m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], c, ref));
+                    sum += s[t][e];
+                }
+            w.l += sum;
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) p[2 * t + e / 8][(e % 8) / 2] = T::pack(s[t][e], s[t][e + 1]);
+        }
+
+        // V^T's fragment of 32 dims d and 16 keys t: keys 16 t + 8 j + 4 (lane / 32) + [0, 4) at slots 4 j.
+        static __device__ __forceinline__ u32x4 v_fragment(const unsigned char* V, int d, int t) {
+            const unsigned char* p = V + ((d >> 1) * (BK / 8) + 2 * t) * 1024 + (d & 1) * 256;
+            const u32x2 a = lds_read_transposed(p), b = lds_read_transposed(p + 1024);
+            return u32x4{a[0], a[1], b[0], b[1]};
+        }
+
+        __device__ __forceinline__ void product(Rows& w, const unsigned char* V, int lane, const u32x4 (&p)[2 * KT]) {
+            const unsigned char* vl = V + (w.d0 >> 1) * (BK / 8) * 1024 + (lane >> 5) * 512 + ((lane >> 4) & 1) * 128 + (lane & 15) * 8;
+            u32x4 ring[kAhead];
+            auto read = [&](int i) { ring[i % kAhead] = v_fragment(vl, i % DT, i / DT); };
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) read(i);
+#pragma unroll
+            for (int i = 0; i < 2 * KT * DT; i++) {
+                __builtin_amdgcn_sched_barrier(0);
+                w.o[i % DT] = T::mfma(ring[i % kAhead], p[i / DT], w.o[i % DT]);
+                if (i + kAhead < 2 * KT * DT) read(i + kAhead);
+            }
+        }
+    };
+
+    // Rows to out, or as unnormalised fp32 with their maximum and sum to the partial rows.
+    __device__ __forceinline__ void finish(const CausalArgs& a, const CausalItem& it, int kvh, int r0, int n, int lane) {
+        const int row = lane & 31, half = lane >> 5;
+        if (row >= n) return;
+        if (it.part == kDirect) {
+            const uint32_t r = uint32_t(r0 + row), g = uint32_t(a.group);
+            uint16_t* p = a.out + (size_t(it.q_token) + r / g) * size_t(a.out_stride) +
+                          (size_t(kvh) * g + r % g) * HD + d0 * 32 + half * 4;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<u32x2*>(p + 32 * d + 2 * e) =
+                        u32x2{T::pack(o[d][e] * inv, o[d][e + 1] * inv), T::pack(o[d][e + 2] * inv, o[d][e + 3] * inv)};
+        } else {
+            const size_t at = size_t(kvh) * a.part_rows + it.part + uint32_t(r0 - int(it.row0) + row);
+            float* p = a.part_o + at * HD + d0 * 32 + half * 4;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<float4_t*>(p + 32 * d + 2 * e) = float4_t{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+            if (half == 0 && d0 == 0) a.part_ml[at] = float2{m, l};
+        }
+    }
+};
+
+// A hidden key's P is 0, which its V, where that is infinite or NaN, would still turn into NaN. Only blocks
+// of which some of the item's rows see a key that others do not can hold such a key. Their V is cleared of
+// such values by the wave that copied them, before anyone reads it; if there were any, they are added at
+// the end to the stored results of the rows that see them, where inf + -inf and NaN come out as in the sum.
+template <typename T, int HD>
+struct HeldBack {
+    int hi_all, hi_any, lo_all, lo_any;  // last and first key that all and that any of the item's rows see
+    bool any;
+
+    __device__ __forceinline__ void init(const CausalArgs& a, const CausalItem& it) {
+        const uint32_t g = uint32_t(a.group);
+        const int i0 = int(it.row0 / g), i1 = int((it.row0 + it.n_rows - 1) / g), last = int(it.k_hi) - 1;
+        hi_all = min(i0 + it.shift, last);
+        hi_any = min(i1 + it.shift, last);
+        const int first = a.window ? it.shift - a.window + 1 : kNoWindow;
+        lo_all = i1 + first;
+        lo_any = i0 + first;
+        any = false;
+    }
+    __device__ __forceinline__ bool mixed(int kb, int bk) const {
+        return (kb + bk - 1 > hi_all && hi_all < hi_any) || (kb < lo_all && lo_any < lo_all);
+    }
+    // This lane's 16 bytes of a landed copy.
+    __device__ __forceinline__ void clear(unsigned char* p) {
+        u32x4 f = *reinterpret_cast<const u32x4*>(p);
+        uint32_t bad = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t t = ((f[j] & 0x7fff7fffu) + T::kNonFinite) & 0x80008000u;
+            f[j] &= ~((t >> 15) * 0xffffu);
+            bad |= t;
+        }
+        if (bad) *reinterpret_cast<u32x4*>(p) = f;
+        any = any || __builtin_amdgcn_ballot_w64(bad != 0);
+    }
+    // Every wave of the workgroup: whether any of them held something back. Uses LDS that no one reads
+    // any more.
+    __device__ __forceinline__ void share(unsigned char* lds) {
+        __syncthreads();
+        int* const flag = reinterpret_cast<int*>(lds);
+        if ((threadIdx.x & 63) == 0) flag[threadIdx.x >> 6] = any;
+        __syncthreads();
+        any = (flag[0] | flag[1] | flag[2] | flag[3]) != 0;
+    }
+    // Rows [r0, r0 + n), dims [d0, d0 + dims), which this wave has stored.
+    __device__ __forceinline__ static void add(const CausalArgs& a, const CausalItem& it, int kvh, int r0, int n, int d0, int dims) {
+        __threadfence();
+        const uint16_t* const v = (it.source ? a.prefix_v : a.v) + size_t(kvh) * HD;
+        const uint32_t g = uint32_t(a.group);
+        for (uint32_t key = it.k_lo; key < it.k_hi; key++)
+            for (int d = d0 + int(threadIdx.x & 63); d < d0 + dims; d += 64) {
+                const uint16_t x = v[(size_t(it.key0) + key) * size_t(a.v_stride) + d];
+                if (((x & 0x7fffu) + (T::kNonFinite & 0xffffu)) < 0x8000u) continue;
+                for (int row = 0; row < n; row++) {
+                    const uint32_t r = uint32_t(r0 + row);
+                    const int i = int(r / g);
+                    if (int(key) > i + it.shift || (a.window && int(key) <= i + it.shift - a.window)) continue;
+                    if (it.part == kDirect) {
+                        uint16_t* o = a.out + (size_t(it.q_token) + r / g) * size_t(a.out_stride) + (size_t(kvh) * g + r % g) * HD + d;
+                        *o = uint16_t(T::pack(T::value(*o) + T::value(x), 0.0f));
+                    } else {
+                        a.part_o[(size_t(kvh) * a.part_rows + it.part + (r - it.row0)) * HD + d] += T::value(x);
+                    }
+                }
+            }
+    }
+};
+
+// ---------------------------------------------------------------------------- many rows: waves over rows
+
+// 128 rows, 32 a wave (64 at head dim 512); the workgroup's waves copy each key block together, two
+// blocks in LDS.
+template <typename T, int HD>
+struct Wide {
+    static constexpr int NW = 4, BK = HD <= 128 ? 64 : 32;
+    static_assert(NW / kDimWaves<HD> * 32 == causal_wide_rows(HD), "rows of a wide item");
+    using Kv = KvBlock<HD, BK>;
+    static constexpr int kLds = 2 * 2 * Kv::kBytes;
+
+    static __device__ __forceinline__ void run(const CausalArgs& a, const CausalItem& it, int kvh, unsigned char* lds) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+        const uint16_t* const kp = it.source ? a.prefix_k : a.k;
+        const uint16_t* const vp = it.source ? a.prefix_v : a.v;
+        const uint32_t kb_bytes = uint32_t(a.k_stride) * 2, vb_bytes = uint32_t(a.v_stride) * 2;
+        static_assert(Kv::kChunks % NW == 0 && (BK / 8) % NW == 0 && NW % 2 == 0, "every wave copies chunks of one key parity");
+        const uint32_t k_off = Kv::k_lane(lane, wave & 1, kb_bytes), v_off = Kv::v_lane(lane, vb_bytes);
+        const int k_lo = int(it.k_lo), k_hi = int(it.k_hi);
+        const int blocks = (k_hi - k_lo + BK - 1) / BK;
+        auto issue = [&](int b) {
+            const int kb = k_lo + b * BK, rows = min(BK, k_hi - kb);
+            unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
+            const auto kr = Kv::rows_of(kp, size_t(it.key0) + kb, a.k_stride, kvh * HD, rows);
+            const auto vr = Kv::rows_of(vp, size_t(it.key0) + kb, a.v_stride, kvh * HD, rows);
+#pragma unroll
+            for (int i = 0; i < Kv::kChunks / NW; i++) Kv::copy(kr, at, wave + i * NW, k_off, kb_bytes);
+#pragma unroll
+            for (int i = 0; i < Kv::kChunks / NW; i++) Kv::copy(vr, at + Kv::kBytes, wave + i * NW, v_off, vb_bytes);
+        };
+        constexpr int DW = kDimWaves<HD>;
+        const int r0 = int(it.row0) + wave / DW * 32, n = min(32, int(it.n_rows) - wave / DW * 32);
+        Rows<T, HD> w;
+        HeldBack<T, HD> held;
+        held.init(a, it);
+        if (blocks > 0) issue(0);
+        if (n > 0) w.init(a, it, kvh, r0, n, wave % DW, lane);
+        for (int b = 0; b < blocks; b++) {
+            const int kb = k_lo + b * BK;
+            wait_vmcnt<0>();
+            if (held.mixed(kb, BK)) {
+                unsigned char* const at = lds + ((b & 1) * 2 + 1) * Kv::kBytes;
+#pragma unroll
+                for (int i = 0; i < Kv::kChunks / NW; i++) held.clear(at + (wave + i * NW) * 1024 + lane * 16);
+            }
+            wait_lgkmcnt0();
+            workgroup_barrier();
+            if (b + 1 < blocks) issue(b + 1);
+            if (n > 0 && kb <= w.hi_any && kb + BK - 1 >= w.lo_any) {
+                const unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
+                typename Rows<T, HD>::template Block<BK> blk;
+                u32x4 p[BK / 16];
+                blk.scores(w, at, lane);
+                blk.softmax(w, kb, a.c, lane, p);
+                blk.product(w, at + Kv::kBytes, lane, p);
+            }
+        }
+        if (n > 0) {
+            w.l = sum_over_halves(w.l);
+            w.finish(a, it, kvh, r0, n, lane);
+        }
+        held.share(lds);
+        if (n > 0 && held.any) held.add(a, it, kvh, r0, n, w.d0 * 32, w.DT * 32);
+    }
+};
+
+// ---------------------------------------------------------------------------- few rows: waves over keys
+
+// 32 rows; the waves (at head dim 512 the pairs of waves that share the dims) take the key blocks in
+// turn, each through LDS of its own, and join at the end. A wave alone on its LDS waits for its own copies
+// only; a pair meets at the workgroup's barriers.
+template <typename T, int HD>
+struct Narrow {
+    static constexpr int DW = kDimWaves<HD>, KW = 4 / DW, BK = 32;
+    using Kv = KvBlock<HD, BK>;
+    static constexpr int kChunks = Kv::kChunks / DW;  // a wave's copies of K, and of V
+    static constexpr int kPerKw = 2 * Kv::kBytes, kAcc = Rows<T, HD>::DT * 16;
+    static constexpr int kJoin = 4 * 64 * (kAcc + 2) * 4;
+    static constexpr int kLds = KW * kPerKw > kJoin ? KW * kPerKw : kJoin;
+
+    static __device__ __forceinline__ void meet() {
+        wait_lgkmcnt0();
+        if (DW > 1)
+            workgroup_barrier();
+        else
+            asm volatile("" ::: "memory");
+    }
+
+    static __device__ __forceinline__ void run(const CausalArgs& a, const CausalItem& it, int kvh, unsigned char* lds) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+        const int kw = wave / DW, dims = wave % DW;
+        const uint16_t* const kp = it.source ? a.prefix_k : a.k;
+        const uint16_t* const vp = it.source ? a.prefix_v : a.v;
+        const uint32_t kb_bytes = uint32_t(a.k_stride) * 2, vb_bytes = uint32_t(a.v_stride) * 2;
+        const uint32_t k_even = Kv::k_lane(lane, 0, kb_bytes), k_odd = Kv::k_lane(lane, 1, kb_bytes);
+        const uint32_t v_off = Kv::v_lane(lane, vb_bytes);
+        const int k_lo = int(it.k_lo), k_hi = int(it.k_hi);
+        const int blocks = (k_hi - k_lo + BK - 1) / BK;
+        unsigned char* const K = lds + kw * kPerKw;
+        unsigned char* const V = K + Kv::kBytes;
+        auto issue_k = [&](int b) {
+            const int kb = k_lo + b * BK;
+            const auto r = Kv::rows_of(kp, size_t(it.key0) + kb, a.k_stride, kvh * HD, min(BK, k_hi - kb));
+#pragma unroll
+            for (int i = 0; i < kChunks; i++) Kv::copy(r, K, dims * kChunks + i, i & 1 ? k_odd : k_even, kb_bytes);
+        };
+        auto issue_v = [&](int b) {
+            const int kb = k_lo + b * BK;
+            const auto r = Kv::rows_of(vp, size_t(it.key0) + kb, a.v_stride, kvh * HD, min(BK, k_hi - kb));
+#pragma unroll
+            for (int i = 0; i < kChunks; i++) Kv::copy(r, V, dims * kChunks + i, v_off, vb_bytes);
+        };
+        const int r0 = int(it.row0), n = int(it.n_rows);
+        Rows<T, HD> w;
+        HeldBack<T, HD> held;
+        held.init(a, it);
+        if (kw < blocks) {
+            issue_k(kw);
+            issue_v(kw);
+        }
+        w.init(a, it, kvh, r0, n, dims, lane);
+        // Waves alone on their LDS leave when their blocks are done; pairs keep meeting until all are.
+        for (int b = kw; b - kw < blocks; b += KW) {
+            const int kb = k_lo + b * BK;
+            const bool mine = b < blocks, more = b + KW < blocks;
+            if (DW == 1 && !mine) break;
+            typename Rows<T, HD>::template Block<BK> blk;
+            u32x4 p[BK / 16];
+            wait_vmcnt<kChunks>();  // all but V's copies
+            meet();
+            if (mine) blk.scores(w, K, lane);
+            meet();  // K's reads have returned before its next block is copied over it
+            if (more) issue_k(b + KW);
+            if (mine) blk.softmax(w, kb, a.c, lane, p);
+            if (more)
+                wait_vmcnt<kChunks>();  // all but the next K's
+            else
+                wait_vmcnt<0>();
+            if (mine && held.mixed(kb, BK)) {
+#pragma unroll
+                for (int i = 0; i < kChunks; i++) held.clear(V + (dims * kChunks + i) * 1024 + lane * 16);
+            }
+            meet();
+            if (mine) blk.product(w, V, lane, p);
+            meet();
+            if (more) issue_v(b + KW);
+        }
+        w.l = sum_over_halves(w.l);
+        held.share(lds);
+        // Join: every wave leaves its maximum, sum and accumulators in LDS, the first of each share of the
+        // dims adds them in order.
+        __syncthreads();
+        float* const j = reinterpret_cast<float*>(lds);
+        if (kw > 0) {
+            float* const p = j + (wave * (kAcc + 2)) * 64 + lane;
+            p[0] = w.m;
+            p[64] = w.l;
+#pragma unroll
+            for (int d = 0; d < Rows<T, HD>::DT; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) p[(2 + d * 16 + e) * 64] = w.o[d][e];
+        }
+        __syncthreads();
+        if (kw > 0) return;
+        float top = w.m;
+#pragma unroll
+        for (int k = 1; k < KW; k++) top = fmaxf(top, j[(k * DW + dims) * (kAcc + 2) * 64 + lane]);
+        const float f0 = w.m == top ? 1.0f : __builtin_amdgcn_exp2f(w.m - top);
+        w.l *= f0;
+#pragma unroll
+        for (int d = 0; d < Rows<T, HD>::DT; d++) w.o[d] *= f0;
+        for (int k = 1; k < KW; k++) {
+            const float* const p = j + (k * DW + dims) * (kAcc + 2) * 64 + lane;
+            const float mk = p[0], f = mk == top ? 1.0f : __builtin_amdgcn_exp2f(mk - top);
+            w.l += p[64] * f;
+#pragma unroll
+            for (int d = 0; d < Rows<T, HD>::DT; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) w.o[d][e] += p[(2 + d * 16 + e) * 64] * f;
+        }
+        w.m = top;
+        w.finish(a, it, kvh, r0, n, lane);
+        if (held.any) held.add(a, it, kvh, r0, n, w.d0 * 32, w.DT * 32);
+    }
+};
+
+// KINDS: the items of the launch: 1 wide, 2 narrow, 3 both.
+template <typename T, int HD, int KINDS>
+constexpr int causal_lds() {
+    const int w = KINDS & 1 ? Wide<T, HD>::kLds : 0, n = KINDS & 2 ? Narrow<T, HD>::kLds : 0;
+    return w > n ? w : n;
+}
+
+template <typename T, int HD, int KINDS>
+__global__ __launch_bounds__(256, HD <= 256 ? 2 : 1) void causal_kernel(const CausalArgs a) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char causal_lds_mem[];
+    // Workgroups go to the 8 XCDs in turn: with the KV head fastest, a head's items share an L2.
+    const uint32_t at = blockIdx.x / uint32_t(a.kv_heads);
+    const int kvh = int(blockIdx.x % uint32_t(a.kv_heads));
+    const CausalItem it = a.items[at];
+    if (KINDS == 1 || (KINDS == 3 && !it.narrow))
+        Wide<T, HD>::run(a, it, kvh, causal_lds_mem);
+    else
+        Narrow<T, HD>::run(a, it, kvh, causal_lds_mem);
+}
+
+// ---------------------------------------------------------------------------- joining the parts
+
+// One wave a row: the parts' maxima and sums, then their rows weighted and added in order.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void causal_join_kernel(const CausalArgs a) {
+    constexpr int E = HD / 64;
+    const int lane = threadIdx.x & 63;
+    const uint32_t at = blockIdx.x / uint32_t(a.kv_heads), kvh = blockIdx.x % uint32_t(a.kv_heads), g = uint32_t(a.group);
+    const CausalJoin jn = a.joins[at];
+    for (uint32_t row = threadIdx.x >> 6; row < jn.n_rows; row += 4) {
+        const size_t base = size_t(kvh) * a.part_rows + row;
+        const uint32_t parts = jn.splits[0] + jn.splits[1];
+        auto place = [&](uint32_t s) {
+            const int side = s < jn.splits[0] ? 0 : 1;
+            return base + jn.part[side] + size_t(side ? s - jn.splits[0] : s) * jn.stride[side];
+        };
+        float top = -INFINITY;
+        for (uint32_t s = 0; s < parts; s++) top = fmaxf(top, a.part_ml[place(s)].x);
+        float sum = 0.0f, o[E] = {};
+        for (uint32_t s = 0; s < parts; s++) {
+            const size_t p = place(s);
+            const float2 ml = a.part_ml[p];
+            if (ml.y == 0.0f) continue;  // it saw no key
+            const float f = ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
+            sum += ml.y * f;
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] += a.part_o[p * HD + lane * E + e] * f;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const uint32_t r = jn.row0 + row;
+        uint16_t* out = a.out + (size_t(jn.q_token) + r / g) * size_t(a.out_stride) + (size_t(kvh) * g + r % g) * HD + lane * E;
+        if constexpr (E == 1) {
+            *out = uint16_t(T::pack(o[0] * inv, 0.0f));
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = T::pack(o[e] * inv, o[e + 1] * inv);
+        }
+    }
+}
+
+template <typename T, int HD, int KINDS>
+hipError_t run_items(hipStream_t s, const CausalArgs& a) {
+    launch_kernel(causal_kernel<T, HD, KINDS>, dim3(uint32_t(a.n_items) * uint32_t(a.kv_heads)), dim3(256), uint32_t(causal_lds<T, HD, KINDS>()), s, a);
+    return hipGetLastError();
+}
+
+template <typename T, int HD>
+hipError_t run_kinds(hipStream_t s, const CausalArgs& a, int kinds) {
+    return kinds == 1 ? run_items<T, HD, 1>(s, a) : kinds == 2 ? run_items<T, HD, 2>(s, a) : run_items<T, HD, 3>(s, a);
+}
+
+template <typename T, int HD>
+hipError_t run_join(hipStream_t s, const CausalArgs& a) {
+    launch_kernel(causal_join_kernel<T, HD>, dim3(uint32_t(a.n_joins) * uint32_t(a.kv_heads)), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+template <typename T, int HD>
+hipError_t configure_hd() {
+    const void* const f[3] = {reinterpret_cast<const void*>(causal_kernel<T, HD, 1>), reinterpret_cast<const void*>(causal_kernel<T, HD, 2>),
+                              reinterpret_cast<const void*>(causal_kernel<T, HD, 3>)};
+    const int lds[3] = {causal_lds<T, HD, 1>(), causal_lds<T, HD, 2>(), causal_lds<T, HD, 3>()};
+    static_assert(causal_lds<T, HD, 3>() <= 160 * 1024, "LDS of a CU");
+    for (int i = 0; i < 3; i++) {
+        const hipError_t e = hipFuncSetAttribute(f[i], hipFuncAttributeMaxDynamicSharedMemorySize, lds[i]);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+bool args_ok(const CausalArgs& a, int hd) {
+    return causal_head_dim_ok(hd) && a.kv_heads > 0 && a.group > 0 && a.n_items >= 0 && a.n_joins >= 0 &&
+           uint64_t(a.n_items) * uint64_t(a.kv_heads) <= kCausalMaxGroups && uint64_t(a.n_joins) * uint64_t(a.kv_heads) <= kCausalMaxGroups;
+}
+
+}  // namespace
+
+bool causal_head_dim_ok(int hd) { return hd == 64 || hd == 128 || hd == 256 || hd == 512; }
+
+hipError_t launch_causal(hipStream_t s, const CausalArgs& a, int hd, bool bf16, int kinds) {
+    if (!args_ok(a, hd) || kinds < 1 || kinds > 3) return hipErrorInvalidValue;
+    if (a.n_items == 0) return hipSuccess;
+    switch (hd) {
+        case 64: return bf16 ? run_kinds<BF16, 64>(s, a, kinds) : run_kinds<F16, 64>(s, a, kinds);
+        case 128: return bf16 ? run_kinds<BF16, 128>(s, a, kinds) : run_kinds<F16, 128>(s, a, kinds);
+        case 256: return bf16 ? run_kinds<BF16, 256>(s, a, kinds) : run_kinds<F16, 256>(s, a, kinds);
+        default: return bf16 ? run_kinds<BF16, 512>(s, a, kinds) : run_kinds<F16, 512>(s, a, kinds);
+    }
+}
+
+hipError_t launch_causal_join(hipStream_t s, const CausalArgs& a, int hd, bool bf16) {
+    if (!args_ok(a, hd)) return hipErrorInvalidValue;
+    if (a.n_joins == 0) return hipSuccess;
+    switch (hd) {
+        case 64: return bf16 ? run_join<BF16, 64>(s, a) : run_join<F16, 64>(s, a);
+        case 128: return bf16 ? run_join<BF16, 128>(s, a) : run_join<F16, 128>(s, a);
+        case 256: return bf16 ? run_join<BF16, 256>(s, a) : run_join<F16, 256>(s, a);
+        default: return bf16 ? run_join<BF16, 512>(s, a) : run_join<F16, 512>(s, a);
+    }
+}
+
+hipError_t causal_configure() {
+    const hipError_t e[8] = {configure_hd<F16, 64>(),  configure_hd<BF16, 64>(),  configure_hd<F16, 128>(), configure_hd<BF16, 128>(),
+                             configure_hd<F16, 256>(), configure_hd<BF16, 256>(), configure_hd<F16, 512>(), configure_hd<BF16, 512>()};
+    for (const hipError_t x : e)
+        if (x != hipSuccess) return x;
+    return hipSuccess;
+}
+
+}  // namespace ge

@@ -1,0 +1,58 @@
+// Attention of causal models (causal.hip): the items the host plans (causal.cpp) and the kernels take.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace ge {
+
+// Stacked rows of a wide item: 32 a wave, or a pair of waves at head dim 512.
+constexpr int causal_wide_rows(int hd) { return hd > 256 ? 64 : 128; }
+constexpr int kCausalNarrowRows = 32;  // of a narrow item, whose waves split the keys
+constexpr uint32_t kDirect = 0xffffffffu;
+// Workgroups of a launch: HIP's grid counts work-items in 32 bits.
+constexpr uint64_t kCausalMaxGroups = (uint64_t(1) << 32) / 256 - 1;
+
+// Stacked rows [row0, row0 + n_rows) (token row / group from q_token on) against the keys
+// [k_lo, k_hi) of the rows that start at key0 of k and v (of the prefix's where source is 1). Row
+// token i sees key j iff j <= i + shift and, with a window, j > i + shift - window.
+struct CausalItem {
+    uint32_t q_token, row0, n_rows;
+    uint32_t key0, k_lo, k_hi;
+    int32_t shift;
+    uint32_t part;  // kDirect: the rows go to out; else to the partial rows from here on
+    uint32_t source, narrow;
+};
+
+// Rows [row0, row0 + n_rows) of q_token's sequence joined from splits[0] parts at partial rows
+// part[0] + s stride[0] and splits[1] parts at part[1] + s stride[1].
+struct CausalJoin {
+    uint32_t q_token, row0, n_rows;
+    uint32_t part[2], stride[2], splits[2];
+};
+
+struct CausalArgs {
+    const uint16_t *q, *k, *v, *prefix_k, *prefix_v;
+    uint16_t* out;
+    const CausalItem* items;
+    const CausalJoin* joins;
+    float* part_o;    // fp32 [kv_heads][part_rows][head_dim], unnormalised
+    float2* part_ml;  // [kv_heads][part_rows]: running maximum (log2) and sum
+    int64_t q_stride, k_stride, v_stride, out_stride;  // elements from one row to the next
+    size_t part_rows;
+    int n_items, n_joins;
+    int group, kv_heads, window;  // window 0: none
+    float c;                      // |scale| log2(e)
+    uint32_t q_flip;              // the sign bits of two values where the scale is negative
+};
+
+// Head dims 64, 128, 256 and 512.
+bool causal_head_dim_ok(int hd);
+// kinds: 1 wide items only, 2 narrow only, 3 both.
+hipError_t launch_causal(hipStream_t s, const CausalArgs& a, int hd, bool bf16, int kinds);
+hipError_t launch_causal_join(hipStream_t s, const CausalArgs& a, int hd, bool bf16);
+// Dynamic LDS limits; once per device.
+hipError_t causal_configure();
+
+}  // namespace ge

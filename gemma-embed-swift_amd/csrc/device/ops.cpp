@@ -42,6 +42,18 @@ unsigned char* OpTemps::base() {
     return static_cast<unsigned char*>(c_->op_buf);
 }
 
+unsigned char* op_lists(ge_ctx* c, size_t bytes) {
+    if (bytes > c->op_host_cap) {
+        if (c->op_host) hip_check(hipHostFree(c->op_host), "hipHostFree");
+        c->op_host = nullptr;
+        c->op_host_cap = 0;
+        const size_t cap = std::max<size_t>(2 * bytes, 64 << 10);
+        hip_check(hipHostMalloc(&c->op_host, cap, hipHostMallocDefault), "hipHostMalloc");
+        c->op_host_cap = cap;
+    }
+    return static_cast<unsigned char*>(c->op_host);
+}
+
 OpTemps::~OpTemps() {
     // A call that fails after its first launch has not waited for it; the next call's constants are
     // written by the host, in no order with the stream.

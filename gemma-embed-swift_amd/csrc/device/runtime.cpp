@@ -1599,6 +1599,7 @@ void ge_destroy(ge_ctx* c) {
     ge::free_vision(c);
     if (c->vec_buf) (void)hipFree(c->vec_buf);
     if (c->op_buf) (void)hipFree(c->op_buf);
+    if (c->op_host) (void)hipHostFree(c->op_host);
     for (auto& p : c->prof_pending) {
         (void)hipEventDestroy(p.a);
         (void)hipEventDestroy(p.b);

@@ -210,6 +210,9 @@ struct ge_ctx {
     // kOpTempsKept bytes.
     void* op_buf = nullptr;
     size_t op_cap = 0;
+    // Pinned memory of one per-op call's work lists (op_lists), which its kernels read in place.
+    void* op_host = nullptr;
+    size_t op_host_cap = 0;
 };
 
 namespace ge {
@@ -262,6 +265,11 @@ private:
     size_t used_ = 0;
     const int unwinding_ = std::uncaught_exceptions();
 };
+// At least `bytes` of the context's pinned memory, for work lists written by the host and read by the
+// call's kernels where they are: a list is read once, by one lane of a workgroup, and a copy to device
+// memory would be one more operation ahead of the kernel. The same rules as OpTemps make it free again
+// when the call returns.
+unsigned char* op_lists(ge_ctx* c, size_t bytes);
 hipEvent_t take_event(ge_ctx* c);
 
 // Runs one launch. When profiling covers `name`, the kernel's dispatch records a start and a

@@ -62,6 +62,16 @@ class ge_embed_options(C.Structure):
                 ("batch_size", C.c_int32)]
 
 
+class ge_attention_shape(C.Structure):
+    _fields_ = [("type", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("q_rows", C.c_int32), ("kv_rows", C.c_int32), ("window", C.c_int32), ("scale", C.c_float),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("out_stride", C.c_int64)]
+
+
+class ge_attention_seq(C.Structure):
+    _fields_ = [("q_start", C.c_uint32), ("q_len", C.c_uint32), ("kv_start", C.c_uint32), ("kv_len", C.c_uint32)]
+
+
 class ge_tensor_desc(C.Structure):
     _fields_ = [("name", C.c_char_p), ("offset", C.c_uint64), ("type", C.c_int32), ("ndim", C.c_int32),
                 ("shape", C.c_int64 * 4)]
@@ -151,6 +161,8 @@ SIGNATURES = {
     "ge_op_mean_pool": (_I, [_P, _P, C.c_int32, C.c_int32, _P, C.c_int32, _P]),
     "ge_op_attention_split": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                    C.c_int32, C.c_float]),
+    "ge_op_attention_causal": (_I, [_P, C.POINTER(ge_attention_shape), _P, _P, _P, _P, C.c_int32, _P]),
+    "ge_op_attention_prefix": (_I, [_P, C.POINTER(ge_attention_shape), _P, _P, _P, C.c_int32, _P, _P, _P, C.c_int32, _P]),
     "ge_model_load": (_I, [C.c_char_p, C.POINTER(ge_load_options), C.POINTER(_P), C.c_char_p, C.c_size_t]),
     "ge_gguf_open": (_I, [C.c_char_p, C.POINTER(_P), C.c_char_p, C.c_size_t]),
     "ge_gguf_close": (None, [_P]),
@@ -632,6 +644,38 @@ class Context:
                                               C.c_void_p(k_lo), C.c_void_p(v), C.c_void_p(out), C.c_void_p(work),
                                               n_work, heads, kv_heads, head_dim, half_window, scale),
                     "ge_op_attention_split")
+
+    # ---- attention of causal models (shape from attention_shape, seqs from attention_seqs)
+    def attention_causal(self, shape: "ge_attention_shape", q: int, k: int, v: int, seqs: np.ndarray, out: int):
+        """ge_op_attention_causal: packed prompts, chunks and single tokens over cached keys."""
+        s = attention_seqs(seqs)
+        self._check(lib.ge_op_attention_causal(self.handle, C.byref(shape), q, k, v, s.ctypes.data, len(s), out),
+                    "ge_op_attention_causal")
+
+    def attention_prefix(self, shape: "ge_attention_shape", q: int, prefix_k: int, prefix_v: int, prefix_len: int, k: int,
+                         v: int, seqs: np.ndarray, out: int):
+        """ge_op_attention_prefix: every sequence's keys are the shared prefix's rows, then its own."""
+        s = attention_seqs(seqs)
+        self._check(lib.ge_op_attention_prefix(self.handle, C.byref(shape), q, prefix_k, prefix_v, prefix_len, k, v,
+                                               s.ctypes.data, len(s), out), "ge_op_attention_prefix")
+
+
+def attention_shape(type: int, heads: int, kv_heads: int, head_dim: int, q_rows: int, kv_rows: int, scale: float = 1.0,
+                    window: int = 0, q_stride: int = 0, k_stride: int = 0, v_stride: int = 0,
+                    out_stride: int = 0) -> "ge_attention_shape":
+    """Operands of attention_causal and attention_prefix (type: GE_TYPE_F16 or GE_TYPE_BF16)."""
+    return ge_attention_shape(type, heads, kv_heads, head_dim, q_rows, kv_rows, window, scale, q_stride, k_stride, v_stride,
+                              out_stride)
+
+
+def attention_seqs(sequences) -> np.ndarray:
+    """(q_start, q_len, kv_start, kv_len) of each sequence as a (n, 4) uint32 array."""
+    s = np.asarray(sequences)
+    if s.dtype != np.uint32:
+        if s.size and (s.min() < 0 or s.max() > 0xffffffff):
+            raise OverflowError("a sequence's rows are counted in 32 bits")
+        s = s.astype(np.uint32)
+    return np.ascontiguousarray(s.reshape(-1, 4))
 
 
 def attention_work(sequences_ranges, queries: Optional[int] = None) -> np.ndarray:

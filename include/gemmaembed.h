@@ -252,6 +252,52 @@ int ge_op_attention_split(ge_ctx* ctx, const void* q, const void* q_lo, const vo
                           void* out, const void* work, int32_t n_work, int32_t heads, int32_t kv_heads, int32_t head_dim,
                           int32_t half_window, float scale);
 
+/* ---- attention of causal models: packed prompts and cached keys, and a batch over a shared prefix. No
+ * counterpart in the reference, whose encoder sees every token both ways; for decoder-style embedding
+ * and scoring models on the same context. Like the other per-op entries they take device memory, run on
+ * the context's stream and return when their results are there; what they read must be complete when
+ * they are called. The sequence list is host memory.
+ *
+ * Operands: rows of heads, a token's heads back to back. q and out have q_rows rows of
+ * heads x head_dim, k and v kv_rows rows of kv_heads x head_dim (query head h reads KV head
+ * h / (heads / kv_heads)); a stride is the elements from one row to the next (0: rows back to back), so q, k
+ * and v may be views of one projection's output. All are of one type, GE_TYPE_F16 or GE_TYPE_BF16. out
+ * overlaps none of the inputs.
+ * Limits: heads a multiple of kv_heads, up to 4096; head_dim 64, 128, 256 or 512; buffers 16-byte aligned;
+ * strides a multiple of 8 up to 2^24; rows, window and prefix under 2^30. Scores, softmax and sums are in
+ * fp32; the softmax weights are rounded to the operands' type before the product with V. */
+typedef struct ge_attention_shape {
+    int32_t type;
+    int32_t heads, kv_heads, head_dim;
+    int32_t q_rows, kv_rows;
+    int32_t window; /* keys a query sees up to and including its own position; 0 = all */
+    float scale;    /* multiplies the scores */
+    int64_t q_stride, k_stride, v_stride, out_stride;
+} ge_attention_shape;
+
+/* One sequence of a call: its query rows [q_start, q_start + q_len) and its key rows [kv_start,
+ * kv_start + kv_len). Query rows of a call ascend and do not overlap; key rows may lie anywhere, and
+ * sequences may share them. */
+typedef struct ge_attention_seq {
+    uint32_t q_start, q_len, kv_start, kv_len;
+} ge_attention_seq;
+
+/* out_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys j that query i of its sequence sees, with the last
+ * query at the last key: j <= i + kv_len - q_len and, with a window, j > i + kv_len - q_len - window. So
+ * q_len = kv_len is a prompt, a shorter q_len a chunk or (1) the next token over cached keys. A query
+ * that sees no key gets zeros. A key no query of a row sees (its score or value infinite or NaN,
+ * say) does not reach that row. Rows of out outside the sequences stay as they were. */
+int ge_op_attention_causal(ge_ctx* ctx, const ge_attention_shape* shape, const void* q, const void* k, const void* v,
+                           const ge_attention_seq* seqs, int32_t n_seqs, void* out);
+
+/* The same where every sequence's keys are the prefix_len rows of prefix_k / prefix_v (k's and v's strides)
+ * followed by its own kv_len rows: n = prefix_len + kv_len keys, j <= i + n - q_len, j > i + n - q_len - window.
+ * The prefix is read once for all sequences whose query rows follow each other and see all of it
+ * (no window, q_len <= kv_len + 1). */
+int ge_op_attention_prefix(ge_ctx* ctx, const ge_attention_shape* shape, const void* q, const void* prefix_k,
+                           const void* prefix_v, int32_t prefix_len, const void* k, const void* v,
+                           const ge_attention_seq* seqs, int32_t n_seqs, void* out);
+
 /* ---- image tower, on the same context as the text encoder.
  * Replaces Metal/VisionTower.swift (VisionTower.upload :113-140, encode :143-185) for a
  * pre-LayerNorm ViT: per layer x += attn_out(attn(LN1(x))) + b, x += down(gelu_tanh(up(LN2(x)))),
