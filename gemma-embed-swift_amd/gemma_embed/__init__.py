@@ -34,6 +34,7 @@ ERRORS = {
 (GE_ERR_INVALID, GE_ERR_GGUF, GE_ERR_MODEL, GE_ERR_GPU, GE_ERR_OPTIONS, GE_ERR_STATE, GE_ERR_CANCELLED,
  GE_ERR_NO_DEVICE) = range(1, 9)
 GE_TYPE_F32, GE_TYPE_F16, GE_TYPE_Q8_0, GE_TYPE_BF16 = 0, 1, 8, 30
+GE_TYPE_Q4_0, GE_TYPE_Q4_1 = 2, 3  # the 4-bit per-op entries
 
 
 class GemmaEmbedError(RuntimeError):
@@ -161,6 +162,10 @@ SIGNATURES = {
     "ge_op_mean_pool": (_I, [_P, _P, C.c_int32, C.c_int32, _P, C.c_int32, _P]),
     "ge_op_attention_split": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                    C.c_int32, C.c_float]),
+    "ge_op_q4_create": (_I, [_P, _P, C.c_int32, C.c_int32, C.c_int32, C.POINTER(_P)]),
+    "ge_op_q4_destroy": (_I, [_P, _P]),
+    "ge_op_gemv_q4": (_I, [_P, _P, _P, C.c_int32, C.c_int32, _P, C.c_int32]),
+    "ge_op_gemv_q4_geglu": (_I, [_P, _P, _P, _P, C.c_int32, C.c_int32, _P, C.c_int32]),
     "ge_op_attention_causal": (_I, [_P, C.POINTER(ge_attention_shape), _P, _P, _P, _P, C.c_int32, _P]),
     "ge_op_attention_prefix": (_I, [_P, C.POINTER(ge_attention_shape), _P, _P, _P, C.c_int32, _P, _P, _P, C.c_int32, _P]),
     "ge_model_load": (_I, [C.c_char_p, C.POINTER(ge_load_options), C.POINTER(_P), C.c_char_p, C.c_size_t]),
@@ -601,6 +606,27 @@ class Context:
     def gemm_q8_geglu(self, gate: int, up: int, x: int, m: int, act: int):
         self._check(lib.ge_op_gemm_q8_geglu(self.handle, C.c_void_p(gate), C.c_void_p(up), C.c_void_p(x), m,
                                             C.c_void_p(act)), "ge_op_gemm_q8_geglu")
+
+    # ---- 4-bit weights
+    def q4_create(self, q4_rows: np.ndarray, type: int, rows: int, cols: int) -> int:
+        """A Q4_0 or Q4_1 matrix (GGUF blocks in host memory) in device memory."""
+        h = C.c_void_p()
+        b = np.ascontiguousarray(q4_rows, dtype=np.uint8)
+        need = rows * cols // 32 * (20 if type == GE_TYPE_Q4_1 else 18)
+        if b.size < need:
+            raise GemmaEmbedError(GE_ERR_INVALID, f"{b.size} bytes of 4-bit blocks, {need} needed")
+        self._check(lib.ge_op_q4_create(self.handle, b.ctypes.data, type, rows, cols, C.byref(h)), "ge_op_q4_create")
+        return h.value
+
+    def q4_destroy(self, h: int):
+        self._check(lib.ge_op_q4_destroy(self.handle, h), "ge_op_q4_destroy")
+
+    def gemv_q4(self, w: int, x: int, x_type: int, m: int, y: int, y_type: int):
+        """y[m][rows] = x[m][cols] W^T; x F16 or BF16, y F32, F16 or BF16."""
+        self._check(lib.ge_op_gemv_q4(self.handle, w, x, x_type, m, y, y_type), "ge_op_gemv_q4")
+
+    def gemv_q4_geglu(self, gate: int, up: int, x: int, x_type: int, m: int, act: int, act_type: int):
+        self._check(lib.ge_op_gemv_q4_geglu(self.handle, gate, up, x, x_type, m, act, act_type), "ge_op_gemv_q4_geglu")
 
     def attention(self, q: int, k: int, v: int, out: int, work: int, n_work: int, heads: int, kv_heads: int,
                   head_dim: int, half_window: int, scale: float = 1.0):

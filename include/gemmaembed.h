@@ -42,6 +42,8 @@ enum {
 
 /* ggml tensor types the loader accepts (GGUF/GGUFValue.swift:84-89). */
 enum { GE_TYPE_F32 = 0, GE_TYPE_F16 = 1, GE_TYPE_Q8_0 = 8, GE_TYPE_BF16 = 30 };
+/* ggml tensor types of the 4-bit per-op entries; the model loader does not accept them. */
+enum { GE_TYPE_Q4_0 = 2, GE_TYPE_Q4_1 = 3 };
 
 /* ===================================================================== device library */
 
@@ -187,6 +189,25 @@ int ge_op_gemm_q8(ge_ctx* ctx, const ge_q8_matrix* w, const void* x, int32_t m, 
  * act[M][F] = gelu_tanh(x * Wg^T) * (x * Wu^T), fp16 out. */
 int ge_op_gemm_q8_geglu(ge_ctx* ctx, const ge_q8_matrix* gate, const ge_q8_matrix* up, const void* x, int32_t m,
                         void* act);
+
+/* 4-bit weights with a scale for each group of 32 columns, for the products of few rows (a token, a handful
+ * of tokens) that are bound by reading the weights. No counterpart in the reference, whose weights are
+ * Q8_0. `rows` GGUF rows of `cols` elements in host memory, cols a multiple of 32, any number of rows:
+ * type GE_TYPE_Q4_0 (18-byte blocks: fp16 d, 16 bytes; w = d (q - 8)) or GE_TYPE_Q4_1 (20-byte blocks: fp16 d
+ * and m, 16 bytes; w = d q + m), element j of a block in byte j % 16's low (j < 16) or high nibble. */
+typedef struct ge_q4_matrix ge_q4_matrix;
+int ge_op_q4_create(ge_ctx* ctx, const void* q4_rows, int32_t type, int32_t rows, int32_t cols, ge_q4_matrix** out);
+int ge_op_q4_destroy(ge_ctx* ctx, ge_q4_matrix* m);
+
+/* y[M][N] = x[M][K] * W^T with W [N][K] in 4 bits: x of x_type GE_TYPE_F16 or GE_TYPE_BF16, y of y_type
+ * GE_TYPE_F32, GE_TYPE_F16 or GE_TYPE_BF16, rows back to back, 16-byte aligned. The weights enter as the
+ * integers they are and the sums are fp32: y is rounded once, to its type. Any M up to 2^20 (the weights
+ * are read once for every 64 rows). */
+int ge_op_gemv_q4(ge_ctx* ctx, const ge_q4_matrix* w, const void* x, int32_t x_type, int32_t m, void* y, int32_t y_type);
+/* The same with the geglu epilogue: act[M][F] = gelu_tanh(x * Wg^T) * (x * Wu^T), gate and up of one shape
+ * and type. */
+int ge_op_gemv_q4_geglu(ge_ctx* ctx, const ge_q4_matrix* gate, const ge_q4_matrix* up, const void* x, int32_t x_type,
+                        int32_t m, void* act, int32_t act_type);
 
 /* The forward's row kernels on device memory (fp32 unless stated; widths a multiple of 4 up to
  * 1024). Integer inputs the kernels gather with (ids, positions, sequence ranges) are checked on
