@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <functional>
 #include <vector>
 
 #include "causal.hpp"
@@ -19,9 +20,8 @@
 namespace ge {
 namespace {
 
-// Split tiles: keys an item takes at least (a split costs its rows' partial results and a share of the
-// joining launch), and the workgroups a launch is split up to.
-constexpr int64_t kSplitMinKeys = 256, kSplitGroups = 512;
+constexpr int kCus = 256;
+constexpr int64_t kSplitMinKeys = 128;
 constexpr int64_t kMaxRows = int64_t(1) << 30, kMaxStride = int64_t(1) << 24;
 
 struct Tile {
@@ -57,6 +57,65 @@ Base make_base(uint32_t q_token, int64_t tokens, uint32_t source, uint32_t key0,
         b.tiles.push_back(t);
     }
     return b;
+}
+
+int64_t splits_of(const Tile& t, int64_t limit) { return (t.hi - t.lo + limit - 1) / limit; }
+// 64-key steps keep the parts' blocks whole.
+int64_t step_of(const Tile& t, int64_t splits) { return splits ? (t.hi - t.lo + splits * 64 - 1) / (splits * 64) * 64 : 0; }
+
+// The most keys of an item. Splitting fills the GPU and evens the items out, and costs the parts' rows
+// (written, and read by the joining launch). Of no split and splits into about 1, 1.5, 2 and 3 items a CU the
+// one whose estimate is least, in microseconds: a key of an item of head dim 128 takes 0.025 with one
+// workgroup on a CU and 0.6 of that each with two (narrow items, which wait for memory, gain nothing by
+// pairs), an item 7 besides its keys, a joining launch 5 and 1 for 3 MB of parts. Calls of few or many
+// items (under 64 keys each, four a CU unsplit) are not split.
+int64_t split_limit(const std::vector<Base>& bases, const ge_attention_shape& s) {
+    constexpr int kBins = 64;
+    const double key_us = 0.025 * s.head_dim / 128;
+    int64_t total = 0, longest = 0, tiles = 0, wide_keys = 0;
+    for (const Base& b : bases)
+        for (const Tile& t : b.tiles) {
+            total += t.hi - t.lo;
+            if (t.n_rows > uint32_t(kCausalNarrowRows)) wide_keys += t.hi - t.lo;
+            longest = std::max(longest, t.hi - t.lo);
+            tiles++;
+        }
+    if (longest <= kSplitMinKeys || tiles * s.kv_heads >= 4 * kCus) return std::max<int64_t>(longest, 64);
+    const double pair = 2 * wide_keys >= total ? 0.6 : 1.0;
+    int64_t best = longest;
+    double best_us = 1e300;
+    for (const double per_cu : {0.0, 1.0, 1.5, 2.0, 3.0}) {
+        const int64_t limit =
+            per_cu == 0.0 ? longest : std::max(kSplitMinKeys, (int64_t(double(total * s.kv_heads) / (per_cu * kCus)) + 63) / 64 * 64);
+        if (per_cu != 0.0 && limit >= longest) continue;
+        // items by their keys, in kBins steps
+        int64_t count[kBins] = {}, items = 0, parts = 0;
+        const int64_t top = std::min(limit, longest);
+        for (const Base& b : bases)
+            for (const Tile& t : b.tiles) {
+                const int64_t n = splits_of(t, limit);
+                if (!n) continue;
+                count[std::min<int64_t>(kBins - 1, (t.hi - t.lo) / n * kBins / (top + 1))] += n * s.kv_heads;
+                items += n * s.kv_heads;
+                if (!b.direct || n > 1) parts += n * t.n_rows;
+            }
+        // at least the work at the rate of full CUs, and, with the items started longest first, two a CU, the
+        // end of the first of each round's first and second half
+        double us = double(total) * double(s.kv_heads) * key_us * pair / kCus;
+        int64_t k = 0, seen = 0;
+        for (int bin = kBins - 1; bin >= 0; bin--) {
+            seen += count[bin];
+            for (; k < seen; k += kCus)
+                us = std::max(us, (double(k / (2 * kCus)) * 2 * pair + (k / kCus % 2 ? 2 * pair : 1.0)) * key_us * double(top) * (bin + 1) / kBins);
+        }
+        us += 7.0 * double((items + 2 * kCus - 1) / (2 * kCus));
+        if (parts) us += 5.0 + double(parts) * s.kv_heads * s.head_dim * 8 / 3e6;
+        if (us < best_us) {
+            best_us = us;
+            best = limit;
+        }
+    }
+    return best;
 }
 
 Plan make_plan(const ge_attention_shape& s, const ge_attention_seq* seqs, int n_seqs, int64_t prefix_len) {
@@ -98,23 +157,17 @@ Plan make_plan(const ge_attention_shape& s, const ge_attention_seq* seqs, int n_
         i = j;
     }
 
-    int64_t keys = 0;
-    for (const Base& b : bases)
-        for (const Tile& t : b.tiles) keys += t.hi - t.lo;
-    const int64_t limit =
-        (std::max(kSplitMinKeys, (keys * s.kv_heads + kSplitGroups - 1) / kSplitGroups) + 63) / 64 * 64;
+    const int64_t limit = split_limit(bases, s);
     Plan p;
     for (Base& b : bases)
         for (Tile& t : b.tiles) {
-            const int64_t n = t.hi - t.lo, splits = (n + limit - 1) / limit;
-            // 64-key steps keep the parts' blocks whole
-            const int64_t step = splits ? (n + splits * 64 - 1) / (splits * 64) * 64 : 0;
+            const int64_t splits = splits_of(t, limit), step = step_of(t, splits);
             const bool narrow = t.n_rows <= uint32_t(kCausalNarrowRows), direct = b.direct && splits <= 1;
             t.part = uint32_t(p.part_rows);
             for (int64_t k = t.lo; k < t.hi || (direct && t.splits == 0); k += step) {
                 p.items.push_back(CausalItem{b.q_token, t.row0, t.n_rows, b.key0, uint32_t(k), uint32_t(std::min(k + step, t.hi)),
                                              int32_t(b.shift), direct ? kDirect : uint32_t(p.part_rows), b.source, narrow});
-                p.kinds |= narrow ? 2 : 1;
+                p.kinds |= narrow ? kCausalNarrow : kCausalWide;
                 t.splits++;
                 if (direct) break;
                 p.part_rows += t.n_rows;
@@ -203,10 +256,12 @@ void attend(ge_ctx* c, const ge_attention_shape* shape, const void* q, const voi
     if (p.items.size() * uint64_t(s.kv_heads) > kCausalMaxGroups || p.joins.size() * uint64_t(s.kv_heads) > kCausalMaxGroups)
         fail(GE_ERR_INVALID, "attention: the call's rows and keys are too many for one call");
     OpTemps temps(c);
+    CausalInline in;
+    const bool few = p.items.size() <= size_t(kCausalInlineItems) && p.joins.size() <= size_t(kCausalInlineJoins);
     const size_t item_bytes = (p.items.size() * sizeof(CausalItem) + 255) / 256 * 256;
-    unsigned char* const lists = op_lists(c, item_bytes + p.joins.size() * sizeof(CausalJoin));
-    std::copy(p.items.begin(), p.items.end(), reinterpret_cast<CausalItem*>(lists));
-    std::copy(p.joins.begin(), p.joins.end(), reinterpret_cast<CausalJoin*>(lists + item_bytes));
+    unsigned char* const lists = few ? nullptr : op_lists(c, item_bytes + p.joins.size() * sizeof(CausalJoin));
+    std::copy(p.items.begin(), p.items.end(), few ? in.items : reinterpret_cast<CausalItem*>(lists));
+    std::copy(p.joins.begin(), p.joins.end(), few ? in.joins : reinterpret_cast<CausalJoin*>(lists + item_bytes));
     const size_t o_at = temps.reserve(p.part_rows * size_t(kv_width) * 4);
     const size_t ml_at = temps.reserve(p.part_rows * size_t(s.kv_heads) * 8);
     unsigned char* const base = p.part_rows ? temps.base() : nullptr;
@@ -219,7 +274,7 @@ void attend(ge_ctx* c, const ge_attention_shape* shape, const void* q, const voi
     a.prefix_v = static_cast<const uint16_t*>(prefix_v);
     a.out = static_cast<uint16_t*>(out);
     a.items = reinterpret_cast<const CausalItem*>(lists);
-    a.joins = reinterpret_cast<const CausalJoin*>(lists + item_bytes);
+    a.joins = few ? nullptr : reinterpret_cast<const CausalJoin*>(lists + item_bytes);
     a.part_o = reinterpret_cast<float*>(base + o_at);
     a.part_ml = reinterpret_cast<float2*>(base + ml_at);
     a.q_stride = s.q_stride;
@@ -229,15 +284,16 @@ void attend(ge_ctx* c, const ge_attention_shape* shape, const void* q, const voi
     a.part_rows = p.part_rows;
     a.n_items = int(p.items.size());
     a.n_joins = int(p.joins.size());
+    for (const CausalJoin& j : p.joins) a.join_rows = std::max(a.join_rows, int(j.n_rows));
     a.group = s.heads / s.kv_heads;
     a.kv_heads = s.kv_heads;
     a.window = s.window;
     // a hidden key's -inf times this stays -inf, also at scale 0
     a.c = std::min(std::max(std::fabs(s.scale) * 1.4426950408889634f, FLT_MIN), FLT_MAX);
     a.q_flip = s.scale < 0.0f ? 0x80008000u : 0u;
-    launch(c, "attention_causal", [&] { return launch_causal(c->stream, a, s.head_dim, s.type == GE_TYPE_BF16, p.kinds); });
+    launch(c, "attention_causal", [&] { return launch_causal(c->stream, a, in, s.head_dim, s.type == GE_TYPE_BF16, p.kinds); });
     if (a.n_joins)
-        launch(c, "attention_join", [&] { return launch_causal_join(c->stream, a, s.head_dim, s.type == GE_TYPE_BF16); });
+        launch(c, "attention_join", [&] { return launch_causal_join(c->stream, a, in, s.head_dim, s.type == GE_TYPE_BF16); });
     hip_check(hipStreamSynchronize(c->stream), "hipStreamSynchronize");
 }
 

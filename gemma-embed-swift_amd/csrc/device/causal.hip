@@ -90,11 +90,23 @@ struct KvBlock {
         const int tile = lane >> 3, key = (tile >> 2) * 4 + ((lane & 7) >> 1), dim = (tile & 3) * 16 + (lane & 1) * 8;
         return uint32_t(key) * row_bytes + uint32_t(dim * 2);
     }
-    // Chunk c of a block whose rows start at r's base; rows past r's size read as zeros.
-    static __device__ __forceinline__ void copy(__amdgpu_buffer_rsrc_t r, unsigned char* block, int c, uint32_t lane_off,
-                                                uint32_t row_bytes) {
-        const int panel = c / (BK / 8), k8 = c % (BK / 8);
-        lds_copy16(r, block + c * 1024, lane_off + uint32_t(k8 * 8) * row_bytes + uint32_t(panel * 128), 0);
+    // Chunk (PANEL, k8) of a block whose rows start at r's base; off: the lane's offset of row 8 k8. Rows past
+    // r's size read as zeros. The panel goes into the instruction's offset, which moves the LDS address as well
+    // as the source's, so that a wave's chunks of a row group share one offset register.
+    template <int PANEL>
+    static __device__ __forceinline__ void copy(__amdgpu_buffer_rsrc_t r, unsigned char* block, int k8, uint32_t off) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            r, (__attribute__((address_space(3))) void*)(block + (PANEL * (BK / 8) + k8) * 1024 - PANEL * 128), 16, off, 0, PANEL * 128, 0);
+    }
+    // The wave's chunks of panels [0, PANELS) and row groups k8, k8 + STEP, ... in this order.
+    template <int PANELS, int STEP, int I = 0>
+    static __device__ __forceinline__ void copies(__amdgpu_buffer_rsrc_t r, unsigned char* block, int k8,
+                                                  const uint32_t (&off)[BK / 8 / STEP]) {
+        constexpr int N = BK / 8 / STEP;
+        if constexpr (I < PANELS * N) {
+            copy<I / N>(r, block, k8 + I % N * STEP, off[I % N]);
+            copies<PANELS, STEP, I + 1>(r, block, k8, off);
+        }
     }
     // Rows [key, key + rows) of a tensor whose row 0 is at base, for the head at element offset `at`.
     static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const uint16_t* base, size_t key, int64_t stride, int at,
@@ -103,20 +115,15 @@ struct KvBlock {
     }
 };
 
-// Waves that hold the same 32 rows, each with its share of the head's dims in its accumulators: at head
-// dim 512 the queries (128 registers) and all accumulators (256) do not fit beside the rest, so two
-// waves both compute the scores and take half of the product each.
+// Fragments read ahead of their products (four spill at head dim 256).
 template <int HD>
-constexpr int kDimWaves = HD > 256 ? 2 : 1;
-// Fragments read ahead of their products (more spill at head dim 256).
-template <int HD>
-constexpr int kFragmentsAhead = HD > 128 ? 2 : 4;
+constexpr int kFragmentsAhead = HD == 256 ? 3 : 4;
 
-// 32 rows of one KV head: queries in registers, accumulators (of the dims' share `part`), running
-// maximum and sum.
-template <typename T, int HD>
+// 32 rows of one KV head: queries in registers, accumulators, running maximum and sum. DW waves can hold
+// the same rows: they all compute the scores and each takes its share of the head's dims in the product.
+template <typename T, int HD, int DW>
 struct Rows {
-    static constexpr int KS = HD / 16, DT = HD / 32 / kDimWaves<HD>;
+    static constexpr int KS = HD / 16, DT = HD / 32 / DW;
     u32x4 q[KS];
     float16_t o[DT];
     float m, l;
@@ -316,6 +323,7 @@ struct HeldBack {
         if ((threadIdx.x & 63) == 0) flag[threadIdx.x >> 6] = any;
         __syncthreads();
         any = (flag[0] | flag[1] | flag[2] | flag[3]) != 0;
+        __syncthreads();
     }
     // Rows [r0, r0 + n), dims [d0, d0 + dims), which this wave has stored.
     __device__ __forceinline__ static void add(const CausalArgs& a, const CausalItem& it, int kvh, int r0, int n, int d0, int dims) {
@@ -343,12 +351,13 @@ struct HeldBack {
 
 // ---------------------------------------------------------------------------- many rows: waves over rows
 
-// 128 rows, 32 a wave (64 at head dim 512); the workgroup's waves copy each key block together, two
-// blocks in LDS.
+// 128 rows, 32 a wave; the workgroup's waves copy each key block together, two blocks in LDS. At head dim
+// 512 the queries (128 registers) and all accumulators (256) do not fit beside the rest: 64 rows, 32 a
+// pair of waves.
 template <typename T, int HD>
 struct Wide {
-    static constexpr int NW = 4, BK = HD <= 128 ? 64 : 32;
-    static_assert(NW / kDimWaves<HD> * 32 == causal_wide_rows(HD), "rows of a wide item");
+    static constexpr int NW = 4, DW = HD > 256 ? 2 : 1, BK = HD <= 128 ? 64 : 32;
+    static_assert(NW / DW * 32 == causal_wide_rows(HD), "rows of a wide item");
     using Kv = KvBlock<HD, BK>;
     static constexpr int kLds = 2 * 2 * Kv::kBytes;
 
@@ -358,7 +367,12 @@ struct Wide {
         const uint16_t* const vp = it.source ? a.prefix_v : a.v;
         const uint32_t kb_bytes = uint32_t(a.k_stride) * 2, vb_bytes = uint32_t(a.v_stride) * 2;
         static_assert(Kv::kChunks % NW == 0 && (BK / 8) % NW == 0 && NW % 2 == 0, "every wave copies chunks of one key parity");
-        const uint32_t k_off = Kv::k_lane(lane, wave & 1, kb_bytes), v_off = Kv::v_lane(lane, vb_bytes);
+        uint32_t k_off[BK / 8 / NW], v_off[BK / 8 / NW];
+#pragma unroll
+        for (int i = 0; i < BK / 8 / NW; i++) {
+            k_off[i] = Kv::k_lane(lane, wave & 1, kb_bytes) + uint32_t((wave + i * NW) * 8) * kb_bytes;
+            v_off[i] = Kv::v_lane(lane, vb_bytes) + uint32_t((wave + i * NW) * 8) * vb_bytes;
+        }
         const int k_lo = int(it.k_lo), k_hi = int(it.k_hi);
         const int blocks = (k_hi - k_lo + BK - 1) / BK;
         auto issue = [&](int b) {
@@ -366,32 +380,29 @@ struct Wide {
             unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
             const auto kr = Kv::rows_of(kp, size_t(it.key0) + kb, a.k_stride, kvh * HD, rows);
             const auto vr = Kv::rows_of(vp, size_t(it.key0) + kb, a.v_stride, kvh * HD, rows);
-#pragma unroll
-            for (int i = 0; i < Kv::kChunks / NW; i++) Kv::copy(kr, at, wave + i * NW, k_off, kb_bytes);
-#pragma unroll
-            for (int i = 0; i < Kv::kChunks / NW; i++) Kv::copy(vr, at + Kv::kBytes, wave + i * NW, v_off, vb_bytes);
+            Kv::template copies<HD / 64, NW>(kr, at, wave, k_off);
+            Kv::template copies<HD / 64, NW>(vr, at + Kv::kBytes, wave, v_off);
         };
-        constexpr int DW = kDimWaves<HD>;
         const int r0 = int(it.row0) + wave / DW * 32, n = min(32, int(it.n_rows) - wave / DW * 32);
-        Rows<T, HD> w;
+        Rows<T, HD, DW> w;
         HeldBack<T, HD> held;
         held.init(a, it);
         if (blocks > 0) issue(0);
         if (n > 0) w.init(a, it, kvh, r0, n, wave % DW, lane);
         for (int b = 0; b < blocks; b++) {
             const int kb = k_lo + b * BK;
+            unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
             wait_vmcnt<0>();
             if (held.mixed(kb, BK)) {
-                unsigned char* const at = lds + ((b & 1) * 2 + 1) * Kv::kBytes;
 #pragma unroll
-                for (int i = 0; i < Kv::kChunks / NW; i++) held.clear(at + (wave + i * NW) * 1024 + lane * 16);
+                for (int i = 0; i < Kv::kChunks / NW; i++)  // the chunks this wave copied
+                    held.clear(at + Kv::kBytes + (wave + i * NW) * 1024 + lane * 16);
             }
             wait_lgkmcnt0();
             workgroup_barrier();
             if (b + 1 < blocks) issue(b + 1);
             if (n > 0 && kb <= w.hi_any && kb + BK - 1 >= w.lo_any) {
-                const unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
-                typename Rows<T, HD>::template Block<BK> blk;
+                typename Rows<T, HD, DW>::template Block<BK> blk;
                 u32x4 p[BK / 16];
                 blk.scores(w, at, lane);
                 blk.softmax(w, kb, a.c, lane, p);
@@ -409,17 +420,60 @@ struct Wide {
 
 // ---------------------------------------------------------------------------- few rows: waves over keys
 
-// 32 rows; the waves (at head dim 512 the pairs of waves that share the dims) take the key blocks in
-// turn, each through LDS of its own, and join at the end. A wave alone on its LDS waits for its own copies
-// only; a pair meets at the workgroup's barriers.
+// The waves that took different key blocks of the same rows join: all but the first leave their maximum, sum
+// and accumulators in LDS, the first adds them in order. Every wave of the workgroup comes here; LDS is
+// no longer read.
+template <typename T, int HD, int DW, int KW>
+struct JoinKeys {
+    using W = Rows<T, HD, DW>;
+    static constexpr int kAcc = W::DT * 16;
+    static constexpr int kLds = (KW - 1) * DW * 64 * (kAcc + 2) * 4;
+    static __device__ __forceinline__ void run(W& w, int kw, int dims, int lane, unsigned char* lds) {
+        float* const j = reinterpret_cast<float*>(lds);
+        if (kw > 0) {
+            float* const p = j + (((kw - 1) * DW + dims) * (kAcc + 2)) * 64 + lane;
+            p[0] = w.m;
+            p[64] = w.l;
+#pragma unroll
+            for (int d = 0; d < W::DT; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) p[(2 + d * 16 + e) * 64] = w.o[d][e];
+        }
+        __syncthreads();
+        if (kw > 0) return;
+        float top = w.m;
+#pragma unroll
+        for (int k = 1; k < KW; k++) top = fmaxf(top, j[((k - 1) * DW + dims) * (kAcc + 2) * 64 + lane]);
+        const float f0 = w.m == top ? 1.0f : __builtin_amdgcn_exp2f(w.m - top);
+        w.l *= f0;
+#pragma unroll
+        for (int d = 0; d < W::DT; d++) w.o[d] *= f0;
+        for (int k = 1; k < KW; k++) {
+            const float* const p = j + ((k - 1) * DW + dims) * (kAcc + 2) * 64 + lane;
+            const float mk = p[0], f = mk == top ? 1.0f : __builtin_amdgcn_exp2f(mk - top);
+            w.l += p[64] * f;
+#pragma unroll
+            for (int d = 0; d < W::DT; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) w.o[d][e] += p[(2 + d * 16 + e) * 64] * f;
+        }
+        w.m = top;
+    }
+};
+
+// 32 rows; the waves take the key blocks in turn, each through LDS of its own, and join at the end. From head
+// dim 256 on pairs of waves take a block together, so that the workgroup's LDS is half as large and
+// two fit a CU (at 256; a launch of both kinds of items takes the larger of their LDS: with four waves'
+// blocks, 128 KB, 128 texts over a prefix of 8192 took 192 us). A wave alone on its LDS waits for its own
+// copies only; pairs meet at the workgroup's barriers.
 template <typename T, int HD>
 struct Narrow {
-    static constexpr int DW = kDimWaves<HD>, KW = 4 / DW, BK = 32;
+    static constexpr int DW = HD > 128 ? 2 : 1, KW = 4 / DW, BK = 32;
     using Kv = KvBlock<HD, BK>;
     static constexpr int kChunks = Kv::kChunks / DW;  // a wave's copies of K, and of V
-    static constexpr int kPerKw = 2 * Kv::kBytes, kAcc = Rows<T, HD>::DT * 16;
-    static constexpr int kJoin = 4 * 64 * (kAcc + 2) * 4;
-    static constexpr int kLds = KW * kPerKw > kJoin ? KW * kPerKw : kJoin;
+    using Join = JoinKeys<T, HD, DW, KW>;
+    static constexpr int kPerKw = 2 * Kv::kBytes;
+    static constexpr int kLds = KW * kPerKw > Join::kLds ? KW * kPerKw : Join::kLds;
 
     static __device__ __forceinline__ void meet() {
         wait_lgkmcnt0();
@@ -435,8 +489,14 @@ struct Narrow {
         const uint16_t* const kp = it.source ? a.prefix_k : a.k;
         const uint16_t* const vp = it.source ? a.prefix_v : a.v;
         const uint32_t kb_bytes = uint32_t(a.k_stride) * 2, vb_bytes = uint32_t(a.v_stride) * 2;
-        const uint32_t k_even = Kv::k_lane(lane, 0, kb_bytes), k_odd = Kv::k_lane(lane, 1, kb_bytes);
-        const uint32_t v_off = Kv::v_lane(lane, vb_bytes);
+        // a wave of a pair copies half of the panels
+        constexpr int kPanels = HD / 64 / DW;
+        uint32_t k_off[BK / 8], v_off[BK / 8];
+#pragma unroll
+        for (int i = 0; i < BK / 8; i++) {
+            k_off[i] = Kv::k_lane(lane, i & 1, kb_bytes) + uint32_t(i * 8) * kb_bytes + uint32_t(dims * kPanels * 128);
+            v_off[i] = Kv::v_lane(lane, vb_bytes) + uint32_t(i * 8) * vb_bytes + uint32_t(dims * kPanels * 128);
+        }
         const int k_lo = int(it.k_lo), k_hi = int(it.k_hi);
         const int blocks = (k_hi - k_lo + BK - 1) / BK;
         unsigned char* const K = lds + kw * kPerKw;
@@ -444,17 +504,15 @@ struct Narrow {
         auto issue_k = [&](int b) {
             const int kb = k_lo + b * BK;
             const auto r = Kv::rows_of(kp, size_t(it.key0) + kb, a.k_stride, kvh * HD, min(BK, k_hi - kb));
-#pragma unroll
-            for (int i = 0; i < kChunks; i++) Kv::copy(r, K, dims * kChunks + i, i & 1 ? k_odd : k_even, kb_bytes);
+            Kv::template copies<kPanels, 1>(r, K + dims * kChunks * 1024, 0, k_off);
         };
         auto issue_v = [&](int b) {
             const int kb = k_lo + b * BK;
             const auto r = Kv::rows_of(vp, size_t(it.key0) + kb, a.v_stride, kvh * HD, min(BK, k_hi - kb));
-#pragma unroll
-            for (int i = 0; i < kChunks; i++) Kv::copy(r, V, dims * kChunks + i, v_off, vb_bytes);
+            Kv::template copies<kPanels, 1>(r, V + dims * kChunks * 1024, 0, v_off);
         };
         const int r0 = int(it.row0), n = int(it.n_rows);
-        Rows<T, HD> w;
+        Rows<T, HD, DW> w;
         HeldBack<T, HD> held;
         held.init(a, it);
         if (kw < blocks) {
@@ -467,7 +525,7 @@ struct Narrow {
             const int kb = k_lo + b * BK;
             const bool mine = b < blocks, more = b + KW < blocks;
             if (DW == 1 && !mine) break;
-            typename Rows<T, HD>::template Block<BK> blk;
+            typename Rows<T, HD, DW>::template Block<BK> blk;
             u32x4 p[BK / 16];
             wait_vmcnt<kChunks>();  // all but V's copies
             meet();
@@ -490,135 +548,166 @@ struct Narrow {
         }
         w.l = sum_over_halves(w.l);
         held.share(lds);
-        // Join: every wave leaves its maximum, sum and accumulators in LDS, the first of each share of the
-        // dims adds them in order.
-        __syncthreads();
-        float* const j = reinterpret_cast<float*>(lds);
-        if (kw > 0) {
-            float* const p = j + (wave * (kAcc + 2)) * 64 + lane;
-            p[0] = w.m;
-            p[64] = w.l;
-#pragma unroll
-            for (int d = 0; d < Rows<T, HD>::DT; d++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) p[(2 + d * 16 + e) * 64] = w.o[d][e];
-        }
-        __syncthreads();
+        Join::run(w, kw, dims, lane, lds);
         if (kw > 0) return;
-        float top = w.m;
-#pragma unroll
-        for (int k = 1; k < KW; k++) top = fmaxf(top, j[(k * DW + dims) * (kAcc + 2) * 64 + lane]);
-        const float f0 = w.m == top ? 1.0f : __builtin_amdgcn_exp2f(w.m - top);
-        w.l *= f0;
-#pragma unroll
-        for (int d = 0; d < Rows<T, HD>::DT; d++) w.o[d] *= f0;
-        for (int k = 1; k < KW; k++) {
-            const float* const p = j + (k * DW + dims) * (kAcc + 2) * 64 + lane;
-            const float mk = p[0], f = mk == top ? 1.0f : __builtin_amdgcn_exp2f(mk - top);
-            w.l += p[64] * f;
-#pragma unroll
-            for (int d = 0; d < Rows<T, HD>::DT; d++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) w.o[d][e] += p[(2 + d * 16 + e) * 64] * f;
-        }
-        w.m = top;
         w.finish(a, it, kvh, r0, n, lane);
         if (held.any) held.add(a, it, kvh, r0, n, w.d0 * 32, w.DT * 32);
     }
 };
 
-// KINDS: the items of the launch: 1 wide, 2 narrow, 3 both.
+// Entry `at` of a list in memory, or of the one among the arguments, in scalar registers.
+template <typename E>
+__device__ __forceinline__ E uniform_entry(const E* list, const E* few, uint32_t at) {
+    constexpr int N = sizeof(E) / 4;
+    uint32_t w[N];
+    if (list) {
+        const uint32_t* const p = reinterpret_cast<const uint32_t*>(list + at);
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = uint32_t(__builtin_amdgcn_readfirstlane(int(p[i])));
+    } else {
+        const uint32_t* const p = reinterpret_cast<const uint32_t*>(few + at);
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = uint32_t(__builtin_amdgcn_readfirstlane(int(p[i])));
+    }
+    E e;
+    __builtin_memcpy(&e, w, sizeof(E));
+    return e;
+}
+
+// KINDS: the items of the launch, kCausalWide and kCausalNarrow or one of them.
 template <typename T, int HD, int KINDS>
 constexpr int causal_lds() {
-    const int w = KINDS & 1 ? Wide<T, HD>::kLds : 0, n = KINDS & 2 ? Narrow<T, HD>::kLds : 0;
-    return w > n ? w : n;
+    int lds = 0;
+    if constexpr ((KINDS & kCausalWide) != 0) lds = Wide<T, HD>::kLds;
+    if constexpr ((KINDS & kCausalNarrow) != 0) lds = lds > Narrow<T, HD>::kLds ? lds : Narrow<T, HD>::kLds;
+    return lds;
 }
 
 template <typename T, int HD, int KINDS>
-__global__ __launch_bounds__(256, HD <= 256 ? 2 : 1) void causal_kernel(const CausalArgs a) {
+__global__ __launch_bounds__(256, HD <= 256 ? 2 : 1) void causal_kernel(const CausalArgs a, const CausalInline in) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char causal_lds_mem[];
     // Workgroups go to the 8 XCDs in turn: with the KV head fastest, a head's items share an L2.
     const uint32_t at = blockIdx.x / uint32_t(a.kv_heads);
     const int kvh = int(blockIdx.x % uint32_t(a.kv_heads));
-    const CausalItem it = a.items[at];
-    if (KINDS == 1 || (KINDS == 3 && !it.narrow))
-        Wide<T, HD>::run(a, it, kvh, causal_lds_mem);
-    else
+    const CausalItem it = uniform_entry<CausalItem>(a.items, in.items, at);
+    if (KINDS == kCausalNarrow || ((KINDS & kCausalNarrow) && it.narrow))
         Narrow<T, HD>::run(a, it, kvh, causal_lds_mem);
+    else if constexpr ((KINDS & kCausalWide) != 0)
+        Wide<T, HD>::run(a, it, kvh, causal_lds_mem);
 }
 
 // ---------------------------------------------------------------------------- joining the parts
 
-// One wave a row: the parts' maxima and sums, then their rows weighted and added in order.
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int x = 32; x; x >>= 1) v = fmaxf(v, __shfl_xor(v, x, 64));
+    return v;
+}
+__device__ __forceinline__ float lane_value(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
+// One wave a row, kJoinRows rows a workgroup: the parts' maxima and sums, a lane a part, then their rows
+// weighted and added in order.
+constexpr int kJoinRows = 4;
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void causal_join_kernel(const CausalArgs a) {
-    constexpr int E = HD / 64;
+__global__ __launch_bounds__(256) void causal_join_kernel(const CausalArgs a, const CausalInline in) {
+    constexpr int E = HD / 64, V = E < 4 ? E : 4;  // dims a lane, and of one load
+    typedef float vec_t __attribute__((ext_vector_type(V)));
     const int lane = threadIdx.x & 63;
     const uint32_t at = blockIdx.x / uint32_t(a.kv_heads), kvh = blockIdx.x % uint32_t(a.kv_heads), g = uint32_t(a.group);
-    const CausalJoin jn = a.joins[at];
-    for (uint32_t row = threadIdx.x >> 6; row < jn.n_rows; row += 4) {
-        const size_t base = size_t(kvh) * a.part_rows + row;
-        const uint32_t parts = jn.splits[0] + jn.splits[1];
-        auto place = [&](uint32_t s) {
-            const int side = s < jn.splits[0] ? 0 : 1;
-            return base + jn.part[side] + size_t(side ? s - jn.splits[0] : s) * jn.stride[side];
-        };
-        float top = -INFINITY;
-        for (uint32_t s = 0; s < parts; s++) top = fmaxf(top, a.part_ml[place(s)].x);
-        float sum = 0.0f, o[E] = {};
-        for (uint32_t s = 0; s < parts; s++) {
-            const size_t p = place(s);
-            const float2 ml = a.part_ml[p];
-            if (ml.y == 0.0f) continue;  // it saw no key
-            const float f = ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
-            sum += ml.y * f;
+    const CausalJoin jn = uniform_entry<CausalJoin>(a.joins, in.joins, at);
+    const uint32_t row = blockIdx.y * kJoinRows + (threadIdx.x >> 6);
+    if (row >= jn.n_rows) return;
+    const size_t base = size_t(kvh) * a.part_rows + row;
+    const uint32_t parts = jn.splits[0] + jn.splits[1];
+    auto place = [&](uint32_t s) {
+        return base + (s < jn.splits[0] ? jn.part[0] + size_t(s) * jn.stride[0] : jn.part[1] + size_t(s - jn.splits[0]) * jn.stride[1]);
+    };
+    auto load = [&](uint32_t s) { return s < parts ? a.part_ml[place(s)] : float2{-INFINITY, 0.0f}; };
+    float top = -INFINITY;
+    for (uint32_t s = lane; s - lane < parts; s += 64) top = fmaxf(top, load(s).x);
+    top = wave_max(top);
+    float sum = 0.0f, o[E] = {};
+    for (uint32_t s0 = 0; s0 < parts; s0 += 64) {
+        const float2 ml = load(s0 + lane);
+        // a part that saw no key has nothing to add, whatever its rows hold
+        const float f = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
+        sum += wave_sum(ml.y == 0.0f ? 0.0f : ml.y * f);
+        const int n = int(min(64u, parts - s0));
+        for (int i0 = 0; i0 < n; i0 += 4) {  // four parts' loads in flight
+            vec_t x[4][E / V];
 #pragma unroll
-            for (int e = 0; e < E; e++) o[e] += a.part_o[p * HD + lane * E + e] * f;
-        }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const uint32_t r = jn.row0 + row;
-        uint16_t* out = a.out + (size_t(jn.q_token) + r / g) * size_t(a.out_stride) + (size_t(kvh) * g + r % g) * HD + lane * E;
-        if constexpr (E == 1) {
-            *out = uint16_t(T::pack(o[0] * inv, 0.0f));
-        } else {
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = T::pack(o[e] * inv, o[e + 1] * inv);
+                for (int e = 0; e < E / V; e++)
+                    x[i][e] = *reinterpret_cast<const vec_t*>(a.part_o + place(s0 + min(i0 + i, n - 1)) * HD + e * 64 * V + lane * V);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int k = min(i0 + i, n - 1);
+                const float w = lane_value(f, k);
+                const bool none = i0 + i >= n || lane_value(ml.y, k) == 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] = none ? o[e] : __builtin_fmaf(x[i][e / V][e % V], w, o[e]);
+            }
         }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const uint32_t r = jn.row0 + row;
+    uint16_t* const out = a.out + (size_t(jn.q_token) + r / g) * size_t(a.out_stride) + (size_t(kvh) * g + r % g) * HD;
+#pragma unroll
+    for (int e = 0; e < E; e += V) {
+        uint16_t* const p = out + e * 64 + lane * V;
+        if constexpr (V == 1)
+            *p = uint16_t(T::pack(o[e] * inv, 0.0f));
+        else if constexpr (V == 2)
+            *reinterpret_cast<uint32_t*>(p) = T::pack(o[e] * inv, o[e + 1] * inv);
+        else
+            *reinterpret_cast<u32x2*>(p) = u32x2{T::pack(o[e] * inv, o[e + 1] * inv), T::pack(o[e + 2] * inv, o[e + 3] * inv)};
     }
 }
 
 template <typename T, int HD, int KINDS>
-hipError_t run_items(hipStream_t s, const CausalArgs& a) {
-    launch_kernel(causal_kernel<T, HD, KINDS>, dim3(uint32_t(a.n_items) * uint32_t(a.kv_heads)), dim3(256), uint32_t(causal_lds<T, HD, KINDS>()), s, a);
+hipError_t run_items(hipStream_t s, const CausalArgs& a, const CausalInline& in) {
+    launch_kernel(causal_kernel<T, HD, KINDS>, dim3(uint32_t(a.n_items) * uint32_t(a.kv_heads)), dim3(256), uint32_t(causal_lds<T, HD, KINDS>()), s, a, in);
     return hipGetLastError();
 }
 
 template <typename T, int HD>
-hipError_t run_kinds(hipStream_t s, const CausalArgs& a, int kinds) {
-    return kinds == 1 ? run_items<T, HD, 1>(s, a) : kinds == 2 ? run_items<T, HD, 2>(s, a) : run_items<T, HD, 3>(s, a);
+hipError_t run_kinds(hipStream_t s, const CausalArgs& a, const CausalInline& in, int kinds) {
+    switch (kinds) {
+        case kCausalWide: return run_items<T, HD, kCausalWide>(s, a, in);
+        case kCausalNarrow: return run_items<T, HD, kCausalNarrow>(s, a, in);
+        case kCausalWide | kCausalNarrow: return run_items<T, HD, kCausalWide | kCausalNarrow>(s, a, in);
+    }
+    return hipErrorInvalidValue;
 }
 
 template <typename T, int HD>
-hipError_t run_join(hipStream_t s, const CausalArgs& a) {
-    launch_kernel(causal_join_kernel<T, HD>, dim3(uint32_t(a.n_joins) * uint32_t(a.kv_heads)), dim3(256), 0, s, a);
+hipError_t run_join(hipStream_t s, const CausalArgs& a, const CausalInline& in) {
+    launch_kernel(causal_join_kernel<T, HD>, dim3(uint32_t(a.n_joins) * uint32_t(a.kv_heads), uint32_t(a.join_rows + kJoinRows - 1) / kJoinRows),
+                  dim3(256), 0, s, a, in);
     return hipGetLastError();
+}
+
+template <typename T, int HD, int KINDS>
+hipError_t configure_kinds() {
+    constexpr int lds = causal_lds<T, HD, KINDS>();
+    static_assert(lds <= 160 * 1024, "LDS of a CU");
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(causal_kernel<T, HD, KINDS>),
+                               hipFuncAttributeMaxDynamicSharedMemorySize, lds);
 }
 
 template <typename T, int HD>
 hipError_t configure_hd() {
-    const void* const f[3] = {reinterpret_cast<const void*>(causal_kernel<T, HD, 1>), reinterpret_cast<const void*>(causal_kernel<T, HD, 2>),
-                              reinterpret_cast<const void*>(causal_kernel<T, HD, 3>)};
-    const int lds[3] = {causal_lds<T, HD, 1>(), causal_lds<T, HD, 2>(), causal_lds<T, HD, 3>()};
-    static_assert(causal_lds<T, HD, 3>() <= 160 * 1024, "LDS of a CU");
-    for (int i = 0; i < 3; i++) {
-        const hipError_t e = hipFuncSetAttribute(f[i], hipFuncAttributeMaxDynamicSharedMemorySize, lds[i]);
-        if (e != hipSuccess) return e;
-    }
-    return hipSuccess;
+    hipError_t e = configure_kinds<T, HD, kCausalWide>();
+    if (e == hipSuccess) e = configure_kinds<T, HD, kCausalNarrow>();
+    if (e == hipSuccess) e = configure_kinds<T, HD, kCausalWide | kCausalNarrow>();
+    return e;
 }
 
 bool args_ok(const CausalArgs& a, int hd) {
-    return causal_head_dim_ok(hd) && a.kv_heads > 0 && a.group > 0 && a.n_items >= 0 && a.n_joins >= 0 &&
+    return causal_head_dim_ok(hd) && a.kv_heads > 0 && a.group > 0 && a.n_items >= 0 && a.n_joins >= 0 && a.join_rows >= 0 && a.join_rows <= 128 &&
            uint64_t(a.n_items) * uint64_t(a.kv_heads) <= kCausalMaxGroups && uint64_t(a.n_joins) * uint64_t(a.kv_heads) <= kCausalMaxGroups;
 }
 
@@ -626,25 +715,25 @@ bool args_ok(const CausalArgs& a, int hd) {
 
 bool causal_head_dim_ok(int hd) { return hd == 64 || hd == 128 || hd == 256 || hd == 512; }
 
-hipError_t launch_causal(hipStream_t s, const CausalArgs& a, int hd, bool bf16, int kinds) {
-    if (!args_ok(a, hd) || kinds < 1 || kinds > 3) return hipErrorInvalidValue;
+hipError_t launch_causal(hipStream_t s, const CausalArgs& a, const CausalInline& in, int hd, bool bf16, int kinds) {
+    if (!args_ok(a, hd)) return hipErrorInvalidValue;
     if (a.n_items == 0) return hipSuccess;
     switch (hd) {
-        case 64: return bf16 ? run_kinds<BF16, 64>(s, a, kinds) : run_kinds<F16, 64>(s, a, kinds);
-        case 128: return bf16 ? run_kinds<BF16, 128>(s, a, kinds) : run_kinds<F16, 128>(s, a, kinds);
-        case 256: return bf16 ? run_kinds<BF16, 256>(s, a, kinds) : run_kinds<F16, 256>(s, a, kinds);
-        default: return bf16 ? run_kinds<BF16, 512>(s, a, kinds) : run_kinds<F16, 512>(s, a, kinds);
+        case 64: return bf16 ? run_kinds<BF16, 64>(s, a, in, kinds) : run_kinds<F16, 64>(s, a, in, kinds);
+        case 128: return bf16 ? run_kinds<BF16, 128>(s, a, in, kinds) : run_kinds<F16, 128>(s, a, in, kinds);
+        case 256: return bf16 ? run_kinds<BF16, 256>(s, a, in, kinds) : run_kinds<F16, 256>(s, a, in, kinds);
+        default: return bf16 ? run_kinds<BF16, 512>(s, a, in, kinds) : run_kinds<F16, 512>(s, a, in, kinds);
     }
 }
 
-hipError_t launch_causal_join(hipStream_t s, const CausalArgs& a, int hd, bool bf16) {
+hipError_t launch_causal_join(hipStream_t s, const CausalArgs& a, const CausalInline& in, int hd, bool bf16) {
     if (!args_ok(a, hd)) return hipErrorInvalidValue;
     if (a.n_joins == 0) return hipSuccess;
     switch (hd) {
-        case 64: return bf16 ? run_join<BF16, 64>(s, a) : run_join<F16, 64>(s, a);
-        case 128: return bf16 ? run_join<BF16, 128>(s, a) : run_join<F16, 128>(s, a);
-        case 256: return bf16 ? run_join<BF16, 256>(s, a) : run_join<F16, 256>(s, a);
-        default: return bf16 ? run_join<BF16, 512>(s, a) : run_join<F16, 512>(s, a);
+        case 64: return bf16 ? run_join<BF16, 64>(s, a, in) : run_join<F16, 64>(s, a, in);
+        case 128: return bf16 ? run_join<BF16, 128>(s, a, in) : run_join<F16, 128>(s, a, in);
+        case 256: return bf16 ? run_join<BF16, 256>(s, a, in) : run_join<F16, 256>(s, a, in);
+        default: return bf16 ? run_join<BF16, 512>(s, a, in) : run_join<F16, 512>(s, a, in);
     }
 }
 

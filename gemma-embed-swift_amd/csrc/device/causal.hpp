@@ -7,9 +7,11 @@
 
 namespace ge {
 
-// Stacked rows of a wide item: 32 a wave, or a pair of waves at head dim 512.
+// Items by the stacked rows they take: wide ones share each key block between the waves' rows, narrow ones
+// have up to 32 rows and a key block a wave.
+enum CausalKind { kCausalWide = 1, kCausalNarrow = 2 };
 constexpr int causal_wide_rows(int hd) { return hd > 256 ? 64 : 128; }
-constexpr int kCausalNarrowRows = 32;  // of a narrow item, whose waves split the keys
+constexpr int kCausalNarrowRows = 32;
 constexpr uint32_t kDirect = 0xffffffffu;
 // Workgroups of a launch: HIP's grid counts work-items in 32 bits.
 constexpr uint64_t kCausalMaxGroups = (uint64_t(1) << 32) / 256 - 1;
@@ -35,23 +37,33 @@ struct CausalJoin {
 struct CausalArgs {
     const uint16_t *q, *k, *v, *prefix_k, *prefix_v;
     uint16_t* out;
-    const CausalItem* items;
+    const CausalItem* items;  // null: in CausalInline, as the joins
     const CausalJoin* joins;
     float* part_o;    // fp32 [kv_heads][part_rows][head_dim], unnormalised
     float2* part_ml;  // [kv_heads][part_rows]: running maximum (log2) and sum
     int64_t q_stride, k_stride, v_stride, out_stride;  // elements from one row to the next
     size_t part_rows;
     int n_items, n_joins;
+    int join_rows;  // the most rows of a join
     int group, kv_heads, window;  // window 0: none
     float c;                      // |scale| log2(e)
     uint32_t q_flip;              // the sign bits of two values where the scale is negative
 };
 
+// The lists of a call that has few of both, among the kernel's arguments: a workgroup finds its item with
+// them instead of after a second read over the bus.
+constexpr int kCausalInlineItems = 48, kCausalInlineJoins = 40;
+struct CausalInline {
+    CausalItem items[kCausalInlineItems];
+    CausalJoin joins[kCausalInlineJoins];
+};
+static_assert(sizeof(CausalArgs) + sizeof(CausalInline) <= 4096, "kernel arguments");
+
 // Head dims 64, 128, 256 and 512.
 bool causal_head_dim_ok(int hd);
-// kinds: 1 wide items only, 2 narrow only, 3 both.
-hipError_t launch_causal(hipStream_t s, const CausalArgs& a, int hd, bool bf16, int kinds);
-hipError_t launch_causal_join(hipStream_t s, const CausalArgs& a, int hd, bool bf16);
+// kinds: the CausalKind of the items.
+hipError_t launch_causal(hipStream_t s, const CausalArgs& a, const CausalInline& in, int hd, bool bf16, int kinds);
+hipError_t launch_causal_join(hipStream_t s, const CausalArgs& a, const CausalInline& in, int hd, bool bf16);
 // Dynamic LDS limits; once per device.
 hipError_t causal_configure();
 

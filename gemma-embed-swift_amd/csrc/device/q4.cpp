@@ -34,7 +34,8 @@ void product(ge_ctx* c, const ge_q4_matrix* w, const ge_q4_matrix* up, const voi
         fail(GE_ERR_INVALID, "4-bit product: x and y, 16-byte aligned");
     Q4Args a{w->m, up ? up->m : Q4Dev{}, static_cast<const uint16_t*>(x), y, rows};
     const Q4Out out = y_type == GE_TYPE_F32 ? kQ4F32 : y_type == GE_TYPE_F16 ? kQ4F16 : kQ4BF16;
-    launch(c, up ? "gemv_q4_geglu" : "gemv_q4", [&] { return launch_gemv_q4(c->stream, a, x_type == GE_TYPE_BF16, up != nullptr, out); });
+    launch(c, up ? "gemv_q4_geglu" : "gemv_q4",
+           [&] { return launch_gemv_q4(c->stream, a, x_type == GE_TYPE_BF16, up != nullptr, out); });
     hip_check(hipStreamSynchronize(c->stream), "hipStreamSynchronize");
 }
 

@@ -35,7 +35,12 @@ class Args(C.Structure):
     _fields_ = [(n, P) for n in ("q", "k", "v", "prefix_k", "prefix_v", "out")] + \
         [("items", C.POINTER(Item)), ("joins", C.POINTER(Join)), ("part_o", P), ("part_ml", P)] + \
         [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + [("part_rows", C.c_size_t)] + \
-        [(n, I) for n in ("n_items", "n_joins", "group", "kv_heads", "window")] + [("c", C.c_float), ("q_flip", C.c_uint32)]
+        [(n, I) for n in ("n_items", "n_joins", "join_rows", "group", "kv_heads", "window")] + [("c", C.c_float), ("q_flip", C.c_uint32)]
+
+
+class Inline(C.Structure):
+    """CausalInline: the lists of a call that has few of both"""
+    _fields_ = [("items", Item * 48), ("joins", Join * 40)]
 
 
 @pytest.fixture(scope="module")
@@ -60,12 +65,15 @@ class Call:
         def on_launch(name, args):
             try:
                 name, a = name.decode(), C.cast(args[0], C.POINTER(Args))[0]
+                few = C.cast(args[1], C.POINTER(Inline))[0]
                 self.names.append(name)
                 self.args = {f: getattr(a, f) for f, _ in Args._fields_ if f not in ("items", "joins")}
                 if "causal_join_kernel" in name:
-                    self.joins = [Join.from_buffer_copy(a.joins[i]) for i in range(a.n_joins)]
+                    assert bool(a.joins) == (a.n_joins > 40 or a.n_items > 48)
+                    self.joins = [Join.from_buffer_copy((a.joins or few.joins)[i]) for i in range(a.n_joins)]
                 else:
-                    self.items = [Item.from_buffer_copy(a.items[i]) for i in range(a.n_items)]
+                    assert bool(a.items) == (a.n_joins > 40 or a.n_items > 48)
+                    self.items = [Item.from_buffer_copy((a.items or few.items)[i]) for i in range(a.n_items)]
             except BaseException as e:  # noqa: BLE001
                 self.error = self.error or e
         self.callback = LAUNCH(on_launch)
@@ -103,6 +111,7 @@ def visible(i, q_len, kv_len, prefix, window):
 def covered(got, seqs, heads, kv_heads, hd, window, prefix):
     """Every row's visible keys are in its parts exactly once, and every row is written exactly once."""
     group, wide = heads // kv_heads, 64 if hd > 256 else 128
+    assert got.args["join_rows"] == max([j.n_rows for j in got.joins], default=0)
     part = {}  # partial row -> (q token, group row, prefix keys, own keys)
     written, longest = {}, 0
 
@@ -266,7 +275,7 @@ def test_refused_pointers(ctx, memory):
 def test_a_failed_call_leaves_nothing_in_flight(ctx, memory):
     """The pinned lists and the partial rows are the next call's: a failing call has waited."""
     seqs = [(0, 1, 0, 9000)]
-    for name in ("hipStreamSynchronize",):
+    for name in ("hipStreamSynchronize", "kernel:causal_kernel", "kernel:causal_join_kernel"):
         lib.host_hip_fail(name.encode(), 1)
         with pytest.raises(ge.GemmaEmbedError) as e:
             call(ctx, memory, seqs, 2, 1, 128)
