@@ -10,9 +10,8 @@ namespace ge {
 // A Q4_0 or Q4_1 matrix in device memory, in tiles of 16 rows by 128 columns (four groups of 32), rows
 // and columns padded with zero weights. Tile t of row block b at index b * (cols_pad / 128) + t:
 //   q: 64 lanes x 4 dwords. Lane l's dword g holds row l % 16, columns 32 g + 8 (l / 16) + [0, 8) of the
-//     tile: its A operand of one v_mfma_f32_16x16x32. Column 2 i at nibble i, 2 i + 1 at nibble 4 + i.
-//   d (and m of Q4_1, w = d q + m; Q4_0 has w = d (q - 8)): fp16 [4 row quads][4 groups][4 rows], the
-//     order of a lane's accumulators (rows 4 (l / 16) + [0, 4)).
+//     tile: its B operand of one v_mfma_f32_16x16x32. Column 2 i at nibble i, 2 i + 1 at nibble 4 + i.
+//   d (and m of Q4_1, w = d q + m; Q4_0 has w = d (q - 8)): fp16 [16 rows][4 groups].
 struct Q4Dev {
     int rows = 0, cols = 0, tiles = 0;  // tiles: column tiles of a row block
     uint32_t* q = nullptr;

@@ -2,7 +2,8 @@
 
 Tolerance. Weights and inputs are exact and products of them exact in fp32 sums; a group's 32 products, its
 scale and the sum over the groups each round at 2^-24 of the running magnitude: at most (32 + 2 + K / 32) steps of
-2^-24 of sum_k |x| (|d| (|q| + 8) + |m|), then half a step of y's type. The GeGLU form adds the gate's slope (at most
+2^-24 of sum_k |x| (|d| (q + 8) + |m|), then half a step of y's type. With bf16 x the products are of 16 + q, which
+the group's sum then starts from -24 sum_k x or has taken off m: magnitudes up to |d| (q + 40) + |m|. The GeGLU form adds the gate's slope (at most
 1.13) and gelu_tanh's own error, a few fp32 steps of its argument's exponent (8 covers exp2 and the reciprocal)."""
 import math
 
@@ -34,7 +35,7 @@ def to_float(b, kind):
 
 
 def matrix(rng, kind, rows, cols):
-    """(GGUF blocks, float64 weights, float64 |d| (|q| + 8) + |m|)."""
+    """(GGUF blocks, float64 weights, float64 |d| (q + 8) + |m|, float64 |d|)."""
     n = rows * cols // 32
     q = rng.integers(0, 16, (n, 32))
     d = (rng.standard_normal(n) * 0.02).astype(np.float16)
@@ -46,10 +47,10 @@ def matrix(rng, kind, rows, cols):
         m = (rng.standard_normal(n) * 0.1).astype(np.float16)
         blocks[:, 2:4] = m.view(np.uint8).reshape(-1, 2)
         m = m.astype(np.float64)[:, None]
-        w, size = d * q + m, np.abs(d) * q + np.abs(m)
+        w, size = d * q + m, np.abs(d) * (q + 8) + np.abs(m)
     else:
         w, size = d * (q - 8), np.abs(d) * (q + 8)
-    return blocks, w.reshape(rows, cols), size.reshape(rows, cols)
+    return blocks, w.reshape(rows, cols), size.reshape(rows, cols), np.repeat(np.abs(d), 32, 1).reshape(rows, cols)
 
 
 def gelu(x):
@@ -71,7 +72,7 @@ def product(ctx, kind, m, rows, cols, x_kind, y_kind, geglu=False, seed=0, edit=
         edit(x)
     dtype = np.float32 if y_kind == F32 else np.uint16
     before = rng.integers(0, 100, m * rows + 64).astype(dtype)  # 64 elements past the end stay
-    handles = [ctx.q4_create(b, kind, rows, cols) for b, _, _ in mats]
+    handles = [ctx.q4_create(b, kind, rows, cols) for b, *_ in mats]
     px, py = ctx.alloc(max(x.nbytes, 16)), ctx.alloc(before.nbytes)
     ctx.upload(px, x)
     ctx.upload(py, before)
@@ -83,8 +84,8 @@ def product(ctx, kind, m, rows, cols, x_kind, y_kind, geglu=False, seed=0, edit=
         ctx.q4_destroy(h)
     assert np.array_equal(raw[m * rows:], before[m * rows:])
     f = to_float(x, x_kind)
-    y, got = [f @ w.T for _, w, _ in mats], to_float(raw[:m * rows], y_kind).reshape(m, rows)
-    err = [(34 + cols / 32) * 2.0 ** -24 * (np.abs(f) @ s.T) for _, _, s in mats]
+    y, got = [f @ w.T for _, w, *_ in mats], to_float(raw[:m * rows], y_kind).reshape(m, rows)
+    err = [(34 + cols / 32) * 2.0 ** -24 * (np.abs(f) @ (s + 32 * d * (x_kind == BF16)).T) for _, _, s, d in mats]
     if geglu:
         g = gelu(y[0])
         want = g * y[1]
@@ -149,7 +150,7 @@ def test_a_rows_bits_do_not_depend_on_its_neighbours(ctx):
 
     def last(n):
         rng = np.random.default_rng(5)
-        blocks, _, _ = matrix(rng, ge.GE_TYPE_Q4_0, 96, 1152)
+        blocks, *_ = matrix(rng, ge.GE_TYPE_Q4_0, 96, 1152)
         x = to_bits(rng.standard_normal((64, 1152)), F16)[:n]
         h, px, py = ctx.q4_create(blocks, ge.GE_TYPE_Q4_0, 96, 1152), ctx.alloc(x.nbytes), ctx.alloc(n * 96 * 4)
         ctx.upload(px, x)
