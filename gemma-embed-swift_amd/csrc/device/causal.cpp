@@ -11,7 +11,6 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
-#include <functional>
 #include <vector>
 
 #include "causal.hpp"
@@ -25,91 +24,98 @@ constexpr int64_t kSplitMinKeys = 128;
 constexpr int64_t kMaxRows = int64_t(1) << 30, kMaxStride = int64_t(1) << 24;
 
 struct Tile {
-    uint32_t row0, n_rows, part;
-    int64_t lo, hi;  // visible keys of its rows
+    uint32_t base, row0, n_rows, part;
+    int32_t lo, hi;  // visible keys of its rows
     uint32_t splits;
 };
 
+// Rows of one sequence, or of a run of them, against one source of keys.
 struct Base {
-    uint32_t q_token, key0, source;
-    int64_t tokens, keys, shift;
+    uint32_t q_token, key0, source, tile0;
+    int64_t keys, shift;
     bool direct;  // its rows have no other part
-    std::vector<Tile> tiles;
 };
 
+// What a call does, planned in a few microseconds: a call of a few dozen takes no longer on the GPU.
 struct Plan {
-    std::vector<CausalItem> items;
+    std::vector<Base> bases;
+    std::vector<Tile> tiles;
+    std::vector<uint32_t> order;  // tiles by their items' length, longest first
     std::vector<CausalJoin> joins;
-    size_t part_rows = 0;
-    int kinds = 0;
+    size_t n_items = 0, part_rows = 0;
+    int kinds = 0, group = 1, wide = 0;
 };
 
-Base make_base(uint32_t q_token, int64_t tokens, uint32_t source, uint32_t key0, int64_t keys, int64_t shift, int group,
-               int window, int wide, bool direct) {
-    Base b{q_token, key0, source, tokens, keys, shift, direct, {}};
-    const int64_t rows = tokens * group;
-    for (int64_t r = 0; r < rows; r += wide) {
-        const int64_t n = std::min<int64_t>(wide, rows - r), i0 = r / group, i1 = (r + n - 1) / group;
-        Tile t{uint32_t(r), uint32_t(n), 0, 0, 0, 0};
-        t.lo = window ? std::max<int64_t>(0, i0 + shift - window + 1) : 0;
-        t.hi = std::min(keys, i1 + shift + 1);
-        if (t.hi <= t.lo) t.lo = t.hi = 0;
-        b.tiles.push_back(t);
-    }
-    return b;
-}
-
-int64_t splits_of(const Tile& t, int64_t limit) { return (t.hi - t.lo + limit - 1) / limit; }
+int64_t divide_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool narrow(const Tile& t) { return t.n_rows <= uint32_t(kCausalNarrowRows); }
 // 64-key steps keep the parts' blocks whole.
-int64_t step_of(const Tile& t, int64_t splits) { return splits ? (t.hi - t.lo + splits * 64 - 1) / (splits * 64) * 64 : 0; }
+int32_t step_of(const Tile& t) { return t.splits > 1 ? int32_t(divide_up(t.hi - t.lo, int64_t(t.splits) * 64) * 64) : t.hi - t.lo; }
+
+void add_base(Plan& p, uint32_t q_token, int64_t tokens, uint32_t source, uint32_t key0, int64_t keys, int64_t shift, int window,
+              bool direct) {
+    const uint32_t at = uint32_t(p.bases.size());
+    p.bases.push_back(Base{q_token, key0, source, uint32_t(p.tiles.size()), keys, shift, direct});
+    const int64_t rows = tokens * p.group;
+    for (int64_t r = 0; r < rows; r += p.wide) {
+        const int64_t n = std::min<int64_t>(p.wide, rows - r);
+        int64_t lo = 0, hi = keys;
+        if (window) lo = std::max<int64_t>(0, r / p.group + shift - window + 1);
+        if (shift < keys) hi = std::min(keys, (r + n - 1) / p.group + shift + 1);
+        if (hi <= lo) lo = hi = 0;
+        p.tiles.push_back(Tile{at, uint32_t(r), uint32_t(n), 0, int32_t(lo), int32_t(hi), 0});
+    }
+}
 
 // The most keys of an item. Splitting fills the GPU and evens the items out, and costs the parts' rows
 // (written, and read by the joining launch). Of no split and splits into about 1, 1.5, 2 and 3 items a CU the
 // one whose estimate is least, in microseconds: a key of an item of head dim 128 takes 0.025 with one
 // workgroup on a CU and 0.6 of that each with two (narrow items, which wait for memory, gain nothing by
 // pairs), an item 7 besides its keys, a joining launch 5 and 1 for 3 MB of parts. Calls of few or many
-// items (under 64 keys each, four a CU unsplit) are not split.
-int64_t split_limit(const std::vector<Base>& bases, const ge_attention_shape& s) {
+// items (under 128 keys each, four a CU unsplit) are not split. Measured, us a call unsplit / 1 / 1.5 / 2 / 3
+// items a CU: one token over 20000 keys (32 heads of 128 over 8) 178 / 35 / 38 / 41 / 46, 48 tokens over 100
+// to 8000 189 / 188 / 165 / 166 / 165, 128 texts over a prefix of 8192 (3 heads of 256) 332 / 200 / 178 / 215 /
+// 203, one prompt of 2048 (32 heads of 128) 67 / 67 / 78 / 83 / 84.
+int64_t split_limit(const Plan& p, int kv_heads, int head_dim) {
     constexpr int kBins = 64;
-    const double key_us = 0.025 * s.head_dim / 128;
-    int64_t total = 0, longest = 0, tiles = 0, wide_keys = 0;
-    for (const Base& b : bases)
-        for (const Tile& t : b.tiles) {
-            total += t.hi - t.lo;
-            if (t.n_rows > uint32_t(kCausalNarrowRows)) wide_keys += t.hi - t.lo;
-            longest = std::max(longest, t.hi - t.lo);
-            tiles++;
-        }
-    if (longest <= kSplitMinKeys || tiles * s.kv_heads >= 4 * kCus) return std::max<int64_t>(longest, 64);
-    const double pair = 2 * wide_keys >= total ? 0.6 : 1.0;
+    const float key_us = 0.025f * float(head_dim) / 128;
+    int64_t total = 0, longest = 0, wide_keys = 0;
+    for (const Tile& t : p.tiles) {
+        const int64_t n = t.hi - t.lo;
+        total += n;
+        wide_keys += narrow(t) ? 0 : n;
+        longest = std::max(longest, n);
+    }
+    if (longest <= kSplitMinKeys || int64_t(p.tiles.size()) * kv_heads >= 4 * kCus) return std::max<int64_t>(longest, 64);
+    const float pair = 2 * wide_keys >= total ? 0.6f : 1.0f;
     int64_t best = longest;
-    double best_us = 1e300;
-    for (const double per_cu : {0.0, 1.0, 1.5, 2.0, 3.0}) {
+    float best_us = 1e30f;
+    for (const float per_cu : {0.0f, 1.0f, 1.5f, 2.0f, 3.0f}) {
         const int64_t limit =
-            per_cu == 0.0 ? longest : std::max(kSplitMinKeys, (int64_t(double(total * s.kv_heads) / (per_cu * kCus)) + 63) / 64 * 64);
-        if (per_cu != 0.0 && limit >= longest) continue;
+            per_cu == 0.0f ? longest : std::max(kSplitMinKeys, (int64_t(float(total * kv_heads) / (per_cu * kCus)) + 63) / 64 * 64);
+        if (per_cu != 0.0f && limit >= longest) continue;
         // items by their keys, in kBins steps
-        int64_t count[kBins] = {}, items = 0, parts = 0;
-        const int64_t top = std::min(limit, longest);
-        for (const Base& b : bases)
-            for (const Tile& t : b.tiles) {
-                const int64_t n = splits_of(t, limit);
-                if (!n) continue;
-                count[std::min<int64_t>(kBins - 1, (t.hi - t.lo) / n * kBins / (top + 1))] += n * s.kv_heads;
-                items += n * s.kv_heads;
-                if (!b.direct || n > 1) parts += n * t.n_rows;
-            }
+        int count[kBins] = {}, items = 0;
+        int64_t parts = 0;
+        const float inv = 1.0f / float(limit), to_bin = kBins / float(limit + 1);
+        for (const Tile& t : p.tiles) {
+            const int n = t.hi - t.lo;
+            if (!n) continue;
+            const int k = n <= limit ? 1 : int(std::ceil(float(n) * inv));
+            count[std::min(kBins - 1, int(float(n) / float(k) * to_bin))] += k * kv_heads;
+            items += k * kv_heads;
+            if (k > 1 || !p.bases[t.base].direct) parts += int64_t(k) * t.n_rows;
+        }
         // at least the work at the rate of full CUs, and, with the items started longest first, two a CU, the
         // end of the first of each round's first and second half
-        double us = double(total) * double(s.kv_heads) * key_us * pair / kCus;
-        int64_t k = 0, seen = 0;
+        float us = float(total) * float(kv_heads) * key_us * pair / kCus;
+        int k = 0, seen = 0;
         for (int bin = kBins - 1; bin >= 0; bin--) {
             seen += count[bin];
             for (; k < seen; k += kCus)
-                us = std::max(us, (double(k / (2 * kCus)) * 2 * pair + (k / kCus % 2 ? 2 * pair : 1.0)) * key_us * double(top) * (bin + 1) / kBins);
+                us = std::max(us, (float(k / (2 * kCus)) * 2 * pair + (k / kCus % 2 ? 2 * pair : 1.0f)) * key_us * float(limit) * float(bin + 1) / kBins);
         }
-        us += 7.0 * double((items + 2 * kCus - 1) / (2 * kCus));
-        if (parts) us += 5.0 + double(parts) * s.kv_heads * s.head_dim * 8 / 3e6;
+        us += 7.0f * float((items + 2 * kCus - 1) / (2 * kCus));
+        if (parts) us += 5.0f + float(parts) * float(kv_heads) * float(head_dim) * 8 / 3e6f;
         if (us < best_us) {
             best_us = us;
             best = limit;
@@ -119,8 +125,11 @@ int64_t split_limit(const std::vector<Base>& bases, const ge_attention_shape& s)
 }
 
 Plan make_plan(const ge_attention_shape& s, const ge_attention_seq* seqs, int n_seqs, int64_t prefix_len) {
-    const int group = s.heads / s.kv_heads, wide = causal_wide_rows(s.head_dim);
-    std::vector<Base> bases;
+    Plan p;
+    p.group = s.heads / s.kv_heads;
+    p.wide = causal_wide_rows(s.head_dim);
+    p.bases.reserve(size_t(n_seqs) * (prefix_len ? 2 : 1));
+    p.tiles.reserve(size_t(n_seqs) * 2 + 64);
     struct Use {
         int own = -1, prefix = -1;
         int64_t prefix_row = 0;  // the sequence's first row in its prefix base
@@ -129,9 +138,8 @@ Plan make_plan(const ge_attention_shape& s, const ge_attention_seq* seqs, int n_
     for (int i = 0; i < n_seqs; i++) {
         const ge_attention_seq& q = seqs[i];
         if (!q.q_len || (prefix_len && !q.kv_len)) continue;
-        use[size_t(i)].own = int(bases.size());
-        bases.push_back(make_base(q.q_start, q.q_len, 0, q.kv_start, q.kv_len, int64_t(q.kv_len) - q.q_len, group, s.window,
-                                  wide, prefix_len == 0));
+        use[size_t(i)].own = int(p.bases.size());
+        add_base(p, q.q_start, q.q_len, 0, q.kv_start, q.kv_len, int64_t(q.kv_len) - q.q_len, s.window, prefix_len == 0);
     }
     for (int i = 0; prefix_len && i < n_seqs;) {
         if (!seqs[i].q_len) {
@@ -143,60 +151,65 @@ Plan make_plan(const ge_attention_shape& s, const ge_attention_seq* seqs, int n_
         int64_t tokens = seqs[i].q_len, shift = prefix_len + seqs[i].kv_len - int64_t(seqs[i].q_len);
         bool alone = seqs[i].kv_len == 0;
         int j = i + 1;
-        use[size_t(i)].prefix = int(bases.size());
+        use[size_t(i)].prefix = int(p.bases.size());
         if (whole(seqs[i])) {
             shift = kMaxRows;
             for (; j < n_seqs && whole(seqs[j]) && seqs[j].q_start == seqs[i].q_start + uint64_t(tokens); j++) {
-                use[size_t(j)].prefix = int(bases.size());
-                use[size_t(j)].prefix_row = tokens * group;
+                use[size_t(j)].prefix = int(p.bases.size());
+                use[size_t(j)].prefix_row = tokens * p.group;
                 tokens += seqs[j].q_len;
                 alone = alone && seqs[j].kv_len == 0;
             }
         }
-        bases.push_back(make_base(seqs[i].q_start, tokens, 1, 0, prefix_len, shift, group, s.window, wide, alone));
+        add_base(p, seqs[i].q_start, tokens, 1, 0, prefix_len, shift, s.window, alone);
         i = j;
     }
 
-    const int64_t limit = split_limit(bases, s);
-    Plan p;
-    for (Base& b : bases)
-        for (Tile& t : b.tiles) {
-            const int64_t splits = splits_of(t, limit), step = step_of(t, splits);
-            const bool narrow = t.n_rows <= uint32_t(kCausalNarrowRows), direct = b.direct && splits <= 1;
-            t.part = uint32_t(p.part_rows);
-            for (int64_t k = t.lo; k < t.hi || (direct && t.splits == 0); k += step) {
-                p.items.push_back(CausalItem{b.q_token, t.row0, t.n_rows, b.key0, uint32_t(k), uint32_t(std::min(k + step, t.hi)),
-                                             int32_t(b.shift), direct ? kDirect : uint32_t(p.part_rows), b.source, narrow});
-                p.kinds |= narrow ? kCausalNarrow : kCausalWide;
-                t.splits++;
-                if (direct) break;
-                p.part_rows += t.n_rows;
-            }
+    const int64_t limit = split_limit(p, s.kv_heads, s.head_dim);
+    // The longest items first, so that the last ones to start are short: tiles by their items' keys (a wide
+    // item's weighing four times), in 256 steps.
+    constexpr int kSteps = 256;
+    const int64_t heaviest = 4 * std::max<int64_t>(limit, 1);
+    auto place = [&](const Tile& t) { return kSteps - 1 - int(int64_t(step_of(t)) * (narrow(t) ? 1 : 4) * (kSteps - 1) / heaviest); };
+    uint32_t first[kSteps + 1] = {};
+    bool joined = false;
+    for (Tile& t : p.tiles) {
+        const bool direct = p.bases[t.base].direct;
+        t.splits = uint32_t(divide_up(t.hi - t.lo, limit));
+        t.part = uint32_t(p.part_rows);
+        if (direct && t.splits <= 1) {
+            t.splits = 1;  // also where its rows see nothing: they are written
+        } else {
+            joined = true;
+            p.part_rows += size_t(t.splits) * t.n_rows;
             if (p.part_rows >= kDirect) fail(GE_ERR_INVALID, "attention: the call's rows and keys are too many for one call");
         }
-    // The longest items first, so the last ones to start are short.
-    std::stable_sort(p.items.begin(), p.items.end(), [](const CausalItem& a, const CausalItem& b) {
-        return (a.k_hi - a.k_lo) * (a.narrow ? 1 : 4) > (b.k_hi - b.k_lo) * (b.narrow ? 1 : 4);
-    });
+        p.n_items += t.splits;
+        if (t.splits) p.kinds |= narrow(t) ? kCausalNarrow : kCausalWide;
+        first[place(t) + 1]++;
+    }
+    for (int i = 0; i < kSteps; i++) first[i + 1] += first[i];
+    p.order.resize(p.tiles.size());
+    for (size_t i = 0; i < p.tiles.size(); i++) p.order[first[place(p.tiles[i])]++] = uint32_t(i);
 
-    for (int i = 0; i < n_seqs; i++) {
+    if (joined) p.joins.reserve(size_t(n_seqs) + p.tiles.size());
+    for (int i = 0; joined && i < n_seqs; i++) {
         const Use& u = use[size_t(i)];
-        const Base* const side[2] = {u.own >= 0 ? &bases[size_t(u.own)] : nullptr,
-                                     u.prefix >= 0 ? &bases[size_t(u.prefix)] : nullptr};
-        const int64_t first[2] = {0, u.prefix_row}, rows = int64_t(seqs[i].q_len) * group;
+        const Base* const side[2] = {u.own >= 0 ? &p.bases[size_t(u.own)] : nullptr, u.prefix >= 0 ? &p.bases[size_t(u.prefix)] : nullptr};
+        const int64_t start[2] = {0, u.prefix_row}, rows = int64_t(seqs[i].q_len) * p.group;
         for (int64_t r = 0; r < rows;) {
             CausalJoin j{seqs[i].q_start, uint32_t(r), 0, {}, {}, {}};
             int64_t end = rows;
             bool written = false;
             for (int k = 0; k < 2; k++) {
                 if (!side[k]) continue;
-                const int64_t at = first[k] + r;
-                const Tile& t = side[k]->tiles[size_t(at / wide)];
+                const int64_t at = start[k] + r;
+                const Tile& t = p.tiles[side[k]->tile0 + size_t(at / p.wide)];
                 j.part[k] = t.part + uint32_t(at - t.row0);
                 j.stride[k] = t.n_rows;
                 j.splits[k] = t.splits;
-                end = std::min(end, int64_t(t.row0) + t.n_rows - first[k]);
-                written = written || (side[k]->direct && t.splits <= 1);
+                end = std::min(end, int64_t(t.row0) + t.n_rows - start[k]);
+                written = written || (side[k]->direct && t.splits == 1);
             }
             j.n_rows = uint32_t(end - r);
             if (!written) p.joins.push_back(j);
@@ -204,6 +217,21 @@ Plan make_plan(const ge_attention_shape& s, const ge_attention_seq* seqs, int n_
         }
     }
     return p;
+}
+
+// The plan's items, n_items of them.
+void write_items(const Plan& p, CausalItem* out) {
+    for (const uint32_t i : p.order) {
+        const Tile& t = p.tiles[i];
+        const Base& b = p.bases[t.base];
+        const int32_t step = step_of(t);
+        for (uint32_t s = 0; s < t.splits; s++) {
+            const int32_t k = t.lo + int32_t(s) * step;
+            const bool direct = b.direct && t.splits == 1;
+            *out++ = CausalItem{b.q_token, t.row0, t.n_rows, b.key0, uint32_t(std::min(k, t.hi)), uint32_t(std::min(k + step, t.hi)),
+                                int32_t(b.shift), direct ? kDirect : t.part + s * t.n_rows, b.source, narrow(t)};
+        }
+    }
 }
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -253,14 +281,14 @@ void attend(ge_ctx* c, const ge_attention_shape* shape, const void* q, const voi
         fail(GE_ERR_INVALID, "attention: buffers are 16-byte aligned");
 
     const Plan p = make_plan(s, seqs, n_seqs, prefix_len);
-    if (p.items.size() * uint64_t(s.kv_heads) > kCausalMaxGroups || p.joins.size() * uint64_t(s.kv_heads) > kCausalMaxGroups)
+    if (p.n_items * uint64_t(s.kv_heads) > kCausalMaxGroups || p.joins.size() * uint64_t(s.kv_heads) > kCausalMaxGroups)
         fail(GE_ERR_INVALID, "attention: the call's rows and keys are too many for one call");
     OpTemps temps(c);
     CausalInline in;
-    const bool few = p.items.size() <= size_t(kCausalInlineItems) && p.joins.size() <= size_t(kCausalInlineJoins);
-    const size_t item_bytes = (p.items.size() * sizeof(CausalItem) + 255) / 256 * 256;
+    const bool few = p.n_items <= size_t(kCausalInlineItems) && p.joins.size() <= size_t(kCausalInlineJoins);
+    const size_t item_bytes = (p.n_items * sizeof(CausalItem) + 255) / 256 * 256;
     unsigned char* const lists = few ? nullptr : op_lists(c, item_bytes + p.joins.size() * sizeof(CausalJoin));
-    std::copy(p.items.begin(), p.items.end(), few ? in.items : reinterpret_cast<CausalItem*>(lists));
+    write_items(p, few ? in.items : reinterpret_cast<CausalItem*>(lists));
     std::copy(p.joins.begin(), p.joins.end(), few ? in.joins : reinterpret_cast<CausalJoin*>(lists + item_bytes));
     const size_t o_at = temps.reserve(p.part_rows * size_t(kv_width) * 4);
     const size_t ml_at = temps.reserve(p.part_rows * size_t(s.kv_heads) * 8);
@@ -282,7 +310,7 @@ void attend(ge_ctx* c, const ge_attention_shape* shape, const void* q, const voi
     a.v_stride = s.v_stride;
     a.out_stride = s.out_stride;
     a.part_rows = p.part_rows;
-    a.n_items = int(p.items.size());
+    a.n_items = int(p.n_items);
     a.n_joins = int(p.joins.size());
     for (const CausalJoin& j : p.joins) a.join_rows = std::max(a.join_rows, int(j.n_rows));
     a.group = s.heads / s.kv_heads;
