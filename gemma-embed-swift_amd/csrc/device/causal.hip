@@ -278,6 +278,55 @@ struct Rows {
             if (half == 0 && d0 == 0) a.part_ml[at] = float2{m, l};
         }
     }
+
+    // The same through this wave's slice of LDS, where a row's pieces come together: whole 16-byte pieces of a
+    // row go out side by side. Straight from the accumulators a store's lanes are all in different rows, and
+    // the stores of an item of head dim 256 took 2.4 to 3.4 us.
+    template <int SLICE>
+    __device__ __forceinline__ void finish_rows(const CausalArgs& a, const CausalItem& it, int kvh, int r0, int n, int lane,
+                                                unsigned char* slice) {
+        const int row = lane & 31, half = lane >> 5;
+        if (it.part == kDirect) {
+            constexpr int ROW = DT * 64, P = ROW / 16;  // bytes and pieces of a row
+            static_assert(32 * ROW <= SLICE, "a slice holds the rows");
+            const uint32_t r = uint32_t(r0 + min(row, n - 1)), g = uint32_t(a.group);
+            const size_t at = ((size_t(it.q_token) + r / g) * size_t(a.out_stride) + (size_t(kvh) * g + r % g) * HD + d0 * 32) * 2;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<u32x2*>(slice + row * ROW + (((4 * d + e / 4) ^ (row & (P - 1))) * 16) + half * 8) =
+                        u32x2{T::pack(o[d][e] * inv, o[d][e + 1] * inv), T::pack(o[d][e + 2] * inv, o[d][e + 3] * inv)};
+#pragma unroll
+            for (int i = 0; i < 32 * P / 64; i++) {
+                const int x = (i * 64 + lane) / P, c = (i * 64 + lane) % P;
+                const size_t row_at = size_t(uint32_t(__shfl(int(uint32_t(at)), x, 64))) | size_t(uint32_t(__shfl(int(uint32_t(at >> 32)), x, 64))) << 32;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(slice + x * ROW + ((c ^ (x & (P - 1))) * 16));
+                if (x < n) *reinterpret_cast<u32x4*>(reinterpret_cast<unsigned char*>(a.out) + row_at + c * 16) = v;
+            }
+        } else {
+            constexpr int D = 32 * DT * 128 <= SLICE ? DT : SLICE / (32 * 128), ROW = D * 128, P = ROW / 16;  // D dim tiles at a time
+            static_assert(DT % D == 0, "whole passes");
+            const size_t at = size_t(kvh) * a.part_rows + it.part + uint32_t(r0 - int(it.row0));
+            if (lane < n && d0 == 0) a.part_ml[at + row] = float2{m, l};
+#pragma unroll
+            for (int p = 0; p < DT; p += D) {
+#pragma unroll
+                for (int d = 0; d < D; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<float4_t*>(slice + row * ROW + (((8 * d + e / 2 + half) ^ (row & 31 & (P - 1))) * 16)) =
+                            float4_t{o[p + d][e], o[p + d][e + 1], o[p + d][e + 2], o[p + d][e + 3]};
+#pragma unroll 4
+                for (int i = 0; i < 32 * P / 64; i++) {
+                    const int x = (i * 64 + lane) / P, c = (i * 64 + lane) % P;
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(slice + x * ROW + ((c ^ (x & 31 & (P - 1))) * 16));
+                    if (x < n) *reinterpret_cast<u32x4*>(a.part_o + (at + x) * HD + (d0 + p) * 32 + c * 4) = v;
+                }
+            }
+        }
+    }
 };
 
 // A hidden key's P is 0, which its V, where that is infinite or NaN, would still turn into NaN. Only blocks
@@ -409,9 +458,11 @@ struct Wide {
                 blk.product(w, at + Kv::kBytes, lane, p);
             }
         }
+        __syncthreads();  // no one reads K and V any more
         if (n > 0) {
+            constexpr int kSlice = kLds / NW;
             w.l = sum_over_halves(w.l);
-            w.finish(a, it, kvh, r0, n, lane);
+            w.template finish_rows<kSlice>(a, it, kvh, r0, n, lane, lds + wave * kSlice);
         }
         held.share(lds);
         if (n > 0 && held.any) held.add(a, it, kvh, r0, n, w.d0 * 32, w.DT * 32);
