@@ -374,12 +374,17 @@ struct HeldBack {
         any = (flag[0] | flag[1] | flag[2] | flag[3]) != 0;
         __syncthreads();
     }
-    // Rows [r0, r0 + n), dims [d0, d0 + dims), which this wave has stored.
-    __device__ __forceinline__ static void add(const CausalArgs& a, const CausalItem& it, int kvh, int r0, int n, int d0, int dims) {
+    // Rows [r0, r0 + n), dims [d0, d0 + dims), which this wave has stored; bk: the item's key blocks.
+    __device__ __forceinline__ void add(const CausalArgs& a, const CausalItem& it, int kvh, int r0, int n, int d0, int dims, int bk) const {
         __threadfence();
         const uint16_t* const v = (it.source ? a.prefix_v : a.v) + size_t(kvh) * HD;
         const uint32_t g = uint32_t(a.group);
-        for (uint32_t key = it.k_lo; key < it.k_hi; key++)
+        for (uint32_t key = it.k_lo; key < it.k_hi; key++) {
+            const int kb = int(it.k_lo) + (int(key) - int(it.k_lo)) / bk * bk;
+            if (!mixed(kb, bk)) {
+                key = uint32_t(kb + bk - 1);
+                continue;
+            }
             for (int d = d0 + int(threadIdx.x & 63); d < d0 + dims; d += 64) {
                 const uint16_t x = v[(size_t(it.key0) + key) * size_t(a.v_stride) + d];
                 if (((x & 0x7fffu) + (T::kNonFinite & 0xffffu)) < 0x8000u) continue;
@@ -395,6 +400,7 @@ struct HeldBack {
                     }
                 }
             }
+        }
     }
 };
 
@@ -465,7 +471,7 @@ struct Wide {
             w.template finish_rows<kSlice>(a, it, kvh, r0, n, lane, lds + wave * kSlice);
         }
         held.share(lds);
-        if (n > 0 && held.any) held.add(a, it, kvh, r0, n, w.d0 * 32, w.DT * 32);
+        if (n > 0 && held.any) held.add(a, it, kvh, r0, n, w.d0 * 32, w.DT * 32, BK);
     }
 };
 
@@ -602,7 +608,7 @@ struct Narrow {
         Join::run(w, kw, dims, lane, lds);
         if (kw > 0) return;
         w.finish(a, it, kvh, r0, n, lane);
-        if (held.any) held.add(a, it, kvh, r0, n, w.d0 * 32, w.DT * 32);
+        if (held.any) held.add(a, it, kvh, r0, n, w.d0 * 32, w.DT * 32, BK);
     }
 };
 

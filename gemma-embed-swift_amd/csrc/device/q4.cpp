@@ -55,6 +55,8 @@ int ge_op_q4_create(ge_ctx* c, const void* q4_rows, int32_t type, int32_t rows, 
         if (type != GE_TYPE_Q4_0 && type != GE_TYPE_Q4_1) fail(GE_ERR_INVALID, "4-bit matrix of type %d (Q4_0 or Q4_1)", type);
         if (!q4_rows || !out || rows <= 0 || cols <= 0 || cols % 32)
             fail(GE_ERR_INVALID, "4-bit matrix needs rows > 0 and cols a multiple of 32");
+        if (rows > ge::kQ4MaxWeightRows || cols > ge::kQ4MaxCols)
+            fail(GE_ERR_INVALID, "4-bit matrix of %d x %d (up to %d x %d)", rows, cols, ge::kQ4MaxWeightRows, ge::kQ4MaxCols);
         std::unique_ptr<ge_q4_matrix> m(new ge_q4_matrix);
         w.rows = rows;
         w.cols = cols;

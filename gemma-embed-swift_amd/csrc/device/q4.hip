@@ -318,7 +318,7 @@ hipError_t run_rows(hipStream_t s, const Q4Args& a, bool geglu, Q4Out out) {
 }  // namespace
 
 hipError_t launch_q4_repack(hipStream_t s, const unsigned char* blocks, const Q4Dev& w) {
-    if (w.rows <= 0 || w.cols <= 0 || w.cols % 32 || w.tiles != q4_tiles(w.cols)) return hipErrorInvalidValue;
+    if (w.rows <= 0 || w.cols <= 0 || w.cols % 32 || w.rows > kQ4MaxWeightRows || w.cols > kQ4MaxCols || w.tiles != q4_tiles(w.cols)) return hipErrorInvalidValue;
     const uint64_t n = uint64_t(q4_row_blocks(w.rows)) * uint64_t(w.tiles);
     if (n >= (uint64_t(1) << 32) / 64) return hipErrorInvalidValue;
     launch_kernel(q4_repack_kernel, dim3(uint32_t(n)), dim3(64), 0, s, blocks, w);

@@ -31,8 +31,9 @@ struct Q4Args {
     void* y;            // [rows][w.rows]
     int rows;
 };
-// Rows of x a call takes: 64 a workgroup, in the grid's second dimension.
-constexpr int kQ4MaxRows = 1 << 20;
+// Rows of x a call takes (16 or more a workgroup, in the grid's second dimension), and a matrix's rows and
+// columns (a workgroup a row block, in the first; columns are counted past the end in 32 bits).
+constexpr int kQ4MaxRows = 1 << 19, kQ4MaxWeightRows = 1 << 26, kQ4MaxCols = 1 << 24;
 enum Q4Out { kQ4F32 = 0, kQ4F16 = 1, kQ4BF16 = 2 };
 
 // y[r][n] = sum_k x[r][k] w[n][k], or gelu_tanh(x w^T) * (x up^T) with geglu; x fp16 or (bf16) bfloat16.

@@ -192,7 +192,7 @@ int ge_op_gemm_q8_geglu(ge_ctx* ctx, const ge_q8_matrix* gate, const ge_q8_matri
 
 /* 4-bit weights with a scale for each group of 32 columns, for the products of few rows (a token, a handful
  * of tokens) that are bound by reading the weights. No counterpart in the reference, whose weights are
- * Q8_0. `rows` GGUF rows of `cols` elements in host memory, cols a multiple of 32, any number of rows:
+ * Q8_0. `rows` GGUF rows (up to 2^26) of `cols` elements (a multiple of 32 up to 2^24) in host memory:
  * type GE_TYPE_Q4_0 (18-byte blocks: fp16 d, 16 bytes; w = d (q - 8)) or GE_TYPE_Q4_1 (20-byte blocks: fp16 d
  * and m, 16 bytes; w = d q + m), element j of a block in byte j % 16's low (j < 16) or high nibble. */
 typedef struct ge_q4_matrix ge_q4_matrix;
@@ -201,8 +201,8 @@ int ge_op_q4_destroy(ge_ctx* ctx, ge_q4_matrix* m);
 
 /* y[M][N] = x[M][K] * W^T with W [N][K] in 4 bits: x of x_type GE_TYPE_F16 or GE_TYPE_BF16, y of y_type
  * GE_TYPE_F32, GE_TYPE_F16 or GE_TYPE_BF16, rows back to back, 16-byte aligned. The weights enter as the
- * integers they are and the sums are fp32: y is rounded once, to its type. Any M up to 2^20 (the weights
- * are read once for every 64 rows). */
+ * integers they are and the sums are fp32: y is rounded once, to its type. Any M up to 2^19 (the weights
+ * are read once for every 16, 32 or 64 rows). */
 int ge_op_gemv_q4(ge_ctx* ctx, const ge_q4_matrix* w, const void* x, int32_t x_type, int32_t m, void* y, int32_t y_type);
 /* The same with the geglu epilogue: act[M][F] = gelu_tanh(x * Wg^T) * (x * Wu^T), gate and up of one shape
  * and type. */
@@ -306,8 +306,8 @@ typedef struct ge_attention_seq {
 /* out_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys j that query i of its sequence sees, with the last
  * query at the last key: j <= i + kv_len - q_len and, with a window, j > i + kv_len - q_len - window. So
  * q_len = kv_len is a prompt, a shorter q_len a chunk or (1) the next token over cached keys. A query
- * that sees no key gets zeros. A key no query of a row sees (its score or value infinite or NaN,
- * say) does not reach that row. Rows of out outside the sequences stay as they were. */
+ * that sees no key gets zeros. What a query does not see does not reach its row, infinities and NaN
+ * included. Rows of out outside the sequences stay as they were. */
 int ge_op_attention_causal(ge_ctx* ctx, const ge_attention_shape* shape, const void* q, const void* k, const void* v,
                            const ge_attention_seq* seqs, int32_t n_seqs, void* out);
 

@@ -40,6 +40,14 @@ def test_refused_matrices(ctx, kind, rows, cols):
     assert e.value.code == ge.GE_ERR_INVALID
 
 
+@pytest.mark.parametrize("rows,cols", [((1 << 26) + 1, 32), (1, (1 << 24) + 32)])
+def test_matrices_past_the_limits(ctx, rows, cols):
+    h = C.c_void_p(1)
+    assert lib.ge_op_q4_create(ctx.handle, 16, ge.GE_TYPE_Q4_0, rows, cols, C.byref(h)) == ge.GE_ERR_INVALID and not h.value
+    assert lib.ge_op_q4_create(ctx.handle, None, ge.GE_TYPE_Q4_0, 4, 32, C.byref(h)) == ge.GE_ERR_INVALID
+    assert lib.ge_op_q4_create(ctx.handle, 16, ge.GE_TYPE_Q4_0, 4, 32, None) == ge.GE_ERR_INVALID
+
+
 def test_too_few_bytes(ctx):
     with pytest.raises(ge.GemmaEmbedError):
         ctx.q4_create(np.zeros(20 * 8 - 1, np.uint8), ge.GE_TYPE_Q4_1, 4, 64)
@@ -48,7 +56,7 @@ def test_too_few_bytes(ctx):
 def test_refused_products(ctx, memory, w):
     good = (w, memory, F16, 3, memory, F32)
     ctx.gemv_q4(*good)
-    for i, bad in ((0, None), (1, None), (1, memory + 4), (2, F32), (2, ge.GE_TYPE_Q4_0), (3, -1), (3, (1 << 20) + 1), (4, None),
+    for i, bad in ((0, None), (1, None), (1, memory + 4), (2, F32), (2, ge.GE_TYPE_Q4_0), (3, -1), (3, (1 << 19) + 1), (4, None),
                    (4, memory + 2), (5, ge.GE_TYPE_Q8_0)):
         with pytest.raises(ge.GemmaEmbedError) as e:
             ctx.gemv_q4(*(good[:i] + (bad,) + good[i + 1:]))

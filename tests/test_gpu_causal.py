@@ -315,3 +315,73 @@ def test_a_prompt_in_two_chunks_and_token_by_token(ctx):
     tokens, _ = attend(ctx, [(i, 1, 0, i + 1) for i in range(n)], heads, kv_heads, hd, F16, seed=15)
     a, b, c = (to_float(x[:n], F16) for x in (whole, chunks, tokens))
     assert np.abs(a - b).max() <= 4 * 2.0 ** -11 * np.abs(a).max() and np.abs(a - c).max() <= 4 * 2.0 ** -11 * np.abs(a).max()
+
+
+def test_sequences_share_key_rows(ctx):
+    """Several sequences over the same cached rows."""
+    for layout in LAYOUTS:
+        attend(ctx, [(0, 1, 0, 300), (1, 1, 0, 300), (2, 5, 100, 100), (7, 60, 0, 300)], *layout, F16, seed=16)
+
+
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_offsets_past_32_bits(ctx, prefix):
+    """Key rows 4 MiB apart: byte offsets from 4.0 to 4.7 GB, past 2^32 within the sequences."""
+    heads, kv_heads, hd, stride, start, n = 2, 1, 64, 1 << 21, 970, 150
+    rng = np.random.default_rng(17)
+    k, v = (to_bits(rng.standard_normal((start + n, hd)), F16) for _ in range(2))
+    pk, pv = (to_bits(rng.standard_normal((prefix, hd)), F16) for _ in range(2))
+    q = to_bits(rng.standard_normal((11, heads * hd)), F16)
+    shape = ge.attention_shape(F16, heads, kv_heads, hd, 11, start + n, scale=0.125, k_stride=stride, v_stride=stride)
+    seqs = [(0, 1, start, n), (1, 10, start + 90, 60)]
+    with Buffers(ctx) as b:
+        big = [ctx.alloc((start + n) * stride * 2) for _ in range(2)]
+        b.held += big
+        for p, a in zip(big, (k, v)):
+            for r in range(start, start + n):
+                ctx.upload(p + r * stride * 2, a[r])
+        small = []
+        for a in (pk, pv):
+            p = ctx.alloc(max(prefix, 1) * stride * 2)
+            b.held.append(p)
+            for r in range(prefix):
+                ctx.upload(p + r * stride * 2, a[r])
+            small.append(p)
+        out, pq = b.put(np.zeros((11, heads * hd), np.uint16)), b.put(q)
+        if prefix:
+            ctx.attention_prefix(shape, pq, small[0], small[1], prefix, big[0], big[1], seqs, out)
+        else:
+            ctx.attention_causal(shape, pq, big[0], big[1], seqs, out)
+        got = to_float(ctx.download(out, (11, heads * hd), np.uint16), F16)
+    for q0, m, k0, length in seqs:
+        ks, vs = (to_float(np.concatenate([x, y[k0:k0 + length]]), F16).reshape(-1, 1, hd) for x, y in ((pk, k), (pv, v)))
+        o, mag = reference(to_float(q[q0:q0 + m], F16).reshape(m, heads, hd), ks, vs, 0.125, 0)
+        assert (np.abs(got[q0:q0 + m].reshape(m, heads, hd) - o) <= 2.0 ** -11 * (1.01 * mag + np.abs(o)) + 1e-6).all()
+
+
+def test_two_contexts_at_once():
+    """Two threads, a context each, on one GPU: each call gets its own results."""
+    import threading
+    seqs = [(i, 1, 0, 2000) for i in range(6)]
+    first = ge.Context.create(0)
+    alone, _ = attend(first, seqs, 8, 2, 128, F16, seed=18, prefix=700)
+    other, _ = attend(first, [(0, 200, 0, 200)], 3, 1, 256, BF16, seed=19)
+    first.close()
+    errors = []
+
+    def run(args, want):
+        try:
+            c = ge.Context.create(0)
+            for _ in range(5):
+                got, _ = attend(c, *args[0], **args[1])
+                assert np.array_equal(got, want)
+            c.close()
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+
+    jobs = [(((seqs, 8, 2, 128, F16), dict(seed=18, prefix=700)), alone), ((([(0, 200, 0, 200)], 3, 1, 256, BF16), dict(seed=19)), other)]
+    threads = [threading.Thread(target=run, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors[0]
