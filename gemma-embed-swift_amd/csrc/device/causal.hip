@@ -655,26 +655,20 @@ __global__ __launch_bounds__(256, HD <= 256 ? 2 : 1) void causal_kernel(const Ca
 
 // ---------------------------------------------------------------------------- joining the parts
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int x = 32; x; x >>= 1) v = fmaxf(v, __shfl_xor(v, x, 64));
-    return v;
-}
-__device__ __forceinline__ float lane_value(float v, int lane) {
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
-}
-
-// One wave a row, kJoinRows rows a workgroup: the parts' maxima and sums, a lane a part, then their rows
-// weighted and added in order.
-constexpr int kJoinRows = 4;
+// HD / 4 lanes a row (64 at most), so that every load is 16 bytes a lane: the parts' maxima and sums, a lane
+// a part, then their rows weighted and added in order. (A wave a row, at head dim 64 4 bytes a lane, took
+// 10.6 us to join 32768 rows of 1.5 parts; this way 4.9.)
+template <int HD>
+constexpr int kJoinLanes = HD < 256 ? HD / 4 : 64;
+template <int HD>
+constexpr int kJoinRows = 256 / kJoinLanes<HD>;  // of a workgroup
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void causal_join_kernel(const CausalArgs a, const CausalInline in) {
-    constexpr int E = HD / 64, V = E < 4 ? E : 4;  // dims a lane, and of one load
-    typedef float vec_t __attribute__((ext_vector_type(V)));
-    const int lane = threadIdx.x & 63;
+    constexpr int L = kJoinLanes<HD>, E = HD / (4 * L);  // 16-byte loads a lane of a row
+    const int lane = int(threadIdx.x) & (L - 1), group0 = int(threadIdx.x & 63) & ~(L - 1);
     const uint32_t at = blockIdx.x / uint32_t(a.kv_heads), kvh = blockIdx.x % uint32_t(a.kv_heads), g = uint32_t(a.group);
     const CausalJoin jn = uniform_entry<CausalJoin>(a.joins, in.joins, at);
-    const uint32_t row = blockIdx.y * kJoinRows + (threadIdx.x >> 6);
+    const uint32_t row = blockIdx.y * kJoinRows<HD> + threadIdx.x / L;
     if (row >= jn.n_rows) return;
     const size_t base = size_t(kvh) * a.part_rows + row;
     const uint32_t parts = jn.splits[0] + jn.splits[1];
@@ -683,45 +677,45 @@ __global__ __launch_bounds__(256) void causal_join_kernel(const CausalArgs a, co
     };
     auto load = [&](uint32_t s) { return s < parts ? a.part_ml[place(s)] : float2{-INFINITY, 0.0f}; };
     float top = -INFINITY;
-    for (uint32_t s = lane; s - lane < parts; s += 64) top = fmaxf(top, load(s).x);
-    top = wave_max(top);
-    float sum = 0.0f, o[E] = {};
-    for (uint32_t s0 = 0; s0 < parts; s0 += 64) {
+    for (uint32_t s = 0; s < parts; s += L) top = fmaxf(top, load(s + lane).x);
+#pragma unroll
+    for (int x = L / 2; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+    float sum = 0.0f;
+    float4_t o[E] = {};
+    for (uint32_t s0 = 0; s0 < parts; s0 += L) {
         const float2 ml = load(s0 + lane);
         // a part that saw no key has nothing to add, whatever its rows hold
         const float f = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
-        sum += wave_sum(ml.y == 0.0f ? 0.0f : ml.y * f);
-        const int n = int(min(64u, parts - s0));
+        sum += ml.y == 0.0f ? 0.0f : ml.y * f;
+        const int n = int(min(uint32_t(L), parts - s0));
         for (int i0 = 0; i0 < n; i0 += 4) {  // four parts' loads in flight
-            vec_t x[4][E / V];
+            float4_t x[4][E];
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int e = 0; e < E / V; e++)
-                    x[i][e] = *reinterpret_cast<const vec_t*>(a.part_o + place(s0 + min(i0 + i, n - 1)) * HD + e * 64 * V + lane * V);
+                for (int e = 0; e < E; e++)
+                    x[i][e] = *reinterpret_cast<const float4_t*>(a.part_o + place(s0 + min(i0 + i, n - 1)) * HD + (e * L + lane) * 4);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int k = min(i0 + i, n - 1);
-                const float w = lane_value(f, k);
-                const bool none = i0 + i >= n || lane_value(ml.y, k) == 0.0f;
+                const int k = group0 + min(i0 + i, n - 1);
+                const float w = __shfl(f, k, 64);
+                const bool none = i0 + i >= n || __shfl(ml.y, k, 64) == 0.0f;
 #pragma unroll
-                for (int e = 0; e < E; e++) o[e] = none ? o[e] : __builtin_fmaf(x[i][e / V][e % V], w, o[e]);
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[e][j] = none ? o[e][j] : __builtin_fmaf(x[i][e][j], w, o[e][j]);
             }
         }
     }
+#pragma unroll
+    for (int x = L / 2; x; x >>= 1) sum += __shfl_xor(sum, x, 64);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const uint32_t r = jn.row0 + row;
     uint16_t* const out = a.out + (size_t(jn.q_token) + r / g) * size_t(a.out_stride) + (size_t(kvh) * g + r % g) * HD;
 #pragma unroll
-    for (int e = 0; e < E; e += V) {
-        uint16_t* const p = out + e * 64 + lane * V;
-        if constexpr (V == 1)
-            *p = uint16_t(T::pack(o[e] * inv, 0.0f));
-        else if constexpr (V == 2)
-            *reinterpret_cast<uint32_t*>(p) = T::pack(o[e] * inv, o[e + 1] * inv);
-        else
-            *reinterpret_cast<u32x2*>(p) = u32x2{T::pack(o[e] * inv, o[e + 1] * inv), T::pack(o[e + 2] * inv, o[e + 3] * inv)};
-    }
+    for (int e = 0; e < E; e++)
+        *reinterpret_cast<u32x2*>(out + (e * L + lane) * 4) =
+            u32x2{T::pack(o[e][0] * inv, o[e][1] * inv), T::pack(o[e][2] * inv, o[e][3] * inv)};
 }
 
 template <typename T, int HD, int KINDS>
@@ -742,7 +736,7 @@ hipError_t run_kinds(hipStream_t s, const CausalArgs& a, const CausalInline& in,
 
 template <typename T, int HD>
 hipError_t run_join(hipStream_t s, const CausalArgs& a, const CausalInline& in) {
-    launch_kernel(causal_join_kernel<T, HD>, dim3(uint32_t(a.n_joins) * uint32_t(a.kv_heads), uint32_t(a.join_rows + kJoinRows - 1) / kJoinRows),
+    launch_kernel(causal_join_kernel<T, HD>, dim3(uint32_t(a.n_joins) * uint32_t(a.kv_heads), uint32_t(a.join_rows + kJoinRows<HD> - 1) / kJoinRows<HD>),
                   dim3(256), 0, s, a, in);
     return hipGetLastError();
 }
