@@ -21,7 +21,6 @@
 // already holds them (keys 4h..4h+3 and 8+4h..8+4h+3 for half h); V^T is read in that order.
 // Scores are kept in the log2 domain (s * scale * log2 e) so the exponentials are v_exp_f32.
 #include "common.hpp"
-#include "causal.hpp"
 #include "kernels.hpp"
 
 namespace ge {
@@ -1451,7 +1450,6 @@ hipError_t configure_kernels() {
                                 hipFuncAttributeMaxDynamicSharedMemorySize, attention_split_lds_bytes<256>());
     if (e == hipSuccess) e = attention_configure_all<256, 256>();
     if (e == hipSuccess) e = attention_configure_all<512, 256>();
-    if (e == hipSuccess) e = causal_configure();
     return e;
 }
 

@@ -280,6 +280,10 @@ void attend(ge_ctx* c, const ge_attention_shape* shape, const void* q, const voi
     if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(out) || !aligned(prefix_k) || !aligned(prefix_v))
         fail(GE_ERR_INVALID, "attention: buffers are 16-byte aligned");
 
+    if (!c->causal_ready) {
+        hip_check(causal_configure(), "hipFuncSetAttribute");
+        c->causal_ready = true;
+    }
     const Plan p = make_plan(s, seqs, n_seqs, prefix_len);
     if (p.n_items * uint64_t(s.kv_heads) > kCausalMaxGroups || p.joins.size() * uint64_t(s.kv_heads) > kCausalMaxGroups)
         fail(GE_ERR_INVALID, "attention: the call's rows and keys are too many for one call");

@@ -15,8 +15,9 @@
 //   O^T += V^T P^T: the same accumulators, rounded to the inputs' type, are the B operand of the
 //     16-key steps when V^T's keys are taken in that order; V^T comes from V's rows in LDS by the
 //     transposing LDS read (4 keys x 16 dims a read of 16 lanes), so no transposed copy of V exists.
-// The running maximum moves only when a score passes it by 2^8 (in log2), as in attention.hip; P is
-// taken 2^6 higher, which uses fp16's range up to 2^14 and keeps keys of 2^-30 of the maximum. Rounding P to
+// The running maximum moves only when a score passes it by 8 (in log2), as in attention.hip. P is taken
+// 2^6 higher in fp16, which uses its range up to 2^14 and keeps keys of 2^-30 of the maximum, and 2^8 lower in
+// bf16, whose values may themselves be near fp32's largest. Rounding P to
 // the inputs' type (half a step, 2^-11 or 2^-8 of a weight at most) is what the matrix instruction
 // takes; the sum of the weights is fp32, of P before rounding.
 //
@@ -36,8 +37,9 @@ typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
-// The two input types: the matrix instruction, two floats rounded to nearest even and packed, and
-// the bits whose sum with a value's magnitude reaches its sign bit iff its exponent is all ones.
+// The two input types: the matrix instruction, two floats rounded to nearest even and packed, the power of
+// two by which P is taken higher, and the bits whose sum with a value's magnitude reaches its sign bit iff
+// its exponent is all ones.
 struct F16 {
     static __device__ __forceinline__ float16_t mfma(u32x4 a, u32x4 b, float16_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
@@ -46,6 +48,7 @@ struct F16 {
         return __builtin_bit_cast(uint32_t, half2_t{_Float16(x), _Float16(y)});
     }
     static __device__ __forceinline__ float value(uint16_t x) { return h2f(x); }
+    static constexpr float kRaise = 6.0f;
     static constexpr uint32_t kNonFinite = 0x04000400u;
 };
 struct BF16 {
@@ -56,10 +59,10 @@ struct BF16 {
         return __builtin_bit_cast(uint32_t, bf16x2_t{__bf16(x), __bf16(y)});
     }
     static __device__ __forceinline__ float value(uint16_t x) { return __uint_as_float(uint32_t(x) << 16); }
+    static constexpr float kRaise = -8.0f;
     static constexpr uint32_t kNonFinite = 0x00800080u;
 };
 
-constexpr float kRaise = 6.0f;       // P = 2^(score - maximum + kRaise)
 constexpr float kLazy = 8.0f;        // the maximum moves when a score passes it by this much (log2)
 constexpr int kNoWindow = -(1 << 30);
 
@@ -221,7 +224,7 @@ struct Rows {
                 for (int d = 0; d < DT; d++) w.o[d] *= fade;
                 w.m = m_new;
             }
-            const float ref = w.m == -INFINITY ? 0.0f : kRaise - w.m;
+            const float ref = w.m == -INFINITY ? 0.0f : T::kRaise - w.m;
             float sum = 0.0f;
 #pragma unroll
             for (int t = 0; t < KT; t++)

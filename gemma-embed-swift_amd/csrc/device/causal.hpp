@@ -64,7 +64,7 @@ bool causal_head_dim_ok(int hd);
 // kinds: the CausalKind of the items.
 hipError_t launch_causal(hipStream_t s, const CausalArgs& a, const CausalInline& in, int hd, bool bf16, int kinds);
 hipError_t launch_causal_join(hipStream_t s, const CausalArgs& a, const CausalInline& in, int hd, bool bf16);
-// Dynamic LDS limits; once per device.
+// Dynamic LDS limits; once per device, before launching (24 kernels: 2 ms of a context's creation otherwise).
 hipError_t causal_configure();
 
 }  // namespace ge

@@ -210,6 +210,7 @@ struct ge_ctx {
     // kOpTempsKept bytes.
     void* op_buf = nullptr;
     size_t op_cap = 0;
+    bool causal_ready = false;  // causal_configure() has run (causal.cpp)
     // Pinned memory of one per-op call's work lists (op_lists), which its kernels read in place.
     void* op_host = nullptr;
     size_t op_host_cap = 0;

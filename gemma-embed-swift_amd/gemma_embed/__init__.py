@@ -675,7 +675,7 @@ class Context:
     def attention_causal(self, shape: "ge_attention_shape", q: int, k: int, v: int, seqs: np.ndarray, out: int):
         """ge_op_attention_causal: packed prompts, chunks and single tokens over cached keys."""
         s = attention_seqs(seqs)
-        self._check(lib.ge_op_attention_causal(self.handle, C.byref(shape), q, k, v, s.ctypes.data, len(s), out),
+        self._check(lib.ge_op_attention_causal(self.handle, C.byref(shape), q, k, v, s.__array_interface__["data"][0], len(s), out),
                     "ge_op_attention_causal")
 
     def attention_prefix(self, shape: "ge_attention_shape", q: int, prefix_k: int, prefix_v: int, prefix_len: int, k: int,
@@ -683,7 +683,7 @@ class Context:
         """ge_op_attention_prefix: every sequence's keys are the shared prefix's rows, then its own."""
         s = attention_seqs(seqs)
         self._check(lib.ge_op_attention_prefix(self.handle, C.byref(shape), q, prefix_k, prefix_v, prefix_len, k, v,
-                                               s.ctypes.data, len(s), out), "ge_op_attention_prefix")
+                                               s.__array_interface__["data"][0], len(s), out), "ge_op_attention_prefix")
 
 
 def attention_shape(type: int, heads: int, kv_heads: int, head_dim: int, q_rows: int, kv_rows: int, scale: float = 1.0,
@@ -696,6 +696,9 @@ def attention_shape(type: int, heads: int, kv_heads: int, head_dim: int, q_rows:
 
 def attention_seqs(sequences) -> np.ndarray:
     """(q_start, q_len, kv_start, kv_len) of each sequence as a (n, 4) uint32 array."""
+    if type(sequences) is np.ndarray and sequences.dtype == np.uint32 and sequences.flags.c_contiguous and sequences.ndim == 2 \
+            and sequences.shape[1] == 4:
+        return sequences
     s = np.asarray(sequences)
     if s.dtype != np.uint32:
         if s.size and (s.min() < 0 or s.max() > 0xffffffff):

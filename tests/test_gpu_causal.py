@@ -385,3 +385,9 @@ def test_two_contexts_at_once():
     for t in threads:
         t.join()
     assert not errors, errors[0]
+
+
+def test_bf16_values_near_the_largest(ctx):
+    """Sums of weights times values of 1e38 stay inside fp32."""
+    for layout in LAYOUTS:
+        attend(ctx, [(0, 70, 0, 70), (70, 1, 0, 200)], *layout, BF16, seed=20, values=2.0 ** 124)
