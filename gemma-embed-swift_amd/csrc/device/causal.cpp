@@ -1,11 +1,11 @@
 // Per-op entries of causal models' attention (ge_op_attention_causal, ge_op_attention_prefix): checks,
 // the plan of a call's work, and its launches.
 //
-// A call's rows are tiled per base: a sequence against its own keys, and, over a shared prefix, either
-// a run of neighbouring sequences whose rows all see the whole prefix (their rows stack up, so the
-// prefix is read once per tile of rows and not once per sequence) or one sequence that does not. Each
-// tile's visible keys are split until the launch fills the GPU; rows that end in more than one part are
-// joined by a second launch.
+// A call's rows are tiled per base: a sequence against all of its keys, the prefix's and its own, or, where
+// neighbouring sequences all see the whole of a prefix that is worth it, their stacked rows against the
+// prefix (read once per tile of rows and not once per sequence) and each against its own keys. Each tile's
+// visible keys are split until the launch fills the GPU; rows that end in more than one part are joined by a
+// second launch.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -29,10 +29,10 @@ struct Tile {
     uint32_t splits;
 };
 
-// Rows of one sequence, or of a run of them, against one source of keys.
+// Rows of one sequence, or of a run of them, against a range of their keys.
 struct Base {
-    uint32_t q_token, key0, source, tile0;
-    int64_t keys, shift;
+    uint32_t q_token, key0, tile0;
+    int64_t shift;
     bool direct;  // its rows have no other part
 };
 
@@ -51,19 +51,31 @@ bool narrow(const Tile& t) { return t.n_rows <= uint32_t(kCausalNarrowRows); }
 // 64-key steps keep the parts' blocks whole.
 int32_t step_of(const Tile& t) { return t.splits > 1 ? int32_t(divide_up(t.hi - t.lo, int64_t(t.splits) * 64) * 64) : t.hi - t.lo; }
 
-void add_base(Plan& p, uint32_t q_token, int64_t tokens, uint32_t source, uint32_t key0, int64_t keys, int64_t shift, int window,
+// Keys [first, end), counted through the prefix.
+void add_base(Plan& p, uint32_t q_token, int64_t tokens, uint32_t key0, int64_t first, int64_t end, int64_t shift, int window,
               bool direct) {
     const uint32_t at = uint32_t(p.bases.size());
-    p.bases.push_back(Base{q_token, key0, source, uint32_t(p.tiles.size()), keys, shift, direct});
+    p.bases.push_back(Base{q_token, key0, uint32_t(p.tiles.size()), shift, direct});
     const int64_t rows = tokens * p.group;
     for (int64_t r = 0; r < rows; r += p.wide) {
         const int64_t n = std::min<int64_t>(p.wide, rows - r);
-        int64_t lo = 0, hi = keys;
-        if (window) lo = std::max<int64_t>(0, r / p.group + shift - window + 1);
-        if (shift < keys) hi = std::min(keys, (r + n - 1) / p.group + shift + 1);
-        if (hi <= lo) lo = hi = 0;
+        int64_t lo = first, hi = end;
+        if (window) lo = std::max(first, r / p.group + shift - window + 1);
+        if (shift < end) hi = std::min(end, (r + n - 1) / p.group + shift + 1);
+        if (hi <= lo) lo = hi = first;
         p.tiles.push_back(Tile{at, uint32_t(r), uint32_t(n), 0, int32_t(lo), int32_t(hi), 0});
     }
+}
+
+// A wide tile's time a key on a full CU; the joining launch, with the writes and reads of its partial rows.
+float wide_key_us(int head_dim) { return 0.025f * float(head_dim) / 128; }
+float parts_us(int64_t rows, int kv_heads, int head_dim) { return 5.0f + float(rows) * float(kv_heads) * float(head_dim) * 8 / 3e6f; }
+
+// Eighths of a full tile's work in the tiles of so many rows: a tile of a quarter or less is a narrow one, a
+// part of a wide one spares its waves' products but not its copies.
+int64_t tile_eighths(const Plan& p, int64_t rows) {
+    const int64_t rest = rows % p.wide;
+    return rows / p.wide * 8 + (rest == 0 ? 0 : rest <= kCausalNarrowRows ? 2 : 4 + divide_up(rest * 4, p.wide));
 }
 
 // The most keys of an item. Splitting fills the GPU and evens the items out, and costs the parts' rows
@@ -77,7 +89,7 @@ void add_base(Plan& p, uint32_t q_token, int64_t tokens, uint32_t source, uint32
 // 203, one prompt of 2048 (32 heads of 128) 67 / 67 / 78 / 83 / 84.
 int64_t split_limit(const Plan& p, int kv_heads, int head_dim) {
     constexpr int kBins = 64;
-    const float key_us = 0.025f * float(head_dim) / 128;
+    const float key_us = wide_key_us(head_dim);
     int64_t total = 0, longest = 0, wide_keys = 0;
     for (const Tile& t : p.tiles) {
         const int64_t n = t.hi - t.lo;
@@ -115,7 +127,7 @@ int64_t split_limit(const Plan& p, int kv_heads, int head_dim) {
                 us = std::max(us, (float(k / (2 * kCus)) * 2 * pair + (k / kCus % 2 ? 2 * pair : 1.0f)) * key_us * float(limit) * float(bin + 1) / kBins);
         }
         us += 7.0f * float((items + 2 * kCus - 1) / (2 * kCus));
-        if (parts) us += 5.0f + float(parts) * float(kv_heads) * float(head_dim) * 8 / 3e6f;
+        if (parts) us += parts_us(parts, kv_heads, head_dim);
         if (us < best_us) {
             best_us = us;
             best = limit;
@@ -135,34 +147,46 @@ Plan make_plan(const ge_attention_shape& s, const ge_attention_seq* seqs, int n_
         int64_t prefix_row = 0;  // the sequence's first row in its prefix base
     };
     std::vector<Use> use(size_t(n_seqs), Use{});
-    for (int i = 0; i < n_seqs; i++) {
-        const ge_attention_seq& q = seqs[i];
-        if (!q.q_len || (prefix_len && !q.kv_len)) continue;
-        use[size_t(i)].own = int(p.bases.size());
-        add_base(p, q.q_start, q.q_len, 0, q.kv_start, q.kv_len, int64_t(q.kv_len) - q.q_len, s.window, prefix_len == 0);
-    }
-    for (int i = 0; prefix_len && i < n_seqs;) {
+    // Sequences whose every row sees the whole prefix, wherever it stands, may stack up.
+    auto stacks = [&](const ge_attention_seq& q) { return prefix_len && s.window == 0 && int64_t(q.q_len) <= int64_t(q.kv_len) + 1; };
+    for (int i = 0; i < n_seqs;) {
         if (!seqs[i].q_len) {
             i++;
             continue;
         }
-        // every row of such a sequence sees the whole prefix, wherever it stands
-        auto whole = [&](const ge_attention_seq& q) { return s.window == 0 && int64_t(q.q_len) <= int64_t(q.kv_len) + 1; };
-        int64_t tokens = seqs[i].q_len, shift = prefix_len + seqs[i].kv_len - int64_t(seqs[i].q_len);
-        bool alone = seqs[i].kv_len == 0;
-        int j = i + 1;
-        use[size_t(i)].prefix = int(p.bases.size());
-        if (whole(seqs[i])) {
-            shift = kMaxRows;
-            for (; j < n_seqs && whole(seqs[j]) && seqs[j].q_start == seqs[i].q_start + uint64_t(tokens); j++) {
-                use[size_t(j)].prefix = int(p.bases.size());
-                use[size_t(j)].prefix_row = tokens * p.group;
-                tokens += seqs[j].q_len;
-                alone = alone && seqs[j].kv_len == 0;
+        const uint32_t q_start = seqs[i].q_start;
+        int64_t tokens = 0, apart = 0;  // of the run from i to j
+        bool alone = true;
+        int j = i;
+        do {
+            tokens += seqs[j].q_len;
+            apart += tile_eighths(p, int64_t(seqs[j].q_len) * p.group);
+            alone = alone && seqs[j].kv_len == 0;
+            j++;
+        } while (stacks(seqs[j - 1]) && j < n_seqs && seqs[j].q_len && stacks(seqs[j]) && seqs[j].q_start == q_start + uint64_t(tokens));
+        // Stacked, the run has fewer tiles to take over the prefix, but two parts a row to join. Of n sequences,
+        // us apart / stacked over 24, 400, 1000 and 4000 keys: one token of 4 heads over each of 2 KV heads of 128,
+        // n = 256: 25 / 36, 31 / 40, 38 / 40, 74 / 45; 4 to 32 tokens of 3 heads of 256, n = 96: 25 / 35, 42 / 44,
+        // 53 / 48, 91 / 69; 20 to 100 tokens of 4 heads over each of 8 of 64, n = 256: 67 / 214, 126 / 246,
+        // 227 / 326, 641 / 698.
+        const int64_t rows = tokens * p.group;
+        const bool stack = j > i + 1 && float(apart - tile_eighths(p, rows)) / 8 * float(prefix_len) * float(s.kv_heads) *
+                                                wide_key_us(s.head_dim) / kCus > (alone ? 0.0f : parts_us(2 * rows, s.kv_heads, s.head_dim));
+        int64_t row = 0;
+        if (stack) add_base(p, q_start, tokens, 0, 0, prefix_len, kMaxRows, 0, alone);
+        const int prefix = int(p.bases.size()) - 1;
+        for (; i < j; i++) {
+            const ge_attention_seq& e = seqs[i];
+            if (stack) {
+                use[size_t(i)].prefix = prefix;
+                use[size_t(i)].prefix_row = row;
+                row += int64_t(e.q_len) * p.group;
+                if (!e.kv_len) continue;
             }
+            use[size_t(i)].own = int(p.bases.size());
+            add_base(p, e.q_start, e.q_len, e.kv_start, stack ? prefix_len : 0, prefix_len + e.kv_len,
+                     prefix_len + e.kv_len - int64_t(e.q_len), s.window, !stack);
         }
-        add_base(p, seqs[i].q_start, tokens, 1, 0, prefix_len, shift, s.window, alone);
-        i = j;
     }
 
     const int64_t limit = split_limit(p, s.kv_heads, s.head_dim);
@@ -229,7 +253,7 @@ void write_items(const Plan& p, CausalItem* out) {
             const int32_t k = t.lo + int32_t(s) * step;
             const bool direct = b.direct && t.splits == 1;
             *out++ = CausalItem{b.q_token, t.row0, t.n_rows, b.key0, uint32_t(std::min(k, t.hi)), uint32_t(std::min(k + step, t.hi)),
-                                int32_t(b.shift), direct ? kDirect : t.part + s * t.n_rows, b.source, narrow(t)};
+                                int32_t(b.shift), direct ? kDirect : t.part + s * t.n_rows, narrow(t)};
         }
     }
 }
@@ -252,8 +276,8 @@ void attend(ge_ctx* c, const ge_attention_shape* shape, const void* q, const voi
     if (s.heads <= 0 || s.kv_heads <= 0 || s.heads % s.kv_heads || s.heads > 4096)
         fail(GE_ERR_INVALID, "attention: %d query heads over %d KV heads (a multiple, up to 4096)", s.heads, s.kv_heads);
     if (s.q_rows < 0 || s.kv_rows < 0 || prefix_len < 0 || s.q_rows >= kMaxRows || s.kv_rows >= kMaxRows ||
-        prefix_len >= kMaxRows || s.window < 0 || s.window >= kMaxRows || n_seqs < 0)
-        fail(GE_ERR_INVALID, "attention: rows, prefix, window and sequences from 0 to under 2^30");
+        int64_t(s.kv_rows) + prefix_len >= kMaxRows || s.window < 0 || s.window >= kMaxRows || n_seqs < 0)
+        fail(GE_ERR_INVALID, "attention: query rows, window, sequences, and key rows and prefix together from 0 to under 2^30");
     if (int64_t(s.q_rows) * (s.heads / s.kv_heads) >= kMaxRows)
         fail(GE_ERR_INVALID, "attention: %d rows of %d query heads a KV head pass 2^30", s.q_rows, s.heads / s.kv_heads);
     if (!std::isfinite(s.scale)) fail(GE_ERR_INVALID, "attention: scale is not finite");
@@ -317,6 +341,7 @@ void attend(ge_ctx* c, const ge_attention_shape* shape, const void* q, const voi
     a.n_items = int(p.n_items);
     a.n_joins = int(p.joins.size());
     for (const CausalJoin& j : p.joins) a.join_rows = std::max(a.join_rows, int(j.n_rows));
+    a.prefix_len = int(prefix_len);
     a.group = s.heads / s.kv_heads;
     a.kv_heads = s.kv_heads;
     a.window = s.window;

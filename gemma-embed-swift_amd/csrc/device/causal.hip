@@ -125,6 +125,32 @@ struct KvBlock {
     }
 };
 
+// The key blocks of an item: those of its prefix keys, then those of its own, none of both.
+template <int BK>
+struct Span {
+    int own0, blocks;      // the first block of own keys, all blocks
+    int lo, end0, skip;    // the item's first key, the end of its prefix keys, the keys that block own0 - 1 lacks
+    int hi;
+    uint32_t own_row;      // + key: its row of k and v, modulo 2^32
+
+    __device__ __forceinline__ Span(const CausalArgs& a, const CausalItem& it) : lo(int(it.k_lo)), hi(int(it.k_hi)) {
+        end0 = min(max(lo, a.prefix_len), hi);
+        own0 = (end0 - lo + BK - 1) / BK;
+        skip = own0 * BK - (end0 - lo);
+        blocks = own0 + (hi - end0 + BK - 1) / BK;
+        own_row = it.key0 - uint32_t(a.prefix_len);
+    }
+    __device__ __forceinline__ int first(int b) const { return lo + b * BK - (b < own0 ? 0 : skip); }
+    __device__ __forceinline__ int end(int b) const { return min(first(b) + BK, b < own0 ? end0 : hi); }
+    // Block b's rows of k or v (own, prefix) for one head.
+    template <int HD>
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(int b, const uint16_t* own, const uint16_t* prefix, int64_t stride,
+                                                          int kvh) const {
+        const bool p = b < own0;
+        return KvBlock<HD, BK>::rows_of(p ? prefix : own, uint32_t(first(b)) + (p ? 0u : own_row), stride, kvh * HD, end(b) - first(b));
+    }
+};
+
 // Fragments read ahead of their products (four spill at head dim 256).
 template <int HD>
 constexpr int kFragmentsAhead = HD == 256 ? 3 : 4;
@@ -194,20 +220,20 @@ struct Rows {
             }
         }
 
-        __device__ __forceinline__ bool sees_all(const Rows& w, int kb) const {
-            return kb + BK - 1 <= w.hi_all && kb >= w.lo_all;
+        __device__ __forceinline__ bool sees_all(const Rows& w, int kb, int end) const {
+            return kb + BK <= end && kb + BK - 1 <= w.hi_all && kb >= w.lo_all;
         }
 
-        // Hidden keys to -inf, the running maximum, and P.
-        __device__ __forceinline__ void softmax(Rows& w, int kb, float c, int lane, u32x4 (&p)[2 * KT]) {
-            if (!sees_all(w, kb)) {
-                const int k0 = kb + (lane >> 5) * 4;
+        // Hidden keys and those from `end` on to -inf, the running maximum, and P.
+        __device__ __forceinline__ void softmax(Rows& w, int kb, int end, float c, int lane, u32x4 (&p)[2 * KT]) {
+            if (!sees_all(w, kb, end)) {
+                const int k0 = kb + (lane >> 5) * 4, hi = min(w.hi, end - 1);
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
                         const int key = k0 + 32 * t + 8 * (e >> 2) + (e & 3);
-                        s[t][e] = key <= w.hi && key >= w.lo ? s[t][e] : -INFINITY;
+                        s[t][e] = key <= hi && key >= w.lo ? s[t][e] : -INFINITY;
                     }
             }
             float top = s[0][0];
@@ -384,29 +410,31 @@ struct HeldBack {
         any = (flag[0] | flag[1] | flag[2] | flag[3]) != 0;
         __syncthreads();
     }
-    // Rows [r0, r0 + n), dims [d0, d0 + dims), which this wave has stored; bk: the item's key blocks.
-    __device__ __forceinline__ void add(const CausalArgs& a, const CausalItem& it, int kvh, int r0, int n, int d0, int dims, int bk) const {
+    // Rows [r0, r0 + n), dims [d0, d0 + dims), which this wave has stored.
+    template <int BK>
+    __device__ __forceinline__ void add(const CausalArgs& a, const CausalItem& it, const Span<BK>& span, int kvh, int r0, int n, int d0,
+                                        int dims) const {
         __threadfence();
-        const uint16_t* const v = (it.source ? a.prefix_v : a.v) + size_t(kvh) * HD;
         const uint32_t g = uint32_t(a.group);
-        for (uint32_t key = it.k_lo; key < it.k_hi; key++) {
-            const int kb = int(it.k_lo) + (int(key) - int(it.k_lo)) / bk * bk;
-            if (!mixed(kb, bk)) {
-                key = uint32_t(kb + bk - 1);
-                continue;
-            }
-            for (int d = d0 + int(threadIdx.x & 63); d < d0 + dims; d += 64) {
-                const uint16_t x = v[(size_t(it.key0) + key) * size_t(a.v_stride) + d];
-                if (((x & 0x7fffu) + (T::kNonFinite & 0xffffu)) < 0x8000u) continue;
-                for (int row = 0; row < n; row++) {
-                    const uint32_t r = uint32_t(r0 + row);
-                    const int i = int(r / g);
-                    if (int(key) > i + it.shift || (a.window && int(key) <= i + it.shift - a.window)) continue;
-                    if (it.part == kDirect) {
-                        uint16_t* o = a.out + (size_t(it.q_token) + r / g) * size_t(a.out_stride) + (size_t(kvh) * g + r % g) * HD + d;
-                        *o = uint16_t(T::pack(T::value(*o) + T::value(x), 0.0f));
-                    } else {
-                        a.part_o[(size_t(kvh) * a.part_rows + it.part + (r - it.row0)) * HD + d] += T::value(x);
+        for (int b = 0; b < span.blocks; b++) {
+            if (!mixed(span.first(b), BK)) continue;
+            for (int key = span.first(b); key < span.end(b); key++) {
+                const uint16_t* const v = (b < span.own0 ? a.prefix_v + size_t(key) * size_t(a.v_stride)
+                                                         : a.v + (size_t(it.key0) + size_t(key - a.prefix_len)) * size_t(a.v_stride)) +
+                                          size_t(kvh) * HD;
+                for (int d = d0 + int(threadIdx.x & 63); d < d0 + dims; d += 64) {
+                    const uint16_t x = v[d];
+                    if (((x & 0x7fffu) + (T::kNonFinite & 0xffffu)) < 0x8000u) continue;
+                    for (int row = 0; row < n; row++) {
+                        const uint32_t r = uint32_t(r0 + row);
+                        const int i = int(r / g);
+                        if (key > i + it.shift || (a.window && key <= i + it.shift - a.window)) continue;
+                        if (it.part == kDirect) {
+                            uint16_t* o = a.out + (size_t(it.q_token) + r / g) * size_t(a.out_stride) + (size_t(kvh) * g + r % g) * HD + d;
+                            *o = uint16_t(T::pack(T::value(*o) + T::value(x), 0.0f));
+                        } else {
+                            a.part_o[(size_t(kvh) * a.part_rows + it.part + (r - it.row0)) * HD + d] += T::value(x);
+                        }
                     }
                 }
             }
@@ -429,8 +457,6 @@ struct Wide {
 
     static __device__ __forceinline__ void run(const CausalArgs& a, const CausalItem& it, int kvh, unsigned char* lds) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-        const uint16_t* const kp = it.source ? a.prefix_k : a.k;
-        const uint16_t* const vp = it.source ? a.prefix_v : a.v;
         const uint32_t kb_bytes = uint32_t(a.k_stride) * 2, vb_bytes = uint32_t(a.v_stride) * 2;
         static_assert(Kv::kChunks % NW == 0 && (BK / 8) % NW == 0 && NW % 2 == 0, "every wave copies chunks of one key parity");
         uint32_t k_off[BK / 8 / NW], v_off[BK / 8 / NW];
@@ -439,13 +465,12 @@ struct Wide {
             k_off[i] = Kv::k_lane(lane, wave & 1, kb_bytes) + uint32_t((wave + i * NW) * 8) * kb_bytes;
             v_off[i] = Kv::v_lane(lane, vb_bytes) + uint32_t((wave + i * NW) * 8) * vb_bytes;
         }
-        const int k_lo = int(it.k_lo), k_hi = int(it.k_hi);
-        const int blocks = (k_hi - k_lo + BK - 1) / BK;
+        const Span<BK> span(a, it);
+        const int blocks = span.blocks;
         auto issue = [&](int b) {
-            const int kb = k_lo + b * BK, rows = min(BK, k_hi - kb);
             unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
-            const auto kr = Kv::rows_of(kp, size_t(it.key0) + kb, a.k_stride, kvh * HD, rows);
-            const auto vr = Kv::rows_of(vp, size_t(it.key0) + kb, a.v_stride, kvh * HD, rows);
+            const auto kr = span.template rows<HD>(b, a.k, a.prefix_k, a.k_stride, kvh);
+            const auto vr = span.template rows<HD>(b, a.v, a.prefix_v, a.v_stride, kvh);
             Kv::template copies<HD / 64, NW>(kr, at, wave, k_off);
             Kv::template copies<HD / 64, NW>(vr, at + Kv::kBytes, wave, v_off);
         };
@@ -456,7 +481,7 @@ struct Wide {
         if (blocks > 0) issue(0);
         if (n > 0) w.init(a, it, kvh, r0, n, wave % DW, lane);
         for (int b = 0; b < blocks; b++) {
-            const int kb = k_lo + b * BK;
+            const int kb = span.first(b);
             unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
             wait_vmcnt<0>();
             if (held.mixed(kb, BK)) {
@@ -471,7 +496,7 @@ struct Wide {
                 typename Rows<T, HD, DW>::template Block<BK> blk;
                 u32x4 p[BK / 16];
                 blk.scores(w, at, lane);
-                blk.softmax(w, kb, a.c, lane, p);
+                blk.softmax(w, kb, span.end(b), a.c, lane, p);
                 blk.product(w, at + Kv::kBytes, lane, p);
             }
         }
@@ -482,7 +507,7 @@ struct Wide {
             w.template finish_rows<kSlice>(a, it, kvh, r0, n, lane, lds + wave * kSlice);
         }
         held.share(lds);
-        if (n > 0 && held.any) held.add(a, it, kvh, r0, n, w.d0 * 32, w.DT * 32, BK);
+        if (n > 0 && held.any) held.add(a, it, span, kvh, r0, n, w.d0 * 32, w.DT * 32);
     }
 };
 
@@ -554,8 +579,6 @@ struct Narrow {
     static __device__ __forceinline__ void run(const CausalArgs& a, const CausalItem& it, int kvh, unsigned char* lds) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
         const int kw = wave / DW, dims = wave % DW;
-        const uint16_t* const kp = it.source ? a.prefix_k : a.k;
-        const uint16_t* const vp = it.source ? a.prefix_v : a.v;
         const uint32_t kb_bytes = uint32_t(a.k_stride) * 2, vb_bytes = uint32_t(a.v_stride) * 2;
         // a wave of a pair copies half of the panels
         constexpr int kPanels = HD / 64 / DW;
@@ -565,18 +588,16 @@ struct Narrow {
             k_off[i] = Kv::k_lane(lane, i & 1, kb_bytes) + uint32_t(i * 8) * kb_bytes + uint32_t(dims * kPanels * 128);
             v_off[i] = Kv::v_lane(lane, vb_bytes) + uint32_t(i * 8) * vb_bytes + uint32_t(dims * kPanels * 128);
         }
-        const int k_lo = int(it.k_lo), k_hi = int(it.k_hi);
-        const int blocks = (k_hi - k_lo + BK - 1) / BK;
+        const Span<BK> span(a, it);
+        const int blocks = span.blocks;
         unsigned char* const K = lds + kw * kPerKw;
         unsigned char* const V = K + Kv::kBytes;
         auto issue_k = [&](int b) {
-            const int kb = k_lo + b * BK;
-            const auto r = Kv::rows_of(kp, size_t(it.key0) + kb, a.k_stride, kvh * HD, min(BK, k_hi - kb));
+            const auto r = span.template rows<HD>(b, a.k, a.prefix_k, a.k_stride, kvh);
             Kv::template copies<kPanels, 1>(r, K + dims * kChunks * 1024, 0, k_off);
         };
         auto issue_v = [&](int b) {
-            const int kb = k_lo + b * BK;
-            const auto r = Kv::rows_of(vp, size_t(it.key0) + kb, a.v_stride, kvh * HD, min(BK, k_hi - kb));
+            const auto r = span.template rows<HD>(b, a.v, a.prefix_v, a.v_stride, kvh);
             Kv::template copies<kPanels, 1>(r, V + dims * kChunks * 1024, 0, v_off);
         };
         const int r0 = int(it.row0), n = int(it.n_rows);
@@ -590,7 +611,7 @@ struct Narrow {
         w.init(a, it, kvh, r0, n, dims, lane);
         // Waves alone on their LDS leave when their blocks are done; pairs keep meeting until all are.
         for (int b = kw; b - kw < blocks; b += KW) {
-            const int kb = k_lo + b * BK;
+            const int kb = span.first(b);
             const bool mine = b < blocks, more = b + KW < blocks;
             if (DW == 1 && !mine) break;
             typename Rows<T, HD, DW>::template Block<BK> blk;
@@ -600,7 +621,7 @@ struct Narrow {
             if (mine) blk.scores(w, K, lane);
             meet();  // K's reads have returned before its next block is copied over it
             if (more) issue_k(b + KW);
-            if (mine) blk.softmax(w, kb, a.c, lane, p);
+            if (mine) blk.softmax(w, kb, span.end(b), a.c, lane, p);
             if (more)
                 wait_vmcnt<kChunks>();  // all but the next K's
             else
@@ -619,7 +640,7 @@ struct Narrow {
         Join::run(w, kw, dims, lane, lds);
         if (kw > 0) return;
         w.finish(a, it, kvh, r0, n, lane);
-        if (held.any) held.add(a, it, kvh, r0, n, w.d0 * 32, w.DT * 32, BK);
+        if (held.any) held.add(a, it, span, kvh, r0, n, w.d0 * 32, w.DT * 32);
     }
 };
 

@@ -16,15 +16,15 @@ constexpr uint32_t kDirect = 0xffffffffu;
 // Workgroups of a launch: HIP's grid counts work-items in 32 bits.
 constexpr uint64_t kCausalMaxGroups = (uint64_t(1) << 32) / 256 - 1;
 
-// Stacked rows [row0, row0 + n_rows) (token row / group from q_token on) against the keys
-// [k_lo, k_hi) of the rows that start at key0 of k and v (of the prefix's where source is 1). Row
-// token i sees key j iff j <= i + shift and, with a window, j > i + shift - window.
+// Stacked rows [row0, row0 + n_rows) (token row / group from q_token on) against the keys [k_lo, k_hi). A
+// sequence's keys count through: the prefix's rows are 0 .. prefix_len - 1, its own, from row key0 of k and v on,
+// prefix_len and up. Row token i sees key j iff j <= i + shift and, with a window, j > i + shift - window.
 struct CausalItem {
     uint32_t q_token, row0, n_rows;
     uint32_t key0, k_lo, k_hi;
     int32_t shift;
     uint32_t part;  // kDirect: the rows go to out; else to the partial rows from here on
-    uint32_t source, narrow;
+    uint32_t narrow;
 };
 
 // Rows [row0, row0 + n_rows) of q_token's sequence joined from splits[0] parts at partial rows
@@ -46,6 +46,7 @@ struct CausalArgs {
     int n_items, n_joins;
     int join_rows;  // the most rows of a join
     int group, kv_heads, window;  // window 0: none
+    int prefix_len;
     float c;                      // |scale| log2(e)
     uint32_t q_flip;              // the sign bits of two values where the scale is negative
 };

@@ -285,8 +285,9 @@ int ge_op_attention_split(ge_ctx* ctx, const void* q, const void* q_lo, const vo
  * and v may be views of one projection's output. All are of one type, GE_TYPE_F16 or GE_TYPE_BF16. out
  * overlaps none of the inputs.
  * Limits: heads a multiple of kv_heads, up to 4096; head_dim 64, 128, 256 or 512; buffers 16-byte aligned;
- * strides a multiple of 8 up to 2^24; rows, window and prefix under 2^30. Scores, softmax and sums are in
- * fp32; the softmax weights are rounded to the operands' type before the product with V. */
+ * strides a multiple of 8 up to 2^24; query rows, the window, and key rows and prefix together under 2^30.
+ * Scores, softmax and sums are in fp32; the softmax weights are rounded to the operands' type before the
+ * product with V. */
 typedef struct ge_attention_shape {
     int32_t type;
     int32_t heads, kv_heads, head_dim;
@@ -313,8 +314,8 @@ int ge_op_attention_causal(ge_ctx* ctx, const ge_attention_shape* shape, const v
 
 /* The same where every sequence's keys are the prefix_len rows of prefix_k / prefix_v (k's and v's strides)
  * followed by its own kv_len rows: n = prefix_len + kv_len keys, j <= i + n - q_len, j > i + n - q_len - window.
- * The prefix is read once for all sequences whose query rows follow each other and see all of it
- * (no window, q_len <= kv_len + 1). */
+ * A prefix worth it is read once for all sequences whose query rows follow each other and see all
+ * of it (no window, q_len <= kv_len + 1). */
 int ge_op_attention_prefix(ge_ctx* ctx, const ge_attention_shape* shape, const void* q, const void* prefix_k,
                            const void* prefix_v, int32_t prefix_len, const void* k, const void* v,
                            const ge_attention_seq* seqs, int32_t n_seqs, void* out);

@@ -21,7 +21,7 @@ DIRECT = 0xffffffff
 class Item(C.Structure):
     """CausalItem, causal.hpp"""
     _fields_ = [(n, C.c_uint32) for n in ("q_token", "row0", "n_rows", "key0", "k_lo", "k_hi")] + \
-        [("shift", C.c_int32)] + [(n, C.c_uint32) for n in ("part", "source", "narrow")]
+        [("shift", C.c_int32)] + [(n, C.c_uint32) for n in ("part", "narrow")]
 
 
 class Join(C.Structure):
@@ -35,7 +35,7 @@ class Args(C.Structure):
     _fields_ = [(n, P) for n in ("q", "k", "v", "prefix_k", "prefix_v", "out")] + \
         [("items", C.POINTER(Item)), ("joins", C.POINTER(Join)), ("part_o", P), ("part_ml", P)] + \
         [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + [("part_rows", C.c_size_t)] + \
-        [(n, I) for n in ("n_items", "n_joins", "join_rows", "group", "kv_heads", "window")] + [("c", C.c_float), ("q_flip", C.c_uint32)]
+        [(n, I) for n in ("n_items", "n_joins", "join_rows", "group", "kv_heads", "window", "prefix_len")] + [("c", C.c_float), ("q_flip", C.c_uint32)]
 
 
 class Inline(C.Structure):
@@ -112,11 +112,12 @@ def covered(got, seqs, heads, kv_heads, hd, window, prefix):
     """Every row's visible keys are in its parts exactly once, and every row is written exactly once."""
     group, wide = heads // kv_heads, 64 if hd > 256 else 128
     assert got.args["join_rows"] == max([j.n_rows for j in got.joins], default=0)
-    part = {}  # partial row -> (q token, group row, prefix keys, own keys)
+    part = {}  # partial row -> (q token, group row, first own key row, keys)
+    assert got.args["prefix_len"] == prefix
     written, longest = {}, 0
 
     def keys(item, token):
-        """The keys of the item that the row of this token sees, as positions of the item's source."""
+        """The keys of the item that the row of this token sees, counted through the prefix."""
         i = token - item.q_token
         last = i + item.shift
         low = last - window + 1 if window else 0
@@ -129,7 +130,7 @@ def covered(got, seqs, heads, kv_heads, hd, window, prefix):
             row = it.row0 + r
             token = it.q_token + row // group
             lo, hi = keys(it, token)
-            entry = (token, row % group, it.source, it.key0, lo, max(lo, hi))
+            entry = (token, row % group, it.key0, lo, max(lo, hi))
             if it.part == DIRECT:
                 assert (token, row % group) not in written
                 written[token, row % group] = [entry]
@@ -153,11 +154,10 @@ def covered(got, seqs, heads, kv_heads, hd, window, prefix):
             lo, hi = visible(i, q_len, kv_len, prefix, window)
             for g in range(group):
                 ranges = []
-                for _, _, source, key0, a, b in written.pop((q0 + i, g)):
-                    assert key0 == (0 if source else k0)
+                for _, _, key0, a, b in written.pop((q0 + i, g)):
                     if b > a:
-                        assert b <= (prefix if source else kv_len)
-                        ranges.append((a, b) if source else (a + prefix, b + prefix))
+                        assert b <= prefix + kv_len and (b <= prefix or key0 == k0)
+                        ranges.append((a, b))
                 ranges.sort()
                 for (_, b), (a, _) in zip(ranges, ranges[1:]):
                     assert a == b
@@ -194,8 +194,15 @@ def test_prefix(ctx, memory, heads, kv_heads, hd, window):
 def test_a_batch_reads_its_prefix_once(ctx, memory):
     seqs = [(i, 1, 10 * i, 10) for i in range(32)]
     got = call(ctx, memory, seqs, 32, 8, 128, 0, 4096)
-    shared = [it for it in got.items if it.source]
+    shared = [it for it in got.items if it.k_lo < 4096]
     assert all(it.n_rows == 128 for it in shared) and sum(it.k_hi - it.k_lo for it in shared) == 4096
+
+
+def test_a_short_prefix_needs_no_parts(ctx, memory):
+    """Where fewer tiles over the prefix save less than the joins cost, each text takes prefix and own keys in one item."""
+    for seqs, prefix in (([(i, 1, 10 * i, 10) for i in range(32)], 100), ([(60 * i, 60, 60 * i, 60) for i in range(32)], 400)):
+        got = call(ctx, memory, seqs, 32, 8, 128, 0, prefix)
+        assert not got.joins and all(it.part == DIRECT and it.k_lo == 0 and it.k_hi > prefix for it in got.items)
 
 
 @pytest.mark.parametrize("seed", range(12))

@@ -191,6 +191,23 @@ def test_prefix_of_texts(ctx, heads, kv_heads, hd, kind, window):
     attend(ctx, seqs, heads, kv_heads, hd, kind, window=window, prefix=333, seed=3)
 
 
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("heads,kv_heads,hd", LAYOUTS)
+@pytest.mark.parametrize("window", [0, 37, 150])
+def test_a_text_behind_a_prefix(ctx, heads, kv_heads, hd, kind, window):
+    """Key blocks end at the prefix's last row; NaN and infinities beside the sequence's keys and in values some rows see."""
+    def edit(t):
+        for row, col in ((80, 0), (99, hd - 1)):
+            t["pv"][row, col] = BITS[kind]["nan"]
+        t["v"][5, 1], t["v"][120, 0], t["k"][125:] = BITS[kind]["inf"], BITS[kind]["ninf"], BITS[kind]["nan"]
+        t["k"][:2] = t["v"][:2] = BITS[kind]["nan"]
+
+    seqs = [(0, 123, 2, 123), (123, 4, 2, 1), (127, 0, 125, 3)]
+    attend(ctx, seqs, heads, kv_heads, hd, kind, window=window, prefix=101, seed=21, edit=edit)
+    seqs = [(0, 1, 0, 9), (1, 1, 9, 0), (2, 30, 20, 30)]
+    attend(ctx, seqs, heads, kv_heads, hd, kind, window=window, prefix=101, seed=22)
+
+
 @pytest.mark.parametrize("heads,kv_heads,hd", LAYOUTS)
 def test_queries_before_their_first_key(ctx, heads, kv_heads, hd):
     """Rows that see no key come out as zeros."""
