@@ -271,6 +271,10 @@ def test_refused_pointers(ctx, memory):
             ctx.attention_prefix(shape, memory, pk, pv, 5, memory, memory, seqs, memory)
     with pytest.raises(ge.GemmaEmbedError):
         ctx.attention_prefix(shape, memory, memory, memory, -1, memory, memory, seqs, memory)
+    half = ge.attention_shape(ge.GE_TYPE_F16, 2, 1, 128, 4, 1 << 29)
+    with pytest.raises(ge.GemmaEmbedError) as e:  # key rows and prefix together
+        ctx.attention_prefix(half, memory, memory, memory, 1 << 29, memory, memory, seqs, memory)
+    assert e.value.code == ge.GE_ERR_INVALID and "prefix together" in e.value.message
     assert lib.ge_op_attention_causal(ctx.handle, None, memory, memory, memory, None, 0, memory) == ge.GE_ERR_INVALID
     assert lib.ge_op_attention_causal(ctx.handle, C.byref(shape), memory, memory, memory, None, 1, memory) == ge.GE_ERR_INVALID
     assert lib.ge_op_attention_causal(None, C.byref(shape), memory, memory, memory, None, 0, memory) == ge.GE_ERR_INVALID
