@@ -19,7 +19,8 @@
 // 2^6 higher in fp16, which uses its range up to 2^14 and keeps keys of 2^-30 of the maximum, and 2^8 lower in
 // bf16, whose values may themselves be near fp32's largest. Rounding P to
 // the inputs' type (half a step, 2^-11 or 2^-8 of a weight at most) is what the matrix instruction
-// takes; the sum of the weights is fp32, of P before rounding.
+// takes; the sum of the weights is fp32, of P as rounded, so that a row is a mean of the values it sees: with P
+// before rounding, 1 to 3% of the results of values that are all the type's largest were infinite.
 //
 // Bounds. Long prompts: the matrix instructions, at the clock the card's power leaves them (16384 tokens, 32
 // heads of 128 over 8: 2.04 to 2.16 ms, 1.02 to 1.08 PFLOP/s of visible pairs; the pipe 59% busy at 1.5 GHz).
@@ -47,6 +48,10 @@ struct F16 {
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         return __builtin_bit_cast(uint32_t, half2_t{_Float16(x), _Float16(y)});
     }
+    // sum + the packed pair's two values
+    static __device__ __forceinline__ float add(uint32_t pair, float sum) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, pair), half2_t{_Float16(1), _Float16(1)}, sum, false);
+    }
     static __device__ __forceinline__ float value(uint16_t x) { return h2f(x); }
     static constexpr float kRaise = 6.0f;
     static constexpr uint32_t kNonFinite = 0x04000400u;
@@ -57,6 +62,9 @@ struct BF16 {
     }
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         return __builtin_bit_cast(uint32_t, bf16x2_t{__bf16(x), __bf16(y)});
+    }
+    static __device__ __forceinline__ float add(uint32_t pair, float sum) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), bf16x2_t{__bf16(1.0f), __bf16(1.0f)}, sum, false);
     }
     static __device__ __forceinline__ float value(uint16_t x) { return __uint_as_float(uint32_t(x) << 16); }
     static constexpr float kRaise = -8.0f;
@@ -251,19 +259,20 @@ struct Rows {
                 w.m = m_new;
             }
             const float ref = w.m == -INFINITY ? 0.0f : T::kRaise - w.m;
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], c, ref));
             float sum = 0.0f;
 #pragma unroll
             for (int t = 0; t < KT; t++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], c, ref));
-                    sum += s[t][e];
+                for (int e = 0; e < 16; e += 2) {
+                    const uint32_t pair = T::pack(s[t][e], s[t][e + 1]);
+                    p[2 * t + e / 8][(e % 8) / 2] = pair;
+                    sum = T::add(pair, sum);
                 }
             w.l += sum;
-#pragma unroll
-            for (int t = 0; t < KT; t++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) p[2 * t + e / 8][(e % 8) / 2] = T::pack(s[t][e], s[t][e + 1]);
         }
 
         // V^T's fragment of 32 dims d and 16 keys t: keys 16 t + 8 j + 4 (lane / 32) + [0, 4) at slots 4 j.
