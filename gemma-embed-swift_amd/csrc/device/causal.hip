@@ -16,8 +16,9 @@
 //     16-key steps when V^T's keys are taken in that order; V^T comes from V's rows in LDS by the
 //     transposing LDS read (4 keys x 16 dims a read of 16 lanes), so no transposed copy of V exists.
 // The running maximum moves only when a score passes it by 8 (in log2), as in attention.hip. P is taken
-// 2^6 higher in fp16, which uses its range up to 2^14 and keeps keys of 2^-30 of the maximum, and 2^8 lower in
-// bf16, whose values may themselves be near fp32's largest. Rounding P to
+// 2^6 higher in fp16, which uses its range up to 2^14 and keeps keys of 2^-30 of the maximum, and 2^32 lower in
+// bf16, whose values may themselves be fp32's largest: the sum of 2^24 of them, each 8 above the maximum, stays
+// in range, and so do keys of 2^-94 of the maximum over ordinary values. Rounding P to
 // the inputs' type (half a step, 2^-11 or 2^-8 of a weight at most) is what the matrix instruction
 // takes; the sum of the weights is fp32, of P as rounded, so that a row is a mean of the values it sees: with P
 // before rounding, 1 to 3% of the results of values that are all the type's largest were infinite.
@@ -67,7 +68,7 @@ struct BF16 {
         return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), bf16x2_t{__bf16(1.0f), __bf16(1.0f)}, sum, false);
     }
     static __device__ __forceinline__ float value(uint16_t x) { return __uint_as_float(uint32_t(x) << 16); }
-    static constexpr float kRaise = -8.0f;
+    static constexpr float kRaise = -32.0f;
     static constexpr uint32_t kNonFinite = 0x00800080u;
 };
 
