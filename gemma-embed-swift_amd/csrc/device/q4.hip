@@ -10,6 +10,10 @@
 // group. Row m of x stands at A's row 4 (m % 4) + m / 4, so that up to 4 rows fill the accumulators'
 // first register only, 8 the first two, and the others are left out of the scaling.
 // The waves of a workgroup take the column tiles in turn and join through LDS.
+//
+// Those steps leave fp32's range where the products w x need not: an infinite x as inf - inf between a product and
+// the sum of x that corrects it, and bf16 x from 2^118 on times the integers, 31 times its size in 32 columns.
+// A sum that comes out infinite or NaN is therefore taken again from the products themselves, in 64 bits.
 #include "common.hpp"
 #include "q4.hpp"
 
@@ -43,6 +47,7 @@ struct F16 {
     static __device__ __forceinline__ float4_t mfma(u32x4 a, u32x4 b, float4_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
     }
+    static __device__ __forceinline__ float value(uint16_t x) { return h2f(x); }
     static constexpr float kOffset = 0.0f;
     static constexpr uint32_t kOnes = 0x3c003c00u, kMinus24 = 0;
 };
@@ -57,6 +62,7 @@ struct BF16 {
     static __device__ __forceinline__ float4_t mfma(u32x4 a, u32x4 b, float4_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     }
+    static __device__ __forceinline__ float value(uint16_t x) { return __uint_as_float(uint32_t(x) << 16); }
     static constexpr float kOffset = 16.0f;
     static constexpr uint32_t kOnes = 0x3f803f80u, kMinus24 = 0xc1c0c1c0u;
 };
@@ -100,6 +106,25 @@ __device__ __forceinline__ void store(void* y, size_t at, float v) {
         static_cast<_Float16*>(y)[at] = _Float16(v);
     else
         static_cast<__bf16*>(y)[at] = __bf16(v);
+}
+
+// sum_k x[k] w[n][k] of one row of x and one of the weights from its definition.
+template <typename T, bool MIN>
+__device__ __forceinline__ float product_again(const Q4Dev& w, const uint16_t* x, int n) {
+    double sum = 0.0;
+    for (int group = 0; group < w.cols / 32 && sum == sum; group++) {
+        const size_t tile = size_t(n >> 4) * w.tiles + (group >> 2);
+        const int at = (n & 15) * 4 + (group & 3);
+        const double d = double(h2f(w.d[tile * 64 + at])), m = MIN ? double(h2f(w.m[tile * 64 + at])) : 0.0;
+        for (int quad = 0; quad < 4; quad++) {
+            const uint32_t q = w.q[tile * 256 + quad * 64 + at];
+            for (int e = 0; e < 8; e++) {
+                const int v = int((q >> (4 * (e & 1 ? 4 + e / 2 : e / 2))) & 15u) - (MIN ? 0 : 8);
+                sum += (d * double(v) + m) * double(T::value(x[group * 32 + quad * 8 + e]));
+            }
+        }
+    }
+    return float(sum);
 }
 
 // What a wave reads of one column tile: its dwords of the weights, the scales (and minima) of its row's
@@ -252,6 +277,7 @@ __global__ __launch_bounds__(512) void gemv_q4_kernel(const Q4Args a) {
         leave(SUMS > 1 && count > first ? wave + kQ4Waves<XLDS> : wave);
         __syncthreads();
     }
+    uint32_t again = 0;  // this lane's results of which a sum is not finite
 #pragma unroll
     for (int j = 0; j < RB * NT; j++) {
         if (j % waves != wave) continue;
@@ -270,8 +296,20 @@ __global__ __launch_bounds__(512) void gemv_q4_kernel(const Q4Args a) {
             }
             const float y = MATS == 2 ? gelu_tanh(sum[0]) * sum[MATS - 1] : sum[0];
             const int r = r0 + 16 * t + quad + 4 * e;
-            if (r < a.rows && n < a.w.rows) store<OUT>(a.y, size_t(r) * a.w.rows + n, y);
+            if (r < a.rows && n < a.w.rows) {
+                store<OUT>(a.y, size_t(r) * a.w.rows + n, y);
+                if (!__builtin_isfinite(sum[0]) || (MATS == 2 && !__builtin_isfinite(sum[MATS - 1]))) again |= 1u << (j * MR + e);
+            }
         }
+    }
+    static_assert(RB * NT * MR <= 32, "a bit a result");
+    for (; again; again &= again - 1) {
+        const int at = __builtin_ctz(again), j = at / MR, e = at % MR;
+        const int n = (int(blockIdx.x) * RB + j / NT) * 16 + (lane & 15), r = r0 + 16 * (j % NT) + quad + 4 * e;
+        const uint16_t* const row = a.x + size_t(r) * cols;
+        float y = product_again<T, MIN>(a.w, row, n);
+        if (MATS == 2) y = gelu_tanh(y) * product_again<T, MIN>(a.up, row, n);
+        store<OUT>(a.y, size_t(r) * a.w.rows + n, y);
     }
 }
 

@@ -200,9 +200,13 @@ int ge_op_q4_create(ge_ctx* ctx, const void* q4_rows, int32_t type, int32_t rows
 int ge_op_q4_destroy(ge_ctx* ctx, ge_q4_matrix* m);
 
 /* y[M][N] = x[M][K] * W^T with W [N][K] in 4 bits: x of x_type GE_TYPE_F16 or GE_TYPE_BF16, y of y_type
- * GE_TYPE_F32, GE_TYPE_F16 or GE_TYPE_BF16, rows back to back, 16-byte aligned. The weights enter as the
- * integers they are and the sums are fp32: y is rounded once, to its type. Any M up to 2^19 (the weights
- * are read once for every 16, 32 or 64 rows). */
+ * GE_TYPE_F32, GE_TYPE_F16 or GE_TYPE_BF16, rows back to back, 16-byte aligned; y overlaps none of the inputs.
+ * The weights enter as the integers they are, the sums are fp32, and y is rounded once, to its type. With F16 x
+ * the sums' error is in steps of 2^-24 of sum_k |x_k| |d| (q + 8) (Q4_1: + |m|); with BF16 x the integers are taken as
+ * 16 + q and the sum of x times 24 (Q4_1: 16) off again, so that it is of sum_k |x_k| |d| (q + 40) (+ |m|). Infinities
+ * and NaN come out as sum_k x_k w_k has them, and a sum that leaves fp32's range on the way only, with BF16 x from
+ * 2^118 on, is taken again in 64 bits. Any M up to 2^19 (the weights are read once for every 16, 32 or 64
+ * rows). */
 int ge_op_gemv_q4(ge_ctx* ctx, const ge_q4_matrix* w, const void* x, int32_t x_type, int32_t m, void* y, int32_t y_type);
 /* The same with the geglu epilogue: act[M][F] = gelu_tanh(x * Wg^T) * (x * Wu^T), gate and up of one shape
  * and type. */
