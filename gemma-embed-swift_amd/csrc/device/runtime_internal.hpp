@@ -224,6 +224,8 @@ template <typename F>
 int guarded(ge_ctx* c, F&& f) {
     if (!c) return GE_ERR_INVALID;
     try {
+        // The launches read the thread's last error, which an earlier call that was refused (an allocation) leaves set.
+        (void)hipGetLastError();
         hipError_t e = hipSetDevice(c->device);
         if (e != hipSuccess) fail(GE_ERR_GPU, "GPU execution failed: hipSetDevice: %s", hipGetErrorString(e));
         f();
