@@ -82,11 +82,13 @@ int64_t tile_eighths(const Plan& p, int64_t rows) {
 // (written, and read by the joining launch). Of no split and splits into about 1, 1.5, 2 and 3 items a CU the
 // one whose estimate is least, in microseconds: a key of an item of head dim 128 takes 0.025 with one
 // workgroup on a CU and 0.6 of that each with two (narrow items, which wait for memory, gain nothing by
-// pairs), an item 7 besides its keys, a joining launch 5 and 1 for 3 MB of parts. Calls of few or many
-// items (under 128 keys each, four a CU unsplit) are not split. Measured, us a call unsplit / 1 / 1.5 / 2 / 3
+// pairs), an item 7 besides its keys, a joining launch 5 and 1 for 3 MB of parts. Calls of short
+// items (up to 128 keys) and of many even ones (four a CU unsplit, the longest no more than a CU's share of all) are
+// not split. Measured, us a call unsplit / 1 / 1.5 / 2 / 3
 // items a CU: one token over 20000 keys (32 heads of 128 over 8) 178 / 35 / 38 / 41 / 46, 48 tokens over 100
 // to 8000 189 / 188 / 165 / 166 / 165, 128 texts over a prefix of 8192 (3 heads of 256) 332 / 200 / 178 / 215 /
-// 203, one prompt of 2048 (32 heads of 128) 67 / 67 / 78 / 83 / 84.
+// 203, one prompt of 2048 (32 heads of 128) 67 / 67 / 78 / 83 / 84. A token over 32768 keys beside 127 over
+// 100: 293 unsplit, 54 split.
 int64_t split_limit(const Plan& p, int kv_heads, int head_dim) {
     constexpr int kBins = 64;
     const float key_us = wide_key_us(head_dim);
@@ -97,8 +99,10 @@ int64_t split_limit(const Plan& p, int kv_heads, int head_dim) {
         wide_keys += narrow(t) ? 0 : n;
         longest = std::max(longest, n);
     }
-    if (longest <= kSplitMinKeys || int64_t(p.tiles.size()) * kv_heads >= 4 * kCus) return std::max<int64_t>(longest, 64);
     const float pair = 2 * wide_keys >= total ? 0.6f : 1.0f;
+    if (longest <= kSplitMinKeys ||
+        (int64_t(p.tiles.size()) * kv_heads >= 4 * kCus && float(longest) <= float(total * kv_heads) * pair / kCus))
+        return std::max<int64_t>(longest, 64);
     int64_t best = longest;
     float best_us = 1e30f;
     for (const float per_cu : {0.0f, 1.0f, 1.5f, 2.0f, 3.0f}) {
