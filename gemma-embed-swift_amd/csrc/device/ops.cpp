@@ -47,7 +47,7 @@ unsigned char* op_lists(ge_ctx* c, size_t bytes) {
         if (c->op_host) hip_check(hipHostFree(c->op_host), "hipHostFree");
         c->op_host = nullptr;
         c->op_host_cap = 0;
-        const size_t cap = std::max<size_t>(2 * bytes, 64 << 10);
+        const size_t cap = std::max(bytes, std::min(std::max<size_t>(2 * bytes, 64 << 10), kOpListsKept));
         hip_check(hipHostMalloc(&c->op_host, cap, hipHostMallocDefault), "hipHostMalloc");
         c->op_host_cap = cap;
     }
@@ -63,6 +63,12 @@ OpTemps::~OpTemps() {
         (void)hipFree(c_->op_buf);
         c_->op_buf = nullptr;
         c_->op_cap = 0;
+    }
+    if (c_->op_host_cap > kOpListsKept) {
+        (void)hipStreamSynchronize(c_->stream);
+        (void)hipHostFree(c_->op_host);
+        c_->op_host = nullptr;
+        c_->op_host_cap = 0;
     }
 }
 

@@ -211,7 +211,8 @@ struct ge_ctx {
     void* op_buf = nullptr;
     size_t op_cap = 0;
     bool causal_ready = false;  // causal_configure() has run (causal.cpp)
-    // Pinned memory of one per-op call's work lists (op_lists), which its kernels read in place.
+    // Pinned memory of one per-op call's work lists (op_lists), which its kernels read in place, kept up to
+    // kOpListsKept bytes.
     void* op_host = nullptr;
     size_t op_host_cap = 0;
 };
@@ -270,9 +271,10 @@ private:
     const int unwinding_ = std::uncaught_exceptions();
 };
 // At least `bytes` of the context's pinned memory, for work lists written by the host and read by the
-// call's kernels where they are: a list is read once, by one lane of a workgroup, and a copy to device
-// memory would be one more operation ahead of the kernel. The same rules as OpTemps make it free again
-// when the call returns.
+// call's kernels where they are: an entry is read at the start of each workgroup that it is for, and a copy to
+// device memory would be one more operation ahead of the kernel. The same rules as OpTemps make it free again
+// when the call returns; take it after the call's OpTemps, whose end gives it back from kOpListsKept bytes on.
+constexpr size_t kOpListsKept = size_t(16) << 20;
 unsigned char* op_lists(ge_ctx* c, size_t bytes);
 hipEvent_t take_event(ge_ctx* c);
 
