@@ -167,8 +167,8 @@ int ge_profile_get(ge_ctx* ctx, int32_t i, const char** name, int64_t* launches,
 
 /* ---- per-op entry points on device memory, for unit tests (the reference's `Kernels`,
  * Metal/MetalForward.swift:427-759). Device buffers come from ge_dev_alloc. A context keeps the temporary memory
- * of its largest call so far for the next ones: up to 512 MiB of device memory, and up to 16 MiB of pinned host
- * memory for work lists; what a call takes beyond that is given back when it returns, the rest by ge_destroy. */
+ * of its largest call so far for the next ones, up to 512 MiB of device memory and up to 16 MiB of pinned host
+ * memory for work lists; a call that takes more of either gives it back when it returns. ge_destroy frees the rest. */
 void* ge_dev_alloc(ge_ctx* ctx, size_t bytes);
 int ge_dev_free(ge_ctx* ctx, void* ptr);
 int ge_dev_upload(ge_ctx* ctx, void* dst, const void* src, size_t bytes);
