@@ -700,6 +700,10 @@ def attention_seqs(sequences) -> np.ndarray:
             and sequences.shape[1] == 4:
         return sequences
     s = np.asarray(sequences)
+    if s.size and not np.issubdtype(s.dtype, np.integer):
+        raise TypeError(f"a sequence is four whole numbers, not {s.dtype}")
+    if s.ndim > 2 or (s.size and s.ndim == 2 and s.shape[1] != 4):
+        raise ValueError(f"sequences of four numbers each, not an array of shape {s.shape}")
     if s.dtype != np.uint32:
         if s.size and (s.min() < 0 or s.max() > 0xffffffff):
             raise OverflowError("a sequence's rows are counted in 32 bits")
