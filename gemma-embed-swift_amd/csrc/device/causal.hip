@@ -24,7 +24,7 @@
 // before rounding, 1 to 3% of the results of values that are all the type's largest were infinite.
 //
 // Bounds. Long prompts: the matrix instructions, at the clock the card's power leaves them (16384 tokens, 32
-// heads of 128 over 8: 2.04 to 2.16 ms, 1.02 to 1.08 PFLOP/s of visible pairs; the pipe 59% busy at 1.5 GHz).
+// heads of 128 over 8: 2.04 to 2.16 ms, 1.02 to 1.08 PFLOP/s of visible pairs; the pipe 55% busy at 1.6 GHz).
 // Single tokens: HBM (48 over caches of up to 8000 keys: 145 us, 5.4 TB/s). Small calls: a chain of reads, the
 // item, q and the first keys, and the stores, 6 to 7 us.
 #include "causal.hpp"
