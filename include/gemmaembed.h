@@ -293,7 +293,7 @@ int ge_op_attention_split(ge_ctx* ctx, const void* q, const void* q_lo, const vo
  * Limits: heads a multiple of kv_heads, up to 4096; head_dim 64, 128, 256 or 512; buffers 16-byte aligned;
  * strides a multiple of 8 up to 2^24; query rows, the window, and key rows and prefix together under 2^30.
  * Scores, softmax and sums are in fp32; the softmax weights are rounded to the operands' type before the
- * product with V. */
+ * product with V and their sum, so that a result is a mean of the values its query sees. */
 typedef struct ge_attention_shape {
     int32_t type;
     int32_t heads, kv_heads, head_dim;
@@ -314,7 +314,8 @@ typedef struct ge_attention_seq {
  * query at the last key: j <= i + kv_len - q_len and, with a window, j > i + kv_len - q_len - window. So
  * q_len = kv_len is a prompt, a shorter q_len a chunk or (1) the next token over cached keys. A query
  * that sees no key gets zeros. What a query does not see does not reach its row, infinities and NaN
- * included. Rows of out outside the sequences stay as they were. */
+ * included; an infinity or NaN in a value that it sees makes its result in that column infinite or NaN. Rows of out
+ * outside the sequences stay as they were. */
 int ge_op_attention_causal(ge_ctx* ctx, const ge_attention_shape* shape, const void* q, const void* k, const void* v,
                            const ge_attention_seq* seqs, int32_t n_seqs, void* out);
 
