@@ -1,0 +1,397 @@
+// Norms and rotary positions of query and key heads, rows to rows or keys and values to their pages (gfx950).
+//   y = x / sqrt(mean(x^2) + eps) w over a head (where normed), then for each pair (a, b) of its first 2 `half`
+//   elements, at angle t = 2 pi position turns[i]:  (a cos t - b sin t, a sin t + b cos t) magnitude.
+//
+// One pass: a group of lanes holds a head from its load to its store, in fp32, and rounds once. The angle is
+// reduced in fp64 (a position of 2^31 keeps 2^-22 of a turn) and its sine and cosine taken in fp32, each once a row
+// for all heads: the wave's lanes take a pair each and share them through LDS.
+//
+// What bounds it: the bytes of long calls, the chain of one load, one reduction and one store in short ones.
+#include "common.hpp"
+#include "half_types.hpp"
+#include "rotary.hpp"
+
+namespace ge {
+namespace {
+
+struct F32 {
+    static __device__ __forceinline__ float value(float x) { return x; }
+};
+
+template <typename T>
+struct StoredAs {
+    typedef uint16_t Type;
+};
+template <>
+struct StoredAs<F32> {
+    typedef float Type;
+};
+
+// The pieces of a head that a lane holds: N elements of `a` and as many of `b`, the pairs' two sides where
+// they turn.
+// Wide: one 16-byte-aligned unit of 8 + 8 elements a lane, head_dim / 16 lanes a head (a power of two of
+// lanes, so that several heads stand side by side in a wave). Narrow, for head dims, parts, strides and
+// addresses that are not in such pieces: single elements, the whole wave on a head.
+template <bool WIDE>
+struct Shape {
+    static constexpr int N = WIDE ? 8 : 4, kIts = WIDE ? 4 : 2;  // kIts: groups of heads of one task, loaded together
+};
+
+// log2 of the lanes a head takes.
+template <bool WIDE>
+__device__ __forceinline__ int lanes_log(int head_dim) {
+    return WIDE ? (head_dim <= 16 ? 0 : 32 - __builtin_clz(uint32_t(head_dim / 16 - 1))) : 6;
+}
+
+// The sum over groups of 2^log lanes: halves of a group hold equal sums, so that a mirrored move is as
+// good as the exchange.
+__device__ __forceinline__ float group_sum(float v, int log) {
+    if (log >= 1) v += dpp_move<0xb1>(v);   // quad_perm 1, 0, 3, 2
+    if (log >= 2) v += dpp_move<0x4e>(v);   // quad_perm 2, 3, 0, 1
+    if (log >= 3) v += dpp_move<0x141>(v);  // row_half_mirror
+    if (log >= 4) v += dpp_move<0x140>(v);  // row_mirror
+    if (log >= 5) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    }
+    if (log >= 6) {
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    }
+    return v;
+}
+
+// Where a lane's elements lie in a head: a's first element and, `step` apart, its others (step 1 wide, 0
+// past the head's end); b likewise; the first pair, or -1 where they do not turn.
+template <bool WIDE>
+struct Place {
+    static constexpr int N = Shape<WIDE>::N;
+    int a[WIDE ? 1 : N], b[WIDE ? 1 : N], pair[WIDE ? 1 : N];
+    bool any;  // wide: the lane has a unit; narrow: a unit has index < head_dim / 2
+
+    __device__ __forceinline__ void init(const HeadsArgs& h, int lane_of_head) {
+        constexpr int E = WIDE ? 8 : 1;
+        any = false;
+#pragma unroll
+        for (int j = 0; j < (WIDE ? 1 : N); j++) {
+            const int u = (lane_of_head + 64 * j) * E;  // the unit's first pair
+            const bool in = u < h.head_dim / 2, turns = u < h.half;
+            any = any || in;
+            pair[j] = in && turns ? u : -1;
+            a[j] = !in ? -1 : turns && !h.pairs ? u : 2 * u;
+            b[j] = !in ? -1 : turns && !h.pairs ? h.half + u : 2 * u + E;
+        }
+    }
+};
+
+template <typename T, bool WIDE>
+struct Raw {
+    typedef typename StoredAs<T>::Type Stored;
+    static constexpr int N = Shape<WIDE>::N, kPieces = WIDE ? int(8 * sizeof(Stored) / 16) : 1;
+    u32x4 wa[kPieces], wb[kPieces];
+    Stored na[WIDE ? 1 : N], nb[WIDE ? 1 : N];
+
+    __device__ __forceinline__ void load(const Stored* p, const Place<WIDE>& at) {
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int i = 0; i < kPieces; i++) {
+                wa[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(p + at.a[0]) + 16 * i);
+                wb[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(p + at.b[0]) + 16 * i);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (at.a[j] >= 0) {
+                    na[j] = p[at.a[j]];
+                    nb[j] = p[at.b[j]];
+                } else {
+                    na[j] = nb[j] = Stored(0);
+                }
+        }
+    }
+    __device__ __forceinline__ void clear() {
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int i = 0; i < kPieces; i++) wa[i] = wb[i] = u32x4{};
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) na[j] = nb[j] = Stored(0);
+        }
+    }
+    static __device__ __forceinline__ float piece(const u32x4 (&w)[kPieces], int i) {
+        if constexpr (sizeof(Stored) == 4)
+            return __uint_as_float(w[i / 4][i % 4]);
+        else
+            return T::value(uint16_t(w[0][i / 2] >> (16 * (i % 2))));
+    }
+    __device__ __forceinline__ void values(float (&a)[N], float (&b)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if constexpr (WIDE) {
+                a[i] = piece(wa, i);
+                b[i] = piece(wb, i);
+            } else {
+                a[i] = T::value(na[i]);
+                b[i] = T::value(nb[i]);
+            }
+        }
+    }
+};
+
+template <bool WIDE>
+__device__ __forceinline__ void load_weights(const float* w, const Place<WIDE>& at, float (&a)[Shape<WIDE>::N], float (&b)[Shape<WIDE>::N]) {
+    constexpr int N = Shape<WIDE>::N;
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4_t x = *reinterpret_cast<const float4_t*>(w + at.a[0] + i), y = *reinterpret_cast<const float4_t*>(w + at.b[0] + i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                a[i + j] = x[j];
+                b[i + j] = y[j];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            a[j] = at.a[j] >= 0 ? w[at.a[j]] : 0.0f;
+            b[j] = at.b[j] >= 0 ? w[at.b[j]] : 0.0f;
+        }
+    }
+}
+
+template <typename O, bool WIDE>
+__device__ __forceinline__ void store(uint16_t* p, const Place<WIDE>& at, const float (&a)[Shape<WIDE>::N], const float (&b)[Shape<WIDE>::N]) {
+    if constexpr (WIDE) {
+        *reinterpret_cast<u32x4*>(p + at.a[0]) = u32x4{O::pack(a[0], a[1]), O::pack(a[2], a[3]), O::pack(a[4], a[5]), O::pack(a[6], a[7])};
+        *reinterpret_cast<u32x4*>(p + at.b[0]) = u32x4{O::pack(b[0], b[1]), O::pack(b[2], b[3]), O::pack(b[4], b[5]), O::pack(b[6], b[7])};
+    } else {
+#pragma unroll
+        for (int j = 0; j < Shape<WIDE>::N; j++)
+            if (at.a[j] >= 0) {
+                p[at.a[j]] = uint16_t(O::pack(a[j], 0.0f));
+                p[at.b[j]] = uint16_t(O::pack(b[j], 0.0f));
+            }
+    }
+}
+
+// x / sqrt(mean(x^2) + eps). Squares that leave fp32's range, or get lost below it where eps does not
+// outweigh them, are taken of x times a power of two.
+template <int N>
+__device__ __forceinline__ void norm(float (&a)[N], float (&b)[N], bool on, int log, float inv_dim, float eps) {
+    auto squares = [&] {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; i++) ss = __builtin_fmaf(a[i], a[i], __builtin_fmaf(b[i], b[i], ss));
+        return group_sum(ss, log);
+    };
+    float ss = squares(), e = eps;
+    const bool large = on && !(ss <= 1e37f), small = on && ss < 0x1p-60f && eps < 0x1p-100f;
+    if (__builtin_amdgcn_ballot_w64(large || small)) {
+        const float f = large ? 0x1p-100f : small ? 0x1p80f : 1.0f;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            a[i] *= f;
+            b[i] *= f;
+        }
+        e = eps * f * f;
+        ss = squares();
+    }
+    const float r = on ? 1.0f / sqrtf(__builtin_fmaf(ss, inv_dim, e)) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        a[i] *= r;
+        b[i] *= r;
+    }
+}
+
+// I: the input type; O: the results'. A workgroup has an item's rows, or (not appending) rows_each rows; its
+// waves take tasks of a row and up to kIts groups of heads.
+template <typename I, typename O, bool WIDE, bool APPEND>
+__device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem& it) {
+    constexpr int N = Shape<WIDE>::N, kIts = Shape<WIDE>::kIts;
+    typedef typename StoredAs<I>::Type Stored;
+    __shared__ float2 shared[WIDE ? 4 * 256 : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+    const int log = lanes_log<WIDE>(h.head_dim), at_once = 64 >> log;
+    const int all = h.heads + (APPEND ? 2 : 1) * h.kv_heads;
+    const int groups = (all + at_once - 1) / at_once, chunks = (groups + kIts - 1) / kIts, each = (groups + chunks - 1) / chunks;
+    Place<WIDE> at;
+    at.init(h, lane & ((1 << log) - 1));
+    const float inv_dim = 1.0f / float(h.head_dim);
+    float2* const mine = shared + (WIDE ? wave * 256 : 0);
+
+    for (int task = wave; task < int(it.n) * chunks; task += 4) {
+        const int r = task / chunks, group0 = task % chunks * each;
+        const size_t row = size_t(it.row0) + uint32_t(r);
+        Raw<I, WIDE> raw[kIts];
+#pragma unroll
+        for (int i = 0; i < kIts; i++) {
+            const int head = (group0 + i) * at_once + (lane >> log);
+            if (i < each && head < all && at.any) {
+                const bool q = head < h.heads, k = head < h.heads + h.kv_heads;
+                const Stored* const p = static_cast<const Stored*>(q ? h.q : k ? h.k : h.v) +
+                                        row * size_t(q ? h.q_stride : k ? h.k_stride : h.v_stride) +
+                                        size_t(q ? head : k ? head - h.heads : head - h.heads - h.kv_heads) * size_t(h.head_dim);
+                raw[i].load(p, at);
+            } else {
+                raw[i].clear();
+            }
+        }
+        size_t page_at = 0;  // of the row, in its page's first head
+        if constexpr (APPEND) {
+            const uint32_t key = it.first + uint32_t(r);
+            const int32_t page = h.table[size_t(it.slot) * size_t(h.slot_pages) + (key >> h.page_shift)];
+            page_at = size_t(page) * size_t(h.page_stride) + size_t(key & ((1u << h.page_shift) - 1)) * size_t(h.head_dim);
+        }
+        float cs[N], sn[N];
+        if (h.half) {
+            const double position = h.positions ? double(h.positions[row]) : double(it.first + uint32_t(r));
+            auto turn = [&](int pair, float& c, float& s) {
+                const double t = position * h.turns[pair];
+                sincospif(2.0f * float(t - rint(t)), &s, &c);
+                c *= h.fade;
+                s *= h.fade;
+            };
+            if constexpr (WIDE) {
+                for (int pair = lane; pair < h.half; pair += 64) turn(pair, mine[pair].x, mine[pair].y);
+                __builtin_amdgcn_wave_barrier();
+                const int first = at.pair[0] < 0 ? 0 : at.pair[0];
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const float2 x = mine[first + i];
+                    cs[i] = x.x;
+                    sn[i] = x.y;
+                }
+                __builtin_amdgcn_wave_barrier();
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; j++) turn(at.pair[j] < 0 ? 0 : at.pair[j], cs[j], sn[j]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kIts; i++) {
+            if (i >= each || (group0 + i) * at_once >= all) continue;
+            const int head = (group0 + i) * at_once + (lane >> log);
+            const bool q = head < h.heads, k = head < h.heads + h.kv_heads;
+            float a[N], b[N];
+            raw[i].values(a, b);
+            if (h.normed) {
+                const bool on = (h.normed & (q ? kNormQ : k ? kNormK : kNormV)) != 0 && head < all;
+                norm(a, b, on, log, inv_dim, h.eps);
+                const float* const w = q ? h.q_norm : k ? h.k_norm : nullptr;
+                if (on && w && at.any) {
+                    float wa[N], wb[N];
+                    load_weights<WIDE>(w, at, wa, wb);
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        a[j] *= wa[j];
+                        b[j] *= wb[j];
+                    }
+                }
+            }
+            if (h.half && k) {
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    if (at.pair[WIDE ? 0 : j] < 0) continue;
+                    if (WIDE && h.pairs) continue;
+                    const float x = a[j], y = b[j];
+                    a[j] = __builtin_fmaf(x, cs[j], -(y * sn[j])) * h.gain;
+                    b[j] = __builtin_fmaf(x, sn[j], y * cs[j]) * h.gain;
+                }
+                if constexpr (WIDE) {  // neighbours: pairs i of a and 4 + i of b
+                    if (h.pairs && at.pair[0] >= 0) {
+#pragma unroll
+                        for (int j = 0; j < N; j += 2) {
+                            const float x = a[j], y = a[j + 1], z = b[j], w = b[j + 1];
+                            a[j] = __builtin_fmaf(x, cs[j / 2], -(y * sn[j / 2])) * h.gain;
+                            a[j + 1] = __builtin_fmaf(x, sn[j / 2], y * cs[j / 2]) * h.gain;
+                            b[j] = __builtin_fmaf(z, cs[4 + j / 2], -(w * sn[4 + j / 2])) * h.gain;
+                            b[j + 1] = __builtin_fmaf(z, sn[4 + j / 2], w * cs[4 + j / 2]) * h.gain;
+                        }
+                    }
+                }
+            }
+            if (head >= all || !at.any) continue;
+            uint16_t* p;
+            if (q) {
+                p = h.q_out + row * size_t(h.q_out_stride) + size_t(head) * size_t(h.head_dim);
+            } else {
+                const size_t kvh = size_t(k ? head - h.heads : head - h.heads - h.kv_heads);
+                uint16_t* const out = k ? h.k_out : h.v_out;
+                if constexpr (APPEND)
+                    p = out + page_at + (kvh << h.page_shift) * size_t(h.head_dim);
+                else
+                    p = out + row * size_t(h.k_out_stride) + kvh * size_t(h.head_dim);
+            }
+            store<O, WIDE>(p, at, a, b);
+        }
+    }
+}
+
+template <typename I, typename O, bool WIDE>
+__global__ __launch_bounds__(256) void rotate_heads_kernel(const HeadsArgs h) {
+    const int row0 = int(blockIdx.x) * h.rows_each;
+    const AppendItem it{uint32_t(row0), uint32_t(min(h.rows_each, h.rows - row0)), 0, 0};
+    heads_body<I, O, WIDE, false>(h, it);
+}
+
+template <typename I, typename O, bool WIDE>
+__global__ __launch_bounds__(256) void append_kernel(const HeadsArgs h, const AppendInline in) {
+    const AppendItem* const p = h.items ? h.items + blockIdx.x : in.items + blockIdx.x;
+    const AppendItem it = *p;
+    heads_body<I, O, WIDE, true>(h, it);
+}
+
+__global__ __launch_bounds__(256) void table_set_kernel(int32_t* table, const uint2* entries, int n) {
+    const int i = int(blockIdx.x) * 256 + int(threadIdx.x);
+    if (i < n) table[entries[i].x] = int32_t(entries[i].y);
+}
+
+bool heads_ok(const HeadsArgs& a) {
+    return a.heads >= 0 && a.kv_heads >= 0 && a.heads + a.kv_heads > 0 && a.head_dim > 0 && a.head_dim <= 512 && a.head_dim % 2 == 0 &&
+           a.half >= 0 && a.half <= a.head_dim / 2 && a.rows >= 0;
+}
+
+template <typename I, typename O>
+hipError_t run_rotate(hipStream_t s, const HeadsArgs& a, bool wide) {
+    const dim3 grid(uint32_t((int64_t(a.rows) + a.rows_each - 1) / a.rows_each));
+    if (wide)
+        launch_kernel(rotate_heads_kernel<I, O, true>, grid, dim3(256), 0, s, a);
+    else
+        launch_kernel(rotate_heads_kernel<I, O, false>, grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+template <typename I, typename O>
+hipError_t run_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool wide) {
+    if (wide)
+        launch_kernel(append_kernel<I, O, true>, dim3(uint32_t(a.n_items)), dim3(256), 0, s, a, in);
+    else
+        launch_kernel(append_kernel<I, O, false>, dim3(uint32_t(a.n_items)), dim3(256), 0, s, a, in);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, bool bf16, bool wide) {
+    if (!heads_ok(a) || a.rows_each <= 0 || (a.half && !a.positions)) return hipErrorInvalidValue;
+    if (a.rows == 0) return hipSuccess;
+    if (in_f32) return bf16 ? run_rotate<F32, BF16>(s, a, wide) : run_rotate<F32, F16>(s, a, wide);
+    return bf16 ? run_rotate<BF16, BF16>(s, a, wide) : run_rotate<F16, F16>(s, a, wide);
+}
+
+hipError_t launch_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool in_f32, bool bf16, bool wide) {
+    if (!heads_ok(a) || a.n_items < 0 || (!a.items && a.n_items > kAppendInlineItems)) return hipErrorInvalidValue;
+    if (a.n_items == 0) return hipSuccess;
+    if (in_f32) return bf16 ? run_append<F32, BF16>(s, a, in, wide) : run_append<F32, F16>(s, a, in, wide);
+    return bf16 ? run_append<BF16, BF16>(s, a, in, wide) : run_append<F16, F16>(s, a, in, wide);
+}
+
+hipError_t launch_table_set(hipStream_t s, int32_t* table, const uint2* entries, int n) {
+    if (n <= 0) return n < 0 ? hipErrorInvalidValue : hipSuccess;
+    launch_kernel(table_set_kernel, dim3(uint32_t((n + 255) / 256)), dim3(256), 0, s, table, entries, n);
+    return hipGetLastError();
+}
+
+}  // namespace ge

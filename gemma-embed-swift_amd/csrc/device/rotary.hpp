@@ -1,0 +1,51 @@
+// Norms and rotary positions of query and key heads, and appending keys and values to pages (rotary.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace ge {
+
+// Rows [row0, row0 + n) of one sequence, cached at rows first, first + 1, ... of table slot `slot`.
+struct AppendItem {
+    uint32_t row0, n, slot, first;
+};
+constexpr int kAppendInlineItems = 200;
+// The list of a call that has few, among the kernel's arguments.
+struct AppendInline {
+    AppendItem items[kAppendInlineItems];
+};
+
+enum { kNormQ = 1, kNormK = 2, kNormV = 4 };
+
+struct HeadsArgs {
+    const void *q, *k, *v;           // rows of heads of the input type; v: appending only
+    uint16_t *q_out, *k_out, *v_out;  // k_out and v_out: rows, or pages when appending
+    const float *q_norm, *k_norm;    // [head_dim], null: no weight
+    const int32_t* positions;        // [rows], null: the cache row (appending only)
+    const double* turns;             // [half]: turns of a full circle a position
+    const int32_t* table;            // [slots][slot_pages]
+    const AppendItem* items;         // null: in AppendInline when appending
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;  // elements from one row to the next
+    int64_t page_stride;             // elements from one page to the next
+    int heads, kv_heads, head_dim, rows;
+    int half;                        // pairs that turn, from the first element on
+    int pairs;                       // 1: neighbours are a pair, 0: elements half apart
+    int normed;                      // kNorm bits
+    float eps, fade, gain;           // fade gain: the magnitude, fade <= 1 <= |gain|
+    int rows_each;                   // rows of a workgroup (not appending)
+    int n_items, slot_pages, page_shift;
+};
+static_assert(sizeof(HeadsArgs) + sizeof(AppendInline) <= 4096, "kernel arguments");
+
+// Rows of a workgroup: about 2048 workgroups in long calls, a row a wave in short ones.
+inline int heads_rows_each(int rows) { return rows <= 8192 ? 4 : (rows / 2048 + 3) / 4 * 4; }
+
+// wide: everything is in whole 16-byte pieces (heads_wide).
+hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, bool bf16, bool wide);
+hipError_t launch_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool in_f32, bool bf16, bool wide);
+// Page numbers into a table: entries of (place in the table, page) pairs.
+hipError_t launch_table_set(hipStream_t s, int32_t* table, const uint2* entries, int n);
+
+}  // namespace ge

@@ -211,6 +211,7 @@ struct ge_ctx {
     void* op_buf = nullptr;
     size_t op_cap = 0;
     bool causal_ready = false;  // causal_configure() has run (causal.cpp)
+    bool paged_ready = false;   // paged_configure() has run (paged.cpp)
     // Pinned memory of one per-op call's work lists (op_lists), which its kernels read in place, kept up to
     // kOpListsKept bytes.
     void* op_host = nullptr;

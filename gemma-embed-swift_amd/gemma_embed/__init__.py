@@ -35,6 +35,10 @@ ERRORS = {
  GE_ERR_NO_DEVICE) = range(1, 9)
 GE_TYPE_F32, GE_TYPE_F16, GE_TYPE_Q8_0, GE_TYPE_BF16 = 0, 1, 8, 30
 GE_TYPE_Q4_0, GE_TYPE_Q4_1 = 2, 3  # the 4-bit per-op entries
+# rotary positions: which elements of a head are a pair, and the scaling of their frequencies
+GE_ROTARY_HALVES, GE_ROTARY_PAIRS = 0, 1
+GE_ROTARY_PLAIN, GE_ROTARY_LINEAR, GE_ROTARY_BY_TURNS = 0, 1, 2
+GE_NORM_Q, GE_NORM_K, GE_NORM_V = 1, 2, 4  # heads that are normed first
 
 
 class GemmaEmbedError(RuntimeError):
@@ -71,6 +75,32 @@ class ge_attention_shape(C.Structure):
 
 class ge_attention_seq(C.Structure):
     _fields_ = [("q_start", C.c_uint32), ("q_len", C.c_uint32), ("kv_start", C.c_uint32), ("kv_len", C.c_uint32)]
+
+
+class ge_rotary_desc(C.Structure):
+    _fields_ = [("dims", C.c_int32), ("layout", C.c_int32), ("scaling", C.c_int32), ("trained", C.c_int32), ("base", C.c_float),
+                ("factor", C.c_float), ("low_turns", C.c_float), ("high_turns", C.c_float), ("magnitude", C.c_float)]
+
+
+class ge_heads_shape(C.Structure):
+    _fields_ = [("in_type", C.c_int32), ("type", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("rows", C.c_int32), ("normed", C.c_int32), ("eps", C.c_float),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_stride", C.c_int64),
+                ("k_out_stride", C.c_int64), ("page_stride", C.c_int64)]
+
+
+class ge_page_entry(C.Structure):
+    _fields_ = [("slot", C.c_uint32), ("index", C.c_uint32), ("page", C.c_int32)]
+
+
+class ge_paged_seq(C.Structure):
+    _fields_ = [("q_start", C.c_uint32), ("q_len", C.c_uint32), ("slot", C.c_uint32), ("kv_len", C.c_uint32)]
+
+
+class ge_paged_shape(C.Structure):
+    _fields_ = [("type", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("q_rows", C.c_int32), ("window", C.c_int32), ("scale", C.c_float), ("cap", C.c_float),
+                ("q_stride", C.c_int64), ("out_stride", C.c_int64), ("page_stride", C.c_int64)]
 
 
 class ge_tensor_desc(C.Structure):
@@ -168,6 +198,14 @@ SIGNATURES = {
     "ge_op_gemv_q4_geglu": (_I, [_P, _P, _P, _P, C.c_int32, C.c_int32, _P, C.c_int32]),
     "ge_op_attention_causal": (_I, [_P, C.POINTER(ge_attention_shape), _P, _P, _P, _P, C.c_int32, _P]),
     "ge_op_attention_prefix": (_I, [_P, C.POINTER(ge_attention_shape), _P, _P, _P, C.c_int32, _P, _P, _P, C.c_int32, _P]),
+    "ge_op_rotary_create": (_I, [_P, C.POINTER(ge_rotary_desc), C.POINTER(_P)]),
+    "ge_op_rotary_destroy": (_I, [_P, _P]),
+    "ge_op_rotate_heads": (_I, [_P, C.POINTER(ge_heads_shape)] + [_P] * 8),
+    "ge_op_page_table_create": (_I, [_P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(_P)]),
+    "ge_op_page_table_set": (_I, [_P, _P, _P, C.c_int32]),
+    "ge_op_page_table_destroy": (_I, [_P, _P]),
+    "ge_op_paged_append": (_I, [_P, C.POINTER(ge_heads_shape)] + [_P] * 9 + [C.c_int32] + [_P] * 3),
+    "ge_op_attention_paged": (_I, [_P, C.POINTER(ge_paged_shape), _P, _P, _P, _P, _P, C.c_int32, _P]),
     "ge_model_load": (_I, [C.c_char_p, C.POINTER(ge_load_options), C.POINTER(_P), C.c_char_p, C.c_size_t]),
     "ge_gguf_open": (_I, [C.c_char_p, C.POINTER(_P), C.c_char_p, C.c_size_t]),
     "ge_gguf_close": (None, [_P]),
@@ -684,6 +722,83 @@ class Context:
         s = attention_seqs(seqs)
         self._check(lib.ge_op_attention_prefix(self.handle, C.byref(shape), q, prefix_k, prefix_v, prefix_len, k, v,
                                                s.__array_interface__["data"][0], len(s), out), "ge_op_attention_prefix")
+
+    # ---- a paged cache of keys and values (shapes from heads_shape and paged_shape, seqs from paged_seqs)
+    def rotary_create(self, dims: int, base: float, layout: int = GE_ROTARY_HALVES, scaling: int = GE_ROTARY_PLAIN,
+                      factor: float = 1.0, low_turns: float = 1.0, high_turns: float = 4.0, trained: int = 0,
+                      magnitude: float = 1.0) -> int:
+        """Rotary positions (ge_rotary_desc) of rotate_heads and paged_append."""
+        d = ge_rotary_desc(dims, layout, scaling, trained, base, factor, low_turns, high_turns, magnitude)
+        h = C.c_void_p()
+        self._check(lib.ge_op_rotary_create(self.handle, C.byref(d), C.byref(h)), "ge_op_rotary_create")
+        return h.value
+
+    def rotary_destroy(self, h: int):
+        self._check(lib.ge_op_rotary_destroy(self.handle, h), "ge_op_rotary_destroy")
+
+    def rotate_heads(self, shape: "ge_heads_shape", rotary: Optional[int], q: Optional[int], k: Optional[int],
+                     q_norm: Optional[int], k_norm: Optional[int], positions: Optional[int], q_out: Optional[int],
+                     k_out: Optional[int]):
+        """ge_op_rotate_heads: rows of query and key heads, normed and turned."""
+        self._check(lib.ge_op_rotate_heads(self.handle, C.byref(shape), rotary, q, k, q_norm, k_norm, positions, q_out, k_out),
+                    "ge_op_rotate_heads")
+
+    def page_table_create(self, slots: int, slot_pages: int, page_rows: int, n_pages: int) -> int:
+        h = C.c_void_p()
+        self._check(lib.ge_op_page_table_create(self.handle, slots, slot_pages, page_rows, n_pages, C.byref(h)),
+                    "ge_op_page_table_create")
+        return h.value
+
+    def page_table_set(self, table: int, entries):
+        """(slot, index, page) of each entry: the page at that index of the slot, -1 for none."""
+        e = np.asarray(entries)
+        if e.size and not np.issubdtype(e.dtype, np.integer):
+            raise TypeError(f"an entry is three whole numbers, not {e.dtype}")
+        if e.ndim > 2 or (e.size and (e.ndim == 1 and e.size != 3 or e.ndim == 2 and e.shape[1] != 3)):
+            raise ValueError(f"entries of three numbers each, not an array of shape {e.shape}")
+        e = e.reshape(-1, 3)
+        if e.size and (e.min() < -0x80000000 or e.max() > 0x7fffffff):
+            raise OverflowError("an entry's numbers are counted in 32 bits")
+        e = np.ascontiguousarray(e, dtype=np.int32)
+        self._check(lib.ge_op_page_table_set(self.handle, table, e.ctypes.data, len(e)), "ge_op_page_table_set")
+
+    def page_table_destroy(self, table: int):
+        self._check(lib.ge_op_page_table_destroy(self.handle, table), "ge_op_page_table_destroy")
+
+    def paged_append(self, shape: "ge_heads_shape", rotary: Optional[int], q: Optional[int], k: int, v: int,
+                     q_norm: Optional[int], k_norm: Optional[int], positions: Optional[int], table: int, seqs: np.ndarray,
+                     q_out: Optional[int], k_pages: int, v_pages: int):
+        """ge_op_paged_append: a call's queries normed and turned, its keys and values into their pages."""
+        s = paged_seqs(seqs)
+        self._check(lib.ge_op_paged_append(self.handle, C.byref(shape), rotary, q, k, v, q_norm, k_norm, positions, table,
+                                           s.__array_interface__["data"][0], len(s), q_out, k_pages, v_pages),
+                    "ge_op_paged_append")
+
+    def attention_paged(self, shape: "ge_paged_shape", q: int, table: int, k_pages: int, v_pages: int, seqs: np.ndarray, out: int):
+        """ge_op_attention_paged: chunks and single tokens over the pages of their slots."""
+        s = paged_seqs(seqs)
+        self._check(lib.ge_op_attention_paged(self.handle, C.byref(shape), q, table, k_pages, v_pages,
+                                              s.__array_interface__["data"][0], len(s), out), "ge_op_attention_paged")
+
+
+def heads_shape(in_type: int, type: int, heads: int, kv_heads: int, head_dim: int, rows: int, normed: int = 0, eps: float = 1e-6,
+                q_stride: int = 0, k_stride: int = 0, v_stride: int = 0, q_out_stride: int = 0, k_out_stride: int = 0,
+                page_stride: int = 0) -> "ge_heads_shape":
+    """Operands of rotate_heads and paged_append (in_type: GE_TYPE_F32 or type; type: GE_TYPE_F16 or GE_TYPE_BF16;
+    normed: GE_NORM_Q, GE_NORM_K and GE_NORM_V)."""
+    return ge_heads_shape(in_type, type, heads, kv_heads, head_dim, rows, normed, eps, q_stride, k_stride, v_stride, q_out_stride,
+                          k_out_stride, page_stride)
+
+
+def paged_shape(type: int, heads: int, kv_heads: int, head_dim: int, q_rows: int, scale: float = 1.0, window: int = 0,
+                cap: float = 0.0, q_stride: int = 0, out_stride: int = 0, page_stride: int = 0) -> "ge_paged_shape":
+    """Operands of attention_paged (type: GE_TYPE_F16 or GE_TYPE_BF16)."""
+    return ge_paged_shape(type, heads, kv_heads, head_dim, q_rows, window, scale, cap, q_stride, out_stride, page_stride)
+
+
+def paged_seqs(sequences) -> np.ndarray:
+    """(q_start, q_len, slot, kv_len) of each sequence as a (n, 4) uint32 array."""
+    return attention_seqs(sequences)
 
 
 def attention_shape(type: int, heads: int, kv_heads: int, head_dim: int, q_rows: int, kv_rows: int, scale: float = 1.0,

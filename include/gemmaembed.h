@@ -327,6 +327,107 @@ int ge_op_attention_prefix(ge_ctx* ctx, const ge_attention_shape* shape, const v
                            const void* prefix_v, int32_t prefix_len, const void* k, const void* v,
                            const ge_attention_seq* seqs, int32_t n_seqs, void* out);
 
+/* ---- a cache of keys and values in pages, for servers of causal models: rotary positions, page tables, appending a
+ * call's tokens, and attention over the pages. No counterpart in the reference. As the other per-op entries they
+ * take device memory (sequence lists, page entries and descriptions: host memory), run on the context's stream and
+ * return when their results are there; what they read must be complete when they are called.
+ *
+ * Rotary positions: the first `dims` elements of a head turn in pairs (a, b), pair i by the angle
+ * position f_i, to (a cos - b sin, a sin + b cos) magnitude. f_i = base^(-2 i / dims), and for positions past those a
+ * model was trained on: LINEAR f_i / factor; BY_TURNS f_i (w + (1 - w) / factor), w = the part, from 0 to 1, of the way
+ * from low_turns to high_turns that the pair's trained f_i / 2 pi turns are. The angle is reduced in fp64. The
+ * handle belongs to the context that made it, as a page table does; destroy both before the context. */
+enum { GE_ROTARY_HALVES = 0, GE_ROTARY_PAIRS = 1 };
+enum { GE_ROTARY_PLAIN = 0, GE_ROTARY_LINEAR = 1, GE_ROTARY_BY_TURNS = 2 };
+typedef struct ge_rotary_desc {
+    int32_t dims;      /* even, 2 to 512 */
+    int32_t layout;    /* HALVES: elements i and dims / 2 + i are a pair; PAIRS: 2 i and 2 i + 1 */
+    int32_t scaling;
+    int32_t trained;   /* BY_TURNS: positions the model was trained on */
+    float base;
+    float factor;      /* LINEAR and BY_TURNS */
+    float low_turns, high_turns; /* BY_TURNS: low_turns < high_turns */
+    float magnitude;   /* 0: 1 */
+} ge_rotary_desc;
+typedef struct ge_rotary ge_rotary;
+int ge_op_rotary_create(ge_ctx* ctx, const ge_rotary_desc* desc, ge_rotary** out);
+int ge_op_rotary_destroy(ge_ctx* ctx, ge_rotary* rotary);
+
+/* Rows of query, key and value heads, a token's heads back to back: q has rows of heads x head_dim elements, k and v
+ * of kv_heads x head_dim; a stride is the elements from one row to the next (0: rows back to back), so that
+ * they may be views of one projection's output. Inputs are of in_type (GE_TYPE_F32 or the results' type), results of
+ * type (GE_TYPE_F16 or GE_TYPE_BF16). Up to 4096 heads of each kind (0 for none, where an entry allows it), head_dim even
+ * up to 512, rows under 2^30, strides up to 2^24. Buffers are aligned to their elements; the fast path needs
+ * 16 bytes (addresses and strides), head_dim a multiple of 16 and dims one of 16.
+ * normed: which heads are RMS-normed first, x / sqrt(mean x^2 + eps) * w over the head, w fp32 [head_dim] (null: 1);
+ * value heads have no weight. All in fp32, rounded once. */
+enum { GE_NORM_Q = 1, GE_NORM_K = 2, GE_NORM_V = 4 };
+typedef struct ge_heads_shape {
+    int32_t in_type, type;
+    int32_t heads, kv_heads, head_dim, rows;
+    int32_t normed;
+    float eps;
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+    int64_t page_stride; /* ge_op_paged_append: elements from one page to the next, 0: back to back */
+} ge_heads_shape;
+
+/* q_out and k_out = the rows of q and k, normed (Q and K) and turned. positions: device int32 [rows], any values; rotary
+ * (and then positions) nullable: not turned. q_out may be q and k_out k, of one type and stride; other overlaps are not
+ * allowed. q and q_out may be null with no query heads, k and k_out with no KV heads. */
+int ge_op_rotate_heads(ge_ctx* ctx, const ge_heads_shape* shape, const ge_rotary* rotary, const void* q, const void* k,
+                       const void* q_norm, const void* k_norm, const void* positions, void* q_out, void* k_out);
+
+/* Which pages hold which keys: slot s's keys [i page_rows, (i + 1) page_rows) are in its page number i, one of
+ * n_pages of a pool (the same in every layer's pools). page_rows: a power of two from 8 to 1024; slots x slot_pages up
+ * to 2^28, slot_pages x page_rows under 2^30. A new table has no pages. ge_op_page_table_set puts `page` at `index` of
+ * `slot`, -1 takes it out (of a page a call needs no more: one before a window); of two entries for one place the later
+ * one counts. Slots may share pages. A refused call changes nothing. */
+typedef struct ge_page_table ge_page_table;
+typedef struct ge_page_entry {
+    uint32_t slot, index;
+    int32_t page;
+} ge_page_entry;
+int ge_op_page_table_create(ge_ctx* ctx, int32_t slots, int32_t slot_pages, int32_t page_rows, int32_t n_pages,
+                            ge_page_table** out);
+int ge_op_page_table_set(ge_ctx* ctx, ge_page_table* table, const ge_page_entry* entries, int32_t n);
+int ge_op_page_table_destroy(ge_ctx* ctx, ge_page_table* table);
+
+/* One sequence of a call: its rows [q_start, q_start + q_len) are its last q_len positions, and its kv_len keys, those
+ * of the call's rows among them, are in its slot. The rows of a call ascend and do not overlap. */
+typedef struct ge_paged_seq {
+    uint32_t q_start, q_len, slot, kv_len;
+} ge_paged_seq;
+
+/* Appends the call's tokens: row i of a sequence is at position and cache row kv_len - q_len + i (positions, device int32
+ * [rows], nullable: other positions to turn by). q_out = q normed and turned; k normed and turned and v (normed with
+ * GE_NORM_V) go to their pages. Pools k_pages and v_pages: page p from element p page_stride on (0: pages back to
+ * back; both may interleave in one buffer), [kv_heads][page_rows][head_dim]. Every page written must be in its slot, and a page
+ * is written by one sequence of a call at one place: else nothing is written and the call refused. Other rows of pages,
+ * and rows of q_out outside the sequences, stay as they were. q_out may be q, of one type and stride; no query heads: q
+ * and q_out may be null. */
+int ge_op_paged_append(ge_ctx* ctx, const ge_heads_shape* shape, const ge_rotary* rotary, const void* q, const void* k,
+                       const void* v, const void* q_norm, const void* k_norm, const void* positions,
+                       const ge_page_table* table, const ge_paged_seq* seqs, int32_t n_seqs, void* q_out, void* k_pages,
+                       void* v_pages);
+
+/* ge_op_attention_causal over pages: out_i = sum_j softmax_j(s_ij) v_j over the keys j <= i + kv_len - q_len of the
+ * sequence's slot and, with a window, j > i + kv_len - q_len - window; s_ij = scale q_i . k_j, or with a cap
+ * cap tanh(scale q_i . k_j / cap). q and out are rows of heads x head_dim (q_stride, out_stride), pools as
+ * ge_op_paged_append has them; what ge_op_attention_causal says of types, limits, precision, rows that see no key, hidden, infinite and
+ * NaN values, and rows outside the sequences holds here too; a cap of up to
+ * 256 moves a weight by at most its 2^-21 part of itself, a larger one a score by 2^-18 of itself. page_stride is a multiple of 8. The pages of every key that a row sees must be in the slot; earlier ones may have been taken out. */
+typedef struct ge_paged_shape {
+    int32_t type;
+    int32_t heads, kv_heads, head_dim;
+    int32_t q_rows;
+    int32_t window; /* keys a query sees up to and including its own position; 0 = all */
+    float scale;    /* multiplies the scores */
+    float cap;      /* 0: none; up to 2^20 */
+    int64_t q_stride, out_stride, page_stride;
+} ge_paged_shape;
+int ge_op_attention_paged(ge_ctx* ctx, const ge_paged_shape* shape, const void* q, const ge_page_table* table,
+                          const void* k_pages, const void* v_pages, const ge_paged_seq* seqs, int32_t n_seqs, void* out);
+
 /* ---- image tower, on the same context as the text encoder.
  * Replaces Metal/VisionTower.swift (VisionTower.upload :113-140, encode :143-185) for a
  * pre-LayerNorm ViT: per layer x += attn_out(attn(LN1(x))) + b, x += down(gelu_tanh(up(LN2(x)))),
