@@ -13,18 +13,38 @@
 #include <cmath>
 #include <vector>
 
-#include "causal_plan.hpp"
+#include "causal.hpp"
+#include "runtime_internal.hpp"
 
 namespace ge {
 namespace {
 
 constexpr int kCus = 256;
 constexpr int64_t kSplitMinKeys = 128;
-constexpr int64_t kMaxRows = kAttentionMaxRows, kMaxStride = kAttentionMaxStride;
+constexpr int64_t kMaxRows = int64_t(1) << 30, kMaxStride = int64_t(1) << 24;
 
-using Tile = CausalTile;
-using Base = CausalBase;
-using Plan = CausalPlan;
+struct Tile {
+    uint32_t base, row0, n_rows, part;
+    int32_t lo, hi;  // visible keys of its rows
+    uint32_t splits;
+};
+
+// Rows of one sequence, or of a run of them, against a range of their keys.
+struct Base {
+    uint32_t q_token, key0, tile0;
+    int64_t shift;
+    bool direct;  // its rows have no other part
+};
+
+// What a call does, planned in a few microseconds: a call of a few dozen takes no longer on the GPU.
+struct Plan {
+    std::vector<Base> bases;
+    std::vector<Tile> tiles;
+    std::vector<uint32_t> order;  // tiles by their items' length, longest first
+    std::vector<CausalJoin> joins;
+    size_t n_items = 0, part_rows = 0;
+    int kinds = 0, group = 1, wide = 0;
+};
 
 int64_t divide_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool narrow(const Tile& t) { return t.n_rows <= uint32_t(kCausalNarrowRows); }
@@ -40,7 +60,7 @@ void add_base(Plan& p, uint32_t q_token, int64_t tokens, uint32_t key0, int64_t 
     for (int64_t r = 0; r < rows; r += p.wide) {
         const int64_t n = std::min<int64_t>(p.wide, rows - r);
         int64_t lo = first, hi = end;
-        if (window) lo = std::max(first, r / p.group + shift - window + 1) / p.key_align * p.key_align;
+        if (window) lo = std::max(first, r / p.group + shift - window + 1);
         if (shift < end) hi = std::min(end, (r + n - 1) / p.group + shift + 1);
         if (hi <= lo) lo = hi = first;
         p.tiles.push_back(Tile{at, uint32_t(r), uint32_t(n), 0, int32_t(lo), int32_t(hi), 0});
@@ -120,11 +140,8 @@ int64_t split_limit(const Plan& p, int kv_heads, int head_dim) {
     return best;
 }
 
-}  // namespace
-
-Plan make_plan(const ge_attention_shape& s, const ge_attention_seq* seqs, int n_seqs, int64_t prefix_len, int key_align) {
+Plan make_plan(const ge_attention_shape& s, const ge_attention_seq* seqs, int n_seqs, int64_t prefix_len) {
     Plan p;
-    p.key_align = key_align;
     p.group = s.heads / s.kv_heads;
     p.wide = causal_wide_rows(s.head_dim);
     p.bases.reserve(size_t(n_seqs) * (prefix_len ? 2 : 1));
@@ -230,6 +247,7 @@ Plan make_plan(const ge_attention_shape& s, const ge_attention_seq* seqs, int n_
     return p;
 }
 
+// The plan's items, n_items of them.
 void write_items(const Plan& p, CausalItem* out) {
     for (const uint32_t i : p.order) {
         const Tile& t = p.tiles[i];
@@ -243,8 +261,6 @@ void write_items(const Plan& p, CausalItem* out) {
         }
     }
 }
-
-namespace {
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -296,7 +312,7 @@ void attend(ge_ctx* c, const ge_attention_shape* shape, const void* q, const voi
         hip_check(causal_configure(), "hipFuncSetAttribute");
         c->causal_ready = true;
     }
-    const Plan p = make_plan(s, seqs, n_seqs, prefix_len, 1);
+    const Plan p = make_plan(s, seqs, n_seqs, prefix_len);
     if (p.n_items * uint64_t(s.kv_heads) > kCausalMaxGroups || p.joins.size() * uint64_t(s.kv_heads) > kCausalMaxGroups)
         fail(GE_ERR_INVALID, "attention: the call's rows and keys are too many for one call");
     OpTemps temps(c);

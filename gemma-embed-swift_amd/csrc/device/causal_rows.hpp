@@ -155,7 +155,9 @@ struct Rows {
         __device__ __forceinline__ void softmax(Rows& w, int kb, int end, float c, int lane, u32x4 (&p)[2 * KT], CURVE curve = {}) {
             if constexpr (CURVE::kCurved) {
 #pragma unroll
-                for (int t = 0; t < KT; t++) curve(s[t]);
+                for (int t = 0; t < KT; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[t][e] = curve(s[t][e]);
             }
             if (!sees_all(w, kb, end)) {
                 const int k0 = kb + (lane >> 5) * 4, hi = min(w.hi, end - 1);

@@ -12,8 +12,7 @@
 #include <memory>
 #include <vector>
 
-#include "causal_plan.hpp"
-#include "paged.hpp"
+#include "paged_plan.hpp"
 #include "rotary.hpp"
 #include "runtime_internal.hpp"
 
@@ -43,9 +42,10 @@ namespace ge {
 namespace {
 
 constexpr double kTwoPi = 6.283185307179586476925286766559;
+constexpr int64_t kAttentionMaxRows = int64_t(1) << 30, kAttentionMaxStride = int64_t(1) << 24;
 constexpr int64_t kMaxTable = int64_t(1) << 28, kMaxPages = int64_t(1) << 28;
 constexpr int kMaxHeads = 4096, kMaxPageRows = 1024;
-constexpr float kMaxCap = 1048576.0f;
+constexpr float kMaxCap = 1024.0f;  // for its accuracy (Capped, paged.hip)
 
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
@@ -380,8 +380,7 @@ void attend(ge_ctx* c, const ge_paged_shape* shape, const void* q, const ge_page
     if (int64_t(s.q_rows) * (s.heads / s.kv_heads) >= kAttentionMaxRows)
         fail(GE_ERR_INVALID, "%s: %d rows of %d query heads a KV head pass 2^30", kAttend, s.q_rows, s.heads / s.kv_heads);
     if (!std::isfinite(s.scale)) fail(GE_ERR_INVALID, "%s: scale is not finite", kAttend);
-    // past it a cap and its reciprocal leave fp32's range
-    if (!(s.cap >= 0.0f && s.cap <= kMaxCap)) fail(GE_ERR_INVALID, "%s: cap %g (0 to 2^20)", kAttend, double(s.cap));
+    if (!(s.cap >= 0.0f && s.cap <= kMaxCap)) fail(GE_ERR_INVALID, "%s: cap %g (0 to 1024)", kAttend, double(s.cap));
     const int64_t q_width = int64_t(s.heads) * s.head_dim;
     check_rows_stride(kAttend, "q", s.q_stride, q_width, 8);
     check_rows_stride(kAttend, "out", s.out_stride, q_width, 8);
@@ -391,10 +390,8 @@ void attend(ge_ctx* c, const ge_paged_shape* shape, const void* q, const ge_page
     if (!seqs) fail(GE_ERR_INVALID, "%s: null sequences", kAttend);
     if (check_seqs(kAttend, t, seqs, n_seqs, s.q_rows) == 0) return;
     bool keys = false;
-    std::vector<ge_attention_seq> list(static_cast<size_t>(n_seqs));
     for (int i = 0; i < n_seqs; i++) {
         const ge_paged_seq& e = seqs[i];
-        list[size_t(i)] = ge_attention_seq{e.q_start, e.q_len, e.slot, e.kv_len};
         if (!e.q_len || !e.kv_len) continue;
         keys = true;
         const int64_t low = s.window ? std::max<int64_t>(0, int64_t(e.kv_len) - e.q_len - s.window + 1) : 0;
@@ -409,21 +406,19 @@ void attend(ge_ctx* c, const ge_paged_shape* shape, const void* q, const ge_page
         hip_check(paged_configure(), "hipFuncSetAttribute");
         c->paged_ready = true;
     }
-    ge_attention_shape plain{};
-    plain.heads = s.heads;
-    plain.kv_heads = s.kv_heads;
-    plain.head_dim = s.head_dim;
-    plain.window = s.window;
-    const CausalPlan p = make_plan(plain, list.data(), n_seqs, 0, kPagedAlign);
-    if (p.n_items * uint64_t(s.kv_heads) > kCausalMaxGroups || p.joins.size() * uint64_t(s.kv_heads) > kCausalMaxGroups)
+    const PagedPlan p = plan_paged(s, seqs, n_seqs);
+    if (p.workgroups * uint64_t(s.kv_heads) > kCausalMaxGroups || p.joins.size() * uint64_t(s.kv_heads) > kCausalMaxGroups ||
+        p.items.size() >= kDirect || p.part_rows >= kDirect)
         fail(GE_ERR_INVALID, "%s: the call's rows and keys are too many for one call", kAttend);
     OpTemps temps(c);
-    CausalInline in;
-    const bool few = p.n_items <= size_t(kCausalInlineItems) && p.joins.size() <= size_t(kCausalInlineJoins);
-    const size_t item_bytes = (p.n_items * sizeof(CausalItem) + 255) / 256 * 256;
-    unsigned char* const lists = few ? nullptr : op_lists(c, item_bytes + p.joins.size() * sizeof(CausalJoin));
-    write_items(p, few ? in.items : reinterpret_cast<CausalItem*>(lists));
-    std::copy(p.joins.begin(), p.joins.end(), few ? in.joins : reinterpret_cast<CausalJoin*>(lists + item_bytes));
+    PagedInline in;
+    CausalInline join_in;
+    const bool few = p.items.size() <= size_t(kPagedInlineItems), few_joins = p.joins.size() <= size_t(kCausalInlineJoins);
+    const size_t item_bytes = few ? 0 : (p.items.size() * sizeof(PagedItem) + 255) / 256 * 256;
+    const size_t join_bytes = few_joins ? 0 : p.joins.size() * sizeof(CausalJoin);
+    unsigned char* const lists = item_bytes + join_bytes ? op_lists(c, item_bytes + join_bytes) : nullptr;
+    std::copy(p.items.begin(), p.items.end(), few ? in.items : reinterpret_cast<PagedItem*>(lists));
+    std::copy(p.joins.begin(), p.joins.end(), few_joins ? join_in.joins : reinterpret_cast<CausalJoin*>(lists + item_bytes));
     const size_t o_at = temps.reserve(p.part_rows * size_t(s.kv_heads) * size_t(s.head_dim) * 4);
     const size_t ml_at = temps.reserve(p.part_rows * size_t(s.kv_heads) * 8);
     unsigned char* const base = p.part_rows ? temps.base() : nullptr;
@@ -433,16 +428,16 @@ void attend(ge_ctx* c, const ge_paged_shape* shape, const void* q, const ge_page
     a.k = static_cast<const uint16_t*>(k_pages);
     a.v = static_cast<const uint16_t*>(v_pages);
     a.out = static_cast<uint16_t*>(out);
-    a.items = reinterpret_cast<const CausalItem*>(lists);
-    a.joins = few ? nullptr : reinterpret_cast<const CausalJoin*>(lists + item_bytes);
+    a.paged_items = few ? nullptr : reinterpret_cast<const PagedItem*>(lists);
+    a.joins = few_joins ? nullptr : reinterpret_cast<const CausalJoin*>(lists + item_bytes);
     a.part_o = reinterpret_cast<float*>(base + o_at);
     a.part_ml = reinterpret_cast<float2*>(base + ml_at);
     a.q_stride = s.q_stride;
     a.out_stride = s.out_stride;
     a.part_rows = p.part_rows;
-    a.n_items = int(p.n_items);
+    a.n_items = int(p.workgroups);
     a.n_joins = int(p.joins.size());
-    for (const CausalJoin& j : p.joins) a.join_rows = std::max(a.join_rows, int(j.n_rows));
+    a.join_rows = p.join_rows;
     a.group = s.heads / s.kv_heads;
     a.kv_heads = s.kv_heads;
     a.window = s.window;
@@ -453,9 +448,8 @@ void attend(ge_ctx* c, const ge_paged_shape* shape, const void* q, const ge_page
     a.page_shift = t->page_shift;
     constexpr float kLog2e = 1.4426950408889634f;
     if (s.cap > 0.0f) {
-        a.cap_z = std::min(std::fabs(s.scale) / s.cap, FLT_MAX);
+        a.cap_z = std::min(2 * kLog2e * (std::fabs(s.scale) / s.cap), FLT_MAX);
         a.cap_top = std::max(s.cap * kLog2e, FLT_MIN);
-        a.cap_fine = s.cap > 256.0f;
         a.c = 1.0f;
     } else {
         // a hidden key's -inf times this stays -inf, also at scale 0
@@ -463,7 +457,7 @@ void attend(ge_ctx* c, const ge_paged_shape* shape, const void* q, const ge_page
     }
     launch(c, kAttend, [&] { return launch_paged(c->stream, a, in, s.head_dim, s.type == GE_TYPE_BF16, p.kinds); });
     if (a.n_joins)
-        launch(c, "attention_join", [&] { return launch_causal_join(c->stream, a, in, s.head_dim, s.type == GE_TYPE_BF16); });
+        launch(c, "attention_join", [&] { return launch_causal_join(c->stream, a, join_in, s.head_dim, s.type == GE_TYPE_BF16); });
     hip_check(hipStreamSynchronize(c->stream), "hipStreamSynchronize");
 }
 

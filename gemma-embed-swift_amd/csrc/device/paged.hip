@@ -14,30 +14,19 @@ namespace ge {
 namespace {
 
 // tanh as 1 - 2 / (1 + e^2x), off by 2^-21.5: a third of 2^-24 for the exponential's argument and 2^-25 for itself after
-// the slope, twice the reciprocal's 2^-23, the last sum's 2^-24. That moves a score by cap 2^-21.5, a weight by as much of
-// itself: 2^-13.5 at a cap of 256, a fifth of fp16's half step. From there on (fine) small arguments take the series
-// to x^7, whose error below 1/8 is 2^-29 of x; the rest are off by 2^-18 of themselves.
+// the slope, twice the reciprocal's 2^-23, the last sum's 2^-24. That moves a score by cap 2^-21.5 and a weight by as much
+// of itself: 2^-16 at a cap of 50, 2^-11.5 at the largest, 1024. (A series for small arguments would keep larger caps
+// exact, at twice the instructions.)
 struct Capped {
     static constexpr bool kCurved = true;
-    float z, top;
-    uint32_t fine;
-    __device__ __forceinline__ void operator()(float16_t& s) const {
-        if (top == 0.0f) return;
-        if (fine) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const float x = s[e] * z, x2 = x * x;
-                const float series = x * __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, -17.0f / 315, 2.0f / 15), -1.0f / 3), 1.0f);
-                s[e] = top * (fabsf(x) < 0.125f ? series : tanh(x));
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = top * tanh(s[e] * z);
-        }
+    float z, top;  // z: 2 log2(e) scale / cap
+    __device__ __forceinline__ float operator()(float s) const {
+        return __builtin_fmaf(-2.0f * top, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * z)), top);
     }
-    static __device__ __forceinline__ float tanh(float x) {
-        return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * 2.8853900817779268f)), 1.0f);
-    }
+};
+struct Uncapped : Straight {
+    __device__ __forceinline__ Uncapped(float, float) {}
+    __device__ __forceinline__ float operator()(float s) const { return s; }
 };
 
 // The key blocks of an item.
@@ -48,19 +37,27 @@ struct PagedSpan {
     const PagedArgs& args;
     Ids ids;  // of the sequence
     int lo, hi, blocks;
+    uint32_t slot;
 
     __device__ __forceinline__ PagedSpan(const PagedArgs& a, const CausalItem& it)
         : args(a), ids((Ids)(a.table + size_t(it.key0) * size_t(a.slot_pages))), lo(int(it.k_lo)), hi(int(it.k_hi)),
-          blocks((hi - lo + BK - 1) / BK) {}
+          blocks((hi - lo + BK - 1) / BK), slot(it.key0) {}
     __device__ __forceinline__ int first(int b) const { return lo + b * BK; }
     __device__ __forceinline__ int end(int b) const { return min(first(b) + BK, hi); }
+    // The page of the item's group `group` of 8 keys, a lane's own; 0 past the last.
+    __device__ __forceinline__ int group_page(int group) const {
+        const int key = lo + group * 8;
+        return key < hi ? (args.table + size_t(slot) * size_t(args.slot_pages))[uint32_t(key) >> args.page_shift] : 0;
+    }
     // The page of key `key`; of the last one's from there on (nothing of it is read).
     __device__ __forceinline__ int page(int key) const { return ids[uint32_t(min(key, hi - 1)) >> args.page_shift]; }
     // The 8 keys from `key` on, which are in page `page`, of one head.
     template <int HD>
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(const uint16_t* pool, int page, int key, int kvh) const {
         const size_t at = size_t(page) * size_t(args.page_stride) + size_t((uint32_t(kvh) << args.page_shift) + (uint32_t(key) & ((1u << args.page_shift) - 1))) * HD;
-        return buffer_rsrc(pool + at, uint32_t(min(max(hi - key, 0), 8)) * uint32_t(HD * 2));
+        // (as a scalar: a maximum of a minimum would be one vector instruction, and the resource a loop over its lanes)
+        const int keys = __builtin_amdgcn_readfirstlane(min(max(hi - key, 0), 8));
+        return buffer_rsrc(pool + at, uint32_t(keys) * uint32_t(HD * 2));
     }
     template <int HD>
     __device__ __forceinline__ const uint16_t* value_row(int, int key, int kvh) const {
@@ -80,68 +77,75 @@ __device__ __forceinline__ void copy_group(__amdgpu_buffer_rsrc_t r, unsigned ch
 
 // ---------------------------------------------------------------------------- many rows: waves over rows
 
-// As causal.hip's wide items: 128 rows (64 at head dim 512), the waves copy each key block together, two in LDS.
-template <typename T, int HD>
+// As causal.hip's wide items: 128 rows, 32 a wave (64 at head dim 512, 32 a pair of waves); the waves copy each key
+// block together, two in LDS.
+template <typename T, int HD, typename CURVE>
 struct Wide {
     static constexpr int NW = 4, DW = HD > 256 ? 2 : 1, BK = HD <= 128 ? 64 : 32, NG = BK / 8 / NW;
-    static_assert(NW / DW * 32 == causal_wide_rows(HD), "rows of a wide item");
+    static_assert(NW / DW * 32 == paged_wide_rows(HD), "rows of a wide item");
+    static_assert(NG >= 1 && NW % 2 == 0, "every wave copies groups of one key parity");
     using Kv = KvBlock<HD, BK>;
     static constexpr int kLds = 2 * 2 * Kv::kBytes;
 
-    static __device__ __forceinline__ void run(const PagedArgs& a, const CausalItem& it, int kvh, unsigned char* lds) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-        static_assert(NG >= 1 && NW % 2 == 0, "every wave copies groups of one key parity");
+    static __device__ __forceinline__ void run(const PagedArgs& a, const CausalItem& it, int kvh, int lane, unsigned char* lds) {
+        const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
         const uint32_t k_off = Kv::k_lane(lane, wave & 1, HD * 2), v_off = Kv::v_lane(lane, HD * 2);
         const PagedSpan<BK> span(a, it);
         const int blocks = span.blocks;
-        int page[NG];
-        auto find = [&](int b) {
-#pragma unroll
-            for (int i = 0; i < NG; i++) page[i] = span.page(span.first(b) + (wave + i * NW) * 8);
-        };
+        // The pages of 64 groups of 8 keys (kBlocks blocks) at a time, a lane a group, read when the ones before them are
+        // taken. (As scalar loads in every block they cost registers across its branches: at head dim 256 150 spilled.)
+        constexpr int kBlocks = 64 * 8 / BK;
+        int ids = 0, ids_next = span.group_page(lane);
         auto issue = [&](int b) {
             unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
+            if (b % kBlocks == 0) {
+                ids = ids_next;
+                ids_next = span.group_page((b + kBlocks) * (BK / 8) + lane);
+            }
 #pragma unroll
             for (int i = 0; i < NG; i++) {
                 const int k8 = wave + i * NW, key = span.first(b) + k8 * 8;
-                copy_group<HD, BK, HD / 64>(span.template rows<HD>(a.k, page[i], key, kvh), at, k8, k_off);
-                copy_group<HD, BK, HD / 64>(span.template rows<HD>(a.v, page[i], key, kvh), at + Kv::kBytes, k8, v_off);
+                const int page = __builtin_amdgcn_readlane(ids, b % kBlocks * (BK / 8) + k8);
+                copy_group<HD, BK, HD / 64>(span.template rows<HD>(a.k, page, key, kvh), at, k8, k_off);
+                copy_group<HD, BK, HD / 64>(span.template rows<HD>(a.v, page, key, kvh), at + Kv::kBytes, k8, v_off);
             }
         };
-        const int r0 = int(it.row0) + wave / DW * 32, n = min(32, int(it.n_rows) - wave / DW * 32);
+        // a wave with no rows repeats the item's last
+        const int row = wave / DW * 32, n = min(32, int(it.n_rows) - row), r0 = int(it.row0) + row;
         Rows<T, HD, DW> w;
         HeldBack<T, HD> held;
         held.init(a, it);
-        if (blocks > 0) {
-            find(0);
-            issue(0);
-            find(1);
-        }
-        if (n > 0) w.init(a, it, kvh, r0, n, wave % DW, lane);
-        const Capped curve{a.cap_z, a.cap_top, a.cap_fine};
-        for (int b = 0; b < blocks; b++) {
-            const int kb = span.first(b);
-            unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
+        if (blocks > 0) issue(0);
+        w.init(a, it, kvh, n > 0 ? r0 : int(it.row0 + it.n_rows) - 1, max(n, 1), wave % DW, lane);
+        const CURVE curve{a.cap_z, a.cap_top};
+        // Block b has landed everywhere, block b - 1 has been read, and the next one's copies start.
+        auto turn = [&](int b) {
             wait_vmcnt<0>();
-            if (held.mixed(kb, BK)) {
+            if (held.mixed(span.first(b), BK)) {
 #pragma unroll
                 for (int i = 0; i < Kv::kChunks / NW; i++)  // the chunks this wave copied
-                    held.clear(at + Kv::kBytes + (wave + i * NW) * 1024 + lane * 16);
+                    held.clear(lds + (b & 1) * 2 * Kv::kBytes + Kv::kBytes + (wave + i * NW) * 1024 + lane * 16);
             }
             wait_lgkmcnt0();
             workgroup_barrier();
-            if (b + 1 < blocks) {
-                issue(b + 1);
-                find(b + 2);
-            }
-            if (n > 0 && kb <= w.hi_any && kb + BK - 1 >= w.lo_any) {
-                typename Rows<T, HD, DW>::template Block<BK> blk;
-                u32x4 p[BK / 16];
-                blk.scores(w, at, lane);
-                blk.softmax(w, kb, span.end(b), a.c, lane, p, curve);
-                blk.product(w, at + Kv::kBytes, lane, p);
-            }
+            if (b + 1 < blocks) issue(b + 1);
+        };
+        // The blocks of which the wave's rows see a key, in a loop of their own: accumulators that only some turns
+        // change cost registers at every join.
+        const int first = min(max((w.lo_any - span.lo) / BK, 0), blocks);
+        const int end = n <= 0 || w.hi_any < span.lo ? first : max(first, min(blocks, (w.hi_any - span.lo) / BK + 1));
+        int b = 0;
+        for (; b < first; b++) turn(b);
+        for (; b < end; b++) {
+            turn(b);
+            unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
+            typename Rows<T, HD, DW>::template Block<BK> blk;
+            u32x4 p[BK / 16];
+            blk.scores(w, at, lane);
+            blk.softmax(w, span.first(b), span.end(b), a.c, lane, p, curve);
+            blk.product(w, at + Kv::kBytes, lane, p);
         }
+        for (; b < blocks; b++) turn(b);
         __syncthreads();  // no one reads K and V any more
         if (n > 0) {
             constexpr int kSlice = kLds / NW;
@@ -157,7 +161,7 @@ struct Wide {
 
 // As causal.hip's narrow items: 32 rows, the waves (pairs of them from head dim 256 on) take the key blocks in
 // turn, each through LDS of its own, and join at the end.
-template <typename T, int HD>
+template <typename T, int HD, typename CURVE>
 struct Narrow {
     static constexpr int DW = HD > 128 ? 2 : 1, KW = 4 / DW, BK = 32, NG = BK / 8;
     using Kv = KvBlock<HD, BK>;
@@ -174,8 +178,8 @@ struct Narrow {
             asm volatile("" ::: "memory");
     }
 
-    static __device__ __forceinline__ void run(const PagedArgs& a, const CausalItem& it, int kvh, unsigned char* lds) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+    static __device__ __forceinline__ void run(const PagedArgs& a, const CausalItem& it, int kvh, int lane, unsigned char* lds) {
+        const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
         const int kw = wave / DW, dims = wave % DW;
         // a wave of a pair copies half of the panels
         constexpr int kPanels = HD / 64 / DW;
@@ -213,7 +217,7 @@ struct Narrow {
             find(kw + KW, page);
         }
         w.init(a, it, kvh, r0, n, dims, lane);
-        const Capped curve{a.cap_z, a.cap_top, a.cap_fine};
+        const CURVE curve{a.cap_z, a.cap_top};
         // Waves alone on their LDS leave when their blocks are done; pairs keep meeting until all are.
         for (int b = kw; b - kw < blocks; b += KW) {
             const int kb = span.first(b);
@@ -257,70 +261,88 @@ struct Narrow {
 };
 
 // KINDS: the items of the launch, kCausalWide and kCausalNarrow or one of them.
-template <typename T, int HD, int KINDS>
+template <typename T, int HD, typename CURVE, int KINDS>
 constexpr int paged_lds() {
     int lds = 0;
-    if constexpr ((KINDS & kCausalWide) != 0) lds = Wide<T, HD>::kLds;
-    if constexpr ((KINDS & kCausalNarrow) != 0) lds = lds > Narrow<T, HD>::kLds ? lds : Narrow<T, HD>::kLds;
+    if constexpr ((KINDS & kCausalWide) != 0) lds = Wide<T, HD, CURVE>::kLds;
+    if constexpr ((KINDS & kCausalNarrow) != 0) lds = lds > Narrow<T, HD, CURVE>::kLds ? lds : Narrow<T, HD, CURVE>::kLds;
     return lds;
 }
 
-template <typename T, int HD, int KINDS>
-__global__ __launch_bounds__(256, HD <= 256 ? 2 : 1) void paged_kernel(const PagedArgs a, const CausalInline in) {
+template <typename T, int HD, typename CURVE, int KINDS>
+__global__ __launch_bounds__(256, paged_workgroups(HD)) void paged_kernel(const PagedArgs a, const PagedInline in) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char paged_lds_mem[];
     // Workgroups go to the 8 XCDs in turn: with the KV head fastest, a head's items share an L2.
-    const uint32_t at = blockIdx.x / uint32_t(a.kv_heads);
+    uint32_t at = blockIdx.x / uint32_t(a.kv_heads);
     const int kvh = int(blockIdx.x % uint32_t(a.kv_heads));
-    const CausalItem it = uniform_entry<CausalItem>(a.items, in.items, at);
-    if (KINDS == kCausalNarrow || ((KINDS & kCausalNarrow) && it.narrow))
-        Narrow<T, HD>::run(a, it, kvh, paged_lds_mem);
-    else if constexpr ((KINDS & kCausalWide) != 0)
-        Wide<T, HD>::run(a, it, kvh, paged_lds_mem);
+    for (;;) {
+        int lane = int(threadIdx.x & 63);
+        asm volatile("" : "+v"(lane));  // what an item makes of it is not kept over the loop, in registers that it needs
+        const PagedItem it = uniform_entry<PagedItem>(a.paged_items, in.items, at);
+        if (KINDS == kCausalNarrow || ((KINDS & kCausalNarrow) && it.narrow))
+            Narrow<T, HD, CURVE>::run(a, it, kvh, lane, paged_lds_mem);
+        else if constexpr ((KINDS & kCausalWide) != 0)
+            Wide<T, HD, CURVE>::run(a, it, kvh, lane, paged_lds_mem);
+        at = it.next;
+        if (at == 0) break;
+        __syncthreads();  // no one reads the item's LDS any more
+    }
 }
 
-template <typename T, int HD, int KINDS>
-hipError_t run_items(hipStream_t s, const PagedArgs& a, const CausalInline& in) {
-    launch_kernel(paged_kernel<T, HD, KINDS>, dim3(uint32_t(a.n_items) * uint32_t(a.kv_heads)), dim3(256), uint32_t(paged_lds<T, HD, KINDS>()), s, a, in);
+template <typename T, int HD, typename CURVE, int KINDS>
+hipError_t run_items(hipStream_t s, const PagedArgs& a, const PagedInline& in) {
+    launch_kernel(paged_kernel<T, HD, CURVE, KINDS>, dim3(uint32_t(a.n_items) * uint32_t(a.kv_heads)), dim3(256), uint32_t(paged_lds<T, HD, CURVE, KINDS>()), s, a, in);
     return hipGetLastError();
 }
 
-template <typename T, int HD>
-hipError_t run_kinds(hipStream_t s, const PagedArgs& a, const CausalInline& in, int kinds) {
+template <typename T, int HD, typename CURVE>
+hipError_t run_kinds(hipStream_t s, const PagedArgs& a, const PagedInline& in, int kinds) {
     switch (kinds) {
-        case kCausalWide: return run_items<T, HD, kCausalWide>(s, a, in);
-        case kCausalNarrow: return run_items<T, HD, kCausalNarrow>(s, a, in);
-        case kCausalWide | kCausalNarrow: return run_items<T, HD, kCausalWide | kCausalNarrow>(s, a, in);
+        case kCausalWide: return run_items<T, HD, CURVE, kCausalWide>(s, a, in);
+        case kCausalNarrow: return run_items<T, HD, CURVE, kCausalNarrow>(s, a, in);
+        case kCausalWide | kCausalNarrow: return run_items<T, HD, CURVE, kCausalWide | kCausalNarrow>(s, a, in);
     }
     return hipErrorInvalidValue;
 }
 
-template <typename T, int HD, int KINDS>
+template <typename T, int HD, typename CURVE, int KINDS>
 hipError_t configure_kinds() {
-    constexpr int lds = paged_lds<T, HD, KINDS>();
+    constexpr int lds = paged_lds<T, HD, CURVE, KINDS>();
     static_assert(lds <= 160 * 1024, "LDS of a CU");
-    return hipFuncSetAttribute(reinterpret_cast<const void*>(paged_kernel<T, HD, KINDS>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(paged_kernel<T, HD, CURVE, KINDS>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+}
+
+template <typename T, int HD, typename CURVE>
+hipError_t configure_curve() {
+    hipError_t e = configure_kinds<T, HD, CURVE, kCausalWide>();
+    if (e == hipSuccess) e = configure_kinds<T, HD, CURVE, kCausalNarrow>();
+    if (e == hipSuccess) e = configure_kinds<T, HD, CURVE, kCausalWide | kCausalNarrow>();
+    return e;
+}
+
+template <typename T, int HD>
+hipError_t run_head(hipStream_t s, const PagedArgs& a, const PagedInline& in, int kinds) {
+    return a.cap_top == 0.0f ? run_kinds<T, HD, Uncapped>(s, a, in, kinds) : run_kinds<T, HD, Capped>(s, a, in, kinds);
 }
 
 template <typename T, int HD>
 hipError_t configure_hd() {
-    hipError_t e = configure_kinds<T, HD, kCausalWide>();
-    if (e == hipSuccess) e = configure_kinds<T, HD, kCausalNarrow>();
-    if (e == hipSuccess) e = configure_kinds<T, HD, kCausalWide | kCausalNarrow>();
-    return e;
+    const hipError_t e = configure_curve<T, HD, Uncapped>();
+    return e == hipSuccess ? configure_curve<T, HD, Capped>() : e;
 }
 
 }  // namespace
 
-hipError_t launch_paged(hipStream_t s, const PagedArgs& a, const CausalInline& in, int hd, bool bf16, int kinds) {
+hipError_t launch_paged(hipStream_t s, const PagedArgs& a, const PagedInline& in, int hd, bool bf16, int kinds) {
     if (!causal_head_dim_ok(hd) || a.kv_heads <= 0 || a.group <= 0 || a.n_items < 0 || a.page_shift < 3 ||
         uint64_t(a.n_items) * uint64_t(a.kv_heads) > kCausalMaxGroups)
         return hipErrorInvalidValue;
     if (a.n_items == 0) return hipSuccess;
     switch (hd) {
-        case 64: return bf16 ? run_kinds<BF16, 64>(s, a, in, kinds) : run_kinds<F16, 64>(s, a, in, kinds);
-        case 128: return bf16 ? run_kinds<BF16, 128>(s, a, in, kinds) : run_kinds<F16, 128>(s, a, in, kinds);
-        case 256: return bf16 ? run_kinds<BF16, 256>(s, a, in, kinds) : run_kinds<F16, 256>(s, a, in, kinds);
-        default: return bf16 ? run_kinds<BF16, 512>(s, a, in, kinds) : run_kinds<F16, 512>(s, a, in, kinds);
+        case 64: return bf16 ? run_head<BF16, 64>(s, a, in, kinds) : run_head<F16, 64>(s, a, in, kinds);
+        case 128: return bf16 ? run_head<BF16, 128>(s, a, in, kinds) : run_head<F16, 128>(s, a, in, kinds);
+        case 256: return bf16 ? run_head<BF16, 256>(s, a, in, kinds) : run_head<F16, 256>(s, a, in, kinds);
+        default: return bf16 ? run_head<BF16, 512>(s, a, in, kinds) : run_head<F16, 512>(s, a, in, kinds);
     }
 }
 

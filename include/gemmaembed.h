@@ -414,15 +414,15 @@ int ge_op_paged_append(ge_ctx* ctx, const ge_heads_shape* shape, const ge_rotary
  * sequence's slot and, with a window, j > i + kv_len - q_len - window; s_ij = scale q_i . k_j, or with a cap
  * cap tanh(scale q_i . k_j / cap). q and out are rows of heads x head_dim (q_stride, out_stride), pools as
  * ge_op_paged_append has them; what ge_op_attention_causal says of types, limits, precision, rows that see no key, hidden, infinite and
- * NaN values, and rows outside the sequences holds here too; a cap of up to
- * 256 moves a weight by at most its 2^-21 part of itself, a larger one a score by 2^-18 of itself. page_stride is a multiple of 8. The pages of every key that a row sees must be in the slot; earlier ones may have been taken out. */
+ * NaN values, and rows outside the sequences holds here too; a cap
+ * moves a weight by 2^-21 cap of itself at most. page_stride is a multiple of 8. The pages of every key that a row sees must be in the slot; earlier ones may have been taken out. */
 typedef struct ge_paged_shape {
     int32_t type;
     int32_t heads, kv_heads, head_dim;
     int32_t q_rows;
     int32_t window; /* keys a query sees up to and including its own position; 0 = all */
     float scale;    /* multiplies the scores */
-    float cap;      /* 0: none; up to 2^20 */
+    float cap;      /* 0: none; up to 1024 */
     int64_t q_stride, out_stride, page_stride;
 } ge_paged_shape;
 int ge_op_attention_paged(ge_ctx* ctx, const ge_paged_shape* shape, const void* q, const ge_page_table* table,

@@ -20,9 +20,9 @@ DIRECT = 0xffffffff
 
 
 class Item(C.Structure):
-    """CausalItem, causal.hpp"""
+    """PagedItem, paged.hpp"""
     _fields_ = [(n, U) for n in ("q_token", "row0", "n_rows", "slot", "k_lo", "k_hi")] + \
-        [("shift", C.c_int32)] + [(n, U) for n in ("part", "narrow")]
+        [("shift", C.c_int32)] + [(n, U) for n in ("part", "narrow", "next")]
 
 
 class Join(C.Structure):
@@ -33,15 +33,21 @@ class Join(C.Structure):
 class Args(C.Structure):
     """PagedArgs, paged.hpp: CausalArgs and the pages"""
     _fields_ = [(n, P) for n in ("q", "k", "v", "prefix_k", "prefix_v", "out")] + \
-        [("items", C.POINTER(Item)), ("joins", C.POINTER(Join)), ("part_o", P), ("part_ml", P)] + \
+        [("unused", P), ("joins", C.POINTER(Join)), ("part_o", P), ("part_ml", P)] + \
         [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + [("part_rows", C.c_size_t)] + \
         [(n, I) for n in ("n_items", "n_joins", "join_rows", "group", "kv_heads", "window", "prefix_len")] + \
-        [("c", C.c_float), ("q_flip", U), ("table", P), ("page_stride", C.c_int64), ("slot_pages", I), ("page_shift", I),
-         ("cap_z", C.c_float), ("cap_top", C.c_float), ("cap_fine", U)]
+        [("c", C.c_float), ("q_flip", U), ("items", C.POINTER(Item)), ("table", P), ("page_stride", C.c_int64), ("slot_pages", I), ("page_shift", I),
+         ("cap_z", C.c_float), ("cap_top", C.c_float)]
 
 
-class Inline(C.Structure):
-    _fields_ = [("items", Item * 48), ("joins", Join * 40)]
+class JoinArgs(C.Structure):
+    """CausalArgs"""
+    _fields_ = Args._fields_[:Args._fields_.index(("items", C.POINTER(Item)))]
+
+
+class JoinInline(C.Structure):
+    """CausalInline, causal.hpp"""
+    _fields_ = [("items", C.c_char * (48 * 36)), ("joins", Join * 40)]
 
 
 class Append(C.Structure):
@@ -76,9 +82,20 @@ class Launches:
                     a = C.cast(args[0], C.POINTER(Heads))[0]
                     self.args = {f: getattr(a, f) for f, _ in Heads._fields_ if f != "items"}
                 elif "paged_kernel" in name:
-                    a, few = C.cast(args[0], C.POINTER(Args))[0], C.cast(args[1], C.POINTER(Inline))[0]
+                    a, few = C.cast(args[0], C.POINTER(Args))[0], C.cast(args[1], C.POINTER(Item * 90))[0]
                     self.args = {f: getattr(a, f) for f, _ in Args._fields_ if f not in ("items", "joins")}
-                    self.items = [Item.from_buffer_copy((a.items or few.items)[i]) for i in range(a.n_items)]
+                    self.chains = []  # of each workgroup
+                    for at in range(a.n_items):
+                        self.chains.append([])
+                        while True:
+                            self.chains[-1].append(Item.from_buffer_copy((a.items or few)[at]))
+                            at = self.chains[-1][-1].next
+                            if not at:
+                                break
+                            assert at >= a.n_items
+                    self.items = [i for chain in self.chains for i in chain]
+                elif "causal_join_kernel" in name:
+                    a, few = C.cast(args[0], C.POINTER(JoinArgs))[0], C.cast(args[1], C.POINTER(JoinInline))[0]
                     self.joins = [Join.from_buffer_copy((a.joins or few.joins)[i]) for i in range(a.n_joins)]
                 elif "table_set_kernel" in name:
                     n = C.cast(args[2], C.POINTER(I))[0]
@@ -432,7 +449,7 @@ def test_refused_attention(ctx, memory, table):
     nan, inf = float("nan"), float("inf")
     for bad in (dict(type=F32), dict(hd=80), dict(hd=0), dict(heads=3), dict(heads=0), dict(kv_heads=0), dict(heads=4098), dict(q_rows=-1),
                 dict(q_rows=1 << 30), dict(window=-1), dict(window=1 << 30), dict(scale=nan), dict(scale=inf), dict(cap=nan), dict(cap=inf),
-                dict(cap=-1.0), dict(cap=3e38), dict(cap=2.0 ** 20 + 1), dict(q_stride=255), dict(q_stride=260), dict(out_stride=8), dict(page_stride=2047), dict(page_stride=100),
+                dict(cap=-1.0), dict(cap=3e38), dict(cap=1025.0), dict(cap=30000.0), dict(q_stride=255), dict(q_stride=260), dict(out_stride=8), dict(page_stride=2047), dict(page_stride=100),
                 dict(q=None), dict(out=None), dict(k_pages=None), dict(v_pages=None), dict(q=memory + 8), dict(out=memory + 2),
                 dict(k_pages=memory + 8), dict(q_rows=1 << 29, heads=8, kv_heads=1)):
         refused(attend, ctx, memory, table, good, **bad)
@@ -478,7 +495,10 @@ def covered(got, seqs, heads, kv_heads, hd, window):
                 keys |= more
             assert (token, head) not in written
             written[token, head] = keys
-    assert not parts
+    assert not parts and (got.joins or not got.args["n_joins"])
+    at_once = {64: 768, 128: 512, 256: 512, 512: 256}[hd] // kv_heads
+    if got.joins:  # equal shares: no more workgroups than run at once
+        assert len(got.chains) <= max(at_once, 1024 // kv_heads)
     for token, (_, shift) in slots.items():
         last = token - first[token] + shift
         for h in range(group):
@@ -491,7 +511,7 @@ def covered(got, seqs, heads, kv_heads, hd, window):
 def test_the_plan_covers_every_key_once(ctx, memory, heads, kv_heads, hd, window):
     h = ctx.page_table_create(100, 600, 8, 600)
     ctx.page_table_set(h, [(s, i, i) for s in range(100) for i in range(600)])
-    for seqs in ([(0, 1, 0, 1)], [(0, 1, 3, 4800)], [(0, 300, 2, 300)], [(0, 200, 1, 4001), (200, 1, 5, 4800), (205, 9, 7, 4)],
+    for seqs in ([(0, 1, 0, 1)], [(0, 1, 3, 4800)], [(0, 300, 2, 300)], [(0, 1500, 2, 4700)], [(0, 200, 1, 4001), (200, 1, 5, 4800), (205, 9, 7, 4)],
                  [(i, 1, i, 1 + 48 * i) for i in range(100)], [(0, 3, 0, 0), (3, 50, 9, 20)]):
         got = attend(ctx, memory, h, seqs, heads, kv_heads, hd, window=window)
         covered(got, seqs, heads, kv_heads, hd, window)
@@ -505,12 +525,10 @@ def test_caps(ctx, memory, table):
     a = attend(ctx, memory, table, seqs, scale=-0.5).args
     assert a["cap_top"] == 0 and a["q_flip"] == 0x80008000 and a["c"] == pytest.approx(0.5 * 1.4426950408889634)
     a = attend(ctx, memory, table, seqs, scale=-0.5, cap=50.0).args
-    assert a["c"] == 1.0 and a["cap_z"] == pytest.approx(0.01) and a["cap_top"] == pytest.approx(50 * 1.4426950408889634)
-    assert a["q_flip"] == 0x80008000 and not a["cap_fine"]
-    assert attend(ctx, memory, table, seqs, cap=1000.0).args["cap_fine"]
+    assert a["c"] == 1.0 and a["cap_z"] == pytest.approx(0.02 * 1.4426950408889634) and a["cap_top"] == pytest.approx(50 * 1.4426950408889634)
+    assert a["q_flip"] == 0x80008000
     a = attend(ctx, memory, table, seqs, scale=3e38, cap=1e-30).args
     assert np.isfinite(a["cap_z"]) and a["cap_top"] > 0
-    assert attend(ctx, memory, table, seqs, cap=2.0 ** 20).args["cap_top"] == pytest.approx(2.0 ** 20 * 1.4426950408889634)
 
 
 @pytest.mark.parametrize("what", [b"kernel:paged_kernel", b"kernel:causal_join", b"hipStreamSynchronize", b"hipMalloc"])
