@@ -275,17 +275,27 @@ void append(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const vo
     if (!aligned(positions, 4)) fail(GE_ERR_INVALID, "%s: positions are not aligned to their elements", kAppend);
     claim_pages(t, seqs, n_seqs);
 
+    // few sequences: one item each; many: one for each workgroup, which need not search them then
     const uint32_t each = uint32_t(heads_rows_each(int(rows)));
-    size_t items = 0;
-    for (int i = 0; i < n_seqs; i++) items += (size_t(seqs[i].q_len) + each - 1) / each;
+    size_t groups = 0, some = 0;
+    for (int i = 0; i < n_seqs; i++) {
+        groups += (size_t(seqs[i].q_len) + each - 1) / each;
+        some += seqs[i].q_len > 0;
+    }
+    const bool inlined = some <= size_t(kAppendInlineItems);
     OpTemps temps(c);
     AppendInline few;
-    AppendItem* const list = items <= size_t(kAppendInlineItems) ? few.items : reinterpret_cast<AppendItem*>(op_lists(c, items * sizeof(AppendItem)));
+    AppendItem* const list = inlined ? few.items : reinterpret_cast<AppendItem*>(op_lists(c, groups * sizeof(AppendItem)));
     AppendItem* out = list;
+    uint32_t group = 0;
     for (int i = 0; i < n_seqs; i++) {
         const ge_paged_seq& e = seqs[i];
-        for (uint32_t at = 0; at < e.q_len; at += each)
-            *out++ = AppendItem{e.q_start + at, std::min(each, e.q_len - at), e.slot, e.kv_len - e.q_len + at};
+        const uint32_t piece = inlined ? e.q_len : each;
+        for (uint32_t at = 0; at < e.q_len; at += piece) {
+            const uint32_t n = std::min(piece, e.q_len - at);
+            *out++ = AppendItem{e.q_start + at, n, e.slot, e.kv_len - e.q_len + at, group};
+            group += (n + each - 1) / each;
+        }
     }
     a.q = q;
     a.k = k;
@@ -297,8 +307,10 @@ void append(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const vo
     a.k_norm = static_cast<const float*>(k_norm);
     a.positions = static_cast<const int32_t*>(positions);
     a.table = t->dev;
-    a.items = list == few.items ? nullptr : list;
-    a.n_items = int(items);
+    a.items = inlined ? nullptr : list;
+    a.n_items = int(out - list);
+    a.workgroups = int(groups);
+    a.rows_each = int(each);
     a.slot_pages = t->slot_pages;
     a.page_shift = t->page_shift;
     a.page_stride = s.page_stride;

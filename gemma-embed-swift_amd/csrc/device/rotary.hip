@@ -34,7 +34,7 @@ struct StoredAs<F32> {
 // addresses that are not in such pieces: single elements, the whole wave on a head.
 template <bool WIDE>
 struct Shape {
-    static constexpr int N = WIDE ? 8 : 4, kIts = WIDE ? 4 : 2;  // kIts: groups of heads of one task, loaded together
+    static constexpr int N = WIDE ? 8 : 4, kIts = 2;  // kIts: groups of heads loaded together
 };
 
 // log2 of the lanes a head takes.
@@ -84,62 +84,67 @@ struct Place {
     }
 };
 
+// A lane's elements of one head as they lie in memory, loaded ahead. (Vectors and single members: arrays that
+// are loaded under a condition went through scratch memory.)
 template <typename T, bool WIDE>
-struct Raw {
-    typedef typename StoredAs<T>::Type Stored;
-    static constexpr int N = Shape<WIDE>::N, kPieces = WIDE ? int(8 * sizeof(Stored) / 16) : 1;
-    u32x4 wa[kPieces], wb[kPieces];
-    Stored na[WIDE ? 1 : N], nb[WIDE ? 1 : N];
-
-    __device__ __forceinline__ void load(const Stored* p, const Place<WIDE>& at) {
-        if constexpr (WIDE) {
+struct Raw;
+template <typename T>
+struct Raw<T, true> {
+    u32x4 a{}, b{};
+    __device__ __forceinline__ void load(const uint16_t* p, const Place<true>& at) {
+        a = *reinterpret_cast<const u32x4*>(p + at.a[0]);
+        b = *reinterpret_cast<const u32x4*>(p + at.b[0]);
+    }
+    __device__ __forceinline__ void values(float (&x)[8], float (&y)[8]) const {
 #pragma unroll
-            for (int i = 0; i < kPieces; i++) {
-                wa[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(p + at.a[0]) + 16 * i);
-                wb[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(p + at.b[0]) + 16 * i);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; j++)
-                if (at.a[j] >= 0) {
-                    na[j] = p[at.a[j]];
-                    nb[j] = p[at.b[j]];
-                } else {
-                    na[j] = nb[j] = Stored(0);
-                }
+        for (int i = 0; i < 8; i++) {
+            x[i] = T::value(uint16_t(a[i / 2] >> (16 * (i % 2))));
+            y[i] = T::value(uint16_t(b[i / 2] >> (16 * (i % 2))));
         }
     }
-    __device__ __forceinline__ void clear() {
-        if constexpr (WIDE) {
+};
+template <>
+struct Raw<F32, true> {
+    float4_t a0{}, a1{}, b0{}, b1{};
+    __device__ __forceinline__ void load(const float* p, const Place<true>& at) {
+        a0 = *reinterpret_cast<const float4_t*>(p + at.a[0]);
+        a1 = *reinterpret_cast<const float4_t*>(p + at.a[0] + 4);
+        b0 = *reinterpret_cast<const float4_t*>(p + at.b[0]);
+        b1 = *reinterpret_cast<const float4_t*>(p + at.b[0] + 4);
+    }
+    __device__ __forceinline__ void values(float (&x)[8], float (&y)[8]) const {
 #pragma unroll
-            for (int i = 0; i < kPieces; i++) wa[i] = wb[i] = u32x4{};
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; j++) na[j] = nb[j] = Stored(0);
+        for (int i = 0; i < 4; i++) {
+            x[i] = a0[i];
+            x[4 + i] = a1[i];
+            y[i] = b0[i];
+            y[4 + i] = b1[i];
         }
     }
-    static __device__ __forceinline__ float piece(const u32x4 (&w)[kPieces], int i) {
-        if constexpr (sizeof(Stored) == 4)
-            return __uint_as_float(w[i / 4][i % 4]);
-        else
-            return T::value(uint16_t(w[0][i / 2] >> (16 * (i % 2))));
-    }
-    __device__ __forceinline__ void values(float (&a)[N], float (&b)[N]) const {
+};
+template <typename T>
+struct Raw<T, false> {
+    float4_t a{}, b{};
+    __device__ __forceinline__ void load(const typename StoredAs<T>::Type* p, const Place<false>& at) {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            if constexpr (WIDE) {
-                a[i] = piece(wa, i);
-                b[i] = piece(wb, i);
-            } else {
-                a[i] = T::value(na[i]);
-                b[i] = T::value(nb[i]);
-            }
+        for (int j = 0; j < 4; j++) {  // a unit past the head's end takes the head's first element, and is not used
+            a[j] = T::value(p[max(at.a[j], 0)]);
+            b[j] = T::value(p[max(at.b[j], 0)]);
+            if (at.a[j] < 0) a[j] = b[j] = 0.0f;
+        }
+    }
+    __device__ __forceinline__ void values(float (&x)[4], float (&y)[4]) const {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[j] = a[j];
+            y[j] = b[j];
         }
     }
 };
 
+// A lane's weights, from the LDS row of its head's kind.
 template <bool WIDE>
-__device__ __forceinline__ void load_weights(const float* w, const Place<WIDE>& at, float (&a)[Shape<WIDE>::N], float (&b)[Shape<WIDE>::N]) {
+__device__ __forceinline__ void weigh(const float* w, const Place<WIDE>& at, float (&a)[Shape<WIDE>::N], float (&b)[Shape<WIDE>::N]) {
     constexpr int N = Shape<WIDE>::N;
     if constexpr (WIDE) {
 #pragma unroll
@@ -147,15 +152,15 @@ __device__ __forceinline__ void load_weights(const float* w, const Place<WIDE>& 
             const float4_t x = *reinterpret_cast<const float4_t*>(w + at.a[0] + i), y = *reinterpret_cast<const float4_t*>(w + at.b[0] + i);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                a[i + j] = x[j];
-                b[i + j] = y[j];
+                a[i + j] *= x[j];
+                b[i + j] *= y[j];
             }
         }
     } else {
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            a[j] = at.a[j] >= 0 ? w[at.a[j]] : 0.0f;
-            b[j] = at.b[j] >= 0 ? w[at.b[j]] : 0.0f;
+            a[j] *= w[at.a[j] < 0 ? 0 : at.a[j]];
+            b[j] *= w[at.b[j] < 0 ? 0 : at.b[j]];
         }
     }
 }
@@ -205,141 +210,190 @@ __device__ __forceinline__ void norm(float (&a)[N], float (&b)[N], bool on, int 
     }
 }
 
-// I: the input type; O: the results'. A workgroup has an item's rows, or (not appending) rows_each rows; its
-// waves take tasks of a row and up to kIts groups of heads.
+// The pairs (a, b) by their angles; gain: 1 but for magnitudes past 1.
+__device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) {
+    const float x = a;
+    a = __builtin_fmaf(x, c, -(b * s));
+    b = __builtin_fmaf(x, s, b * c);
+}
+
+// I: the input type; O: the results'. A workgroup has up to rows_each rows. A wave takes a row, or, where there are
+// fewer rows than waves, a part of its heads, kIts groups of heads at a time: with four groups instead of two, at
+// half the waves a SIMD, 8192 tokens of 32 + 8 + 8 heads of 128 took 59 us to append and not 52. The norms' weights are in LDS, a row for each kind of head: in registers, picked by each lane's kind, they took
+// 10% of that time.
 template <typename I, typename O, bool WIDE, bool APPEND>
 __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem& it) {
-    constexpr int N = Shape<WIDE>::N, kIts = Shape<WIDE>::kIts;
+    constexpr int N = Shape<WIDE>::N, kIts = Shape<WIDE>::kIts, kMaxDim = 512;
     typedef typename StoredAs<I>::Type Stored;
-    __shared__ float2 shared[WIDE ? 4 * 256 : 1];
+    __shared__ float2 angles[WIDE ? 4 * kMaxDim / 2 : 1];
+    __shared__ __attribute__((aligned(16))) float weights[3][kMaxDim];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     const int log = lanes_log<WIDE>(h.head_dim), at_once = 64 >> log;
     const int all = h.heads + (APPEND ? 2 : 1) * h.kv_heads;
-    const int groups = (all + at_once - 1) / at_once, chunks = (groups + kIts - 1) / kIts, each = (groups + chunks - 1) / chunks;
+    const int groups = (all + at_once - 1) / at_once, chunks = (groups + kIts - 1) / kIts;
     Place<WIDE> at;
     at.init(h, lane & ((1 << log) - 1));
     const float inv_dim = 1.0f / float(h.head_dim);
-    float2* const mine = shared + (WIDE ? wave * 256 : 0);
+    float2* const mine = angles + (WIDE ? wave * (kMaxDim / 2) : 0);
+    // a head's kind: 0 q, 1 k, 2 v; its number among them
+    auto kind_of = [&](int head) { return head < h.heads ? 0 : head < h.heads + h.kv_heads ? 1 : 2; };
+    auto number_of = [&](int head, int kind) { return kind == 0 ? head : kind == 1 ? head - h.heads : head - h.heads - h.kv_heads; };
+    auto load = [&](Raw<I, WIDE>& raw, int r, int group) {
+        const int head = group * at_once + (lane >> log), kind = kind_of(head);
+        if (group < groups && head < all && at.any) {
+            const void* const base = kind == 0 ? h.q : kind == 1 ? h.k : h.v;
+            const int64_t stride = kind == 0 ? h.q_stride : kind == 1 ? h.k_stride : h.v_stride;
+            raw.load(static_cast<const Stored*>(base) + (size_t(it.row0) + uint32_t(r)) * size_t(stride) + size_t(number_of(head, kind)) * size_t(h.head_dim), at);
+        } else {
+            raw = Raw<I, WIDE>{};
+        }
+    };
+    // A wave's steps: chunks [chunk0, chunk1) of its rows r, r + stride, ..., each loaded a step ahead.
+    const bool split = int(it.n) < 4;  // parts of a row
+    const int chunk0 = split ? wave / int(it.n) : 0, step = split ? (4 + int(it.n) - 1 - wave % int(it.n)) / int(it.n) : 1;
+    const int stride = split ? int(it.n) : 4;
+    int r = split ? wave % int(it.n) : wave, chunk = chunk0;
+    if (chunk >= chunks) r = int(it.n);
+    Raw<I, WIDE> raw[kIts];
+    if (r < int(it.n)) {
+#pragma unroll
+        for (int i = 0; i < kIts; i++) load(raw[i], r, chunk * kIts + i);
+    }
+    if (h.normed) {
+        for (int i = threadIdx.x; i < h.head_dim; i += 256) {
+            weights[0][i] = h.normed & kNormQ && h.q_norm ? h.q_norm[i] : 1.0f;
+            weights[1][i] = h.normed & kNormK && h.k_norm ? h.k_norm[i] : 1.0f;
+            weights[2][i] = 1.0f;
+        }
+        __syncthreads();
+    }
 
-    for (int task = wave; task < int(it.n) * chunks; task += 4) {
-        const int r = task / chunks, group0 = task % chunks * each;
+    float cs[N], sn[N];
+    size_t page_at = 0;  // of the row, in its page's first head
+    while (r < int(it.n)) {
         const size_t row = size_t(it.row0) + uint32_t(r);
-        Raw<I, WIDE> raw[kIts];
-#pragma unroll
-        for (int i = 0; i < kIts; i++) {
-            const int head = (group0 + i) * at_once + (lane >> log);
-            if (i < each && head < all && at.any) {
-                const bool q = head < h.heads, k = head < h.heads + h.kv_heads;
-                const Stored* const p = static_cast<const Stored*>(q ? h.q : k ? h.k : h.v) +
-                                        row * size_t(q ? h.q_stride : k ? h.k_stride : h.v_stride) +
-                                        size_t(q ? head : k ? head - h.heads : head - h.heads - h.kv_heads) * size_t(h.head_dim);
-                raw[i].load(p, at);
-            } else {
-                raw[i].clear();
+        if (chunk == chunk0) {
+            if constexpr (APPEND) {
+                const uint32_t key = it.first + uint32_t(r);
+                const int page = __builtin_amdgcn_readfirstlane(h.table[size_t(it.slot) * size_t(h.slot_pages) + (key >> h.page_shift)]);
+                page_at = size_t(page) * size_t(h.page_stride) + size_t(key & ((1u << h.page_shift) - 1)) * size_t(h.head_dim);
             }
-        }
-        size_t page_at = 0;  // of the row, in its page's first head
-        if constexpr (APPEND) {
-            const uint32_t key = it.first + uint32_t(r);
-            const int32_t page = h.table[size_t(it.slot) * size_t(h.slot_pages) + (key >> h.page_shift)];
-            page_at = size_t(page) * size_t(h.page_stride) + size_t(key & ((1u << h.page_shift) - 1)) * size_t(h.head_dim);
-        }
-        float cs[N], sn[N];
-        if (h.half) {
-            const double position = h.positions ? double(h.positions[row]) : double(it.first + uint32_t(r));
-            auto turn = [&](int pair, float& c, float& s) {
-                const double t = position * h.turns[pair];
-                sincospif(2.0f * float(t - rint(t)), &s, &c);
-                c *= h.fade;
-                s *= h.fade;
-            };
-            if constexpr (WIDE) {
-                for (int pair = lane; pair < h.half; pair += 64) turn(pair, mine[pair].x, mine[pair].y);
-                __builtin_amdgcn_wave_barrier();
-                const int first = at.pair[0] < 0 ? 0 : at.pair[0];
+            if (h.half) {
+                const double position = h.positions ? double(h.positions[row]) : double(it.first + uint32_t(r));
+                auto turn = [&](int pair, float& c, float& s) {
+                    const double t = position * h.turns[pair];
+                    sincospif(2.0f * float(t - rint(t)), &s, &c);
+                    c *= h.fade;
+                    s *= h.fade;
+                };
+                if constexpr (WIDE) {
+                    for (int pair = lane; pair < h.half; pair += 64) {
+                        float c, s;
+                        turn(pair, c, s);
+                        mine[pair] = float2{c, s};
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                    const int first = at.pair[0] < 0 ? 0 : at.pair[0];
 #pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const float2 x = mine[first + i];
-                    cs[i] = x.x;
-                    sn[i] = x.y;
+                    for (int i = 0; i < N; i++) {
+                        const float2 x = mine[first + i];
+                        cs[i] = x.x;
+                        sn[i] = x.y;
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; j++) turn(at.pair[j] < 0 ? 0 : at.pair[j], cs[j], sn[j]);
                 }
-                __builtin_amdgcn_wave_barrier();
-            } else {
-#pragma unroll
-                for (int j = 0; j < N; j++) turn(at.pair[j] < 0 ? 0 : at.pair[j], cs[j], sn[j]);
             }
         }
+        const bool last = chunk + step >= chunks;
+        const int r_next = last ? r + stride : r, chunk_next = last ? chunk0 : chunk + step;
 #pragma unroll
         for (int i = 0; i < kIts; i++) {
-            if (i >= each || (group0 + i) * at_once >= all) continue;
-            const int head = (group0 + i) * at_once + (lane >> log);
-            const bool q = head < h.heads, k = head < h.heads + h.kv_heads;
+            const int group = chunk * kIts + i, head = group * at_once + (lane >> log), kind = kind_of(head);
+            const bool here = group < groups && head < all;
             float a[N], b[N];
             raw[i].values(a, b);
+            if (r_next < int(it.n)) load(raw[i], r_next, chunk_next * kIts + i);
             if (h.normed) {
-                const bool on = (h.normed & (q ? kNormQ : k ? kNormK : kNormV)) != 0 && head < all;
-                norm(a, b, on, log, inv_dim, h.eps);
-                const float* const w = q ? h.q_norm : k ? h.k_norm : nullptr;
-                if (on && w && at.any) {
-                    float wa[N], wb[N];
-                    load_weights<WIDE>(w, at, wa, wb);
-#pragma unroll
-                    for (int j = 0; j < N; j++) {
-                        a[j] *= wa[j];
-                        b[j] *= wb[j];
-                    }
-                }
+                norm(a, b, here && (h.normed >> kind & 1), log, inv_dim, h.eps);
+                if (here && at.any) weigh<WIDE>(weights[kind], at, a, b);
             }
-            if (h.half && k) {
+            if (!here || !at.any) continue;
+            if (h.half && kind < 2) {
+                if constexpr (WIDE) {
+                    if (at.pair[0] >= 0) {
+                        if (h.pairs) {  // neighbours: pairs i of a and 4 + i of b
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    if (at.pair[WIDE ? 0 : j] < 0) continue;
-                    if (WIDE && h.pairs) continue;
-                    const float x = a[j], y = b[j];
-                    a[j] = __builtin_fmaf(x, cs[j], -(y * sn[j])) * h.gain;
-                    b[j] = __builtin_fmaf(x, sn[j], y * cs[j]) * h.gain;
-                }
-                if constexpr (WIDE) {  // neighbours: pairs i of a and 4 + i of b
-                    if (h.pairs && at.pair[0] >= 0) {
+                            for (int j = 0; j < N; j += 2) {
+                                turn_pair(a[j], a[j + 1], cs[j / 2], sn[j / 2]);
+                                turn_pair(b[j], b[j + 1], cs[4 + j / 2], sn[4 + j / 2]);
+                            }
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < N; j += 2) {
-                            const float x = a[j], y = a[j + 1], z = b[j], w = b[j + 1];
-                            a[j] = __builtin_fmaf(x, cs[j / 2], -(y * sn[j / 2])) * h.gain;
-                            a[j + 1] = __builtin_fmaf(x, sn[j / 2], y * cs[j / 2]) * h.gain;
-                            b[j] = __builtin_fmaf(z, cs[4 + j / 2], -(w * sn[4 + j / 2])) * h.gain;
-                            b[j + 1] = __builtin_fmaf(z, sn[4 + j / 2], w * cs[4 + j / 2]) * h.gain;
+                            for (int j = 0; j < N; j++) turn_pair(a[j], b[j], cs[j], sn[j]);
                         }
                     }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; j++)
+                        if (at.pair[j] >= 0) turn_pair(a[j], b[j], cs[j], sn[j]);
+                }
+                if (h.gain != 1.0f) {
+#pragma unroll
+                    for (int j = 0; j < N; j++)
+                        if (at.pair[WIDE ? 0 : j] >= 0) {
+                            a[j] *= h.gain;
+                            b[j] *= h.gain;
+                        }
                 }
             }
-            if (head >= all || !at.any) continue;
+            const size_t number = size_t(number_of(head, kind));
             uint16_t* p;
-            if (q) {
-                p = h.q_out + row * size_t(h.q_out_stride) + size_t(head) * size_t(h.head_dim);
-            } else {
-                const size_t kvh = size_t(k ? head - h.heads : head - h.heads - h.kv_heads);
-                uint16_t* const out = k ? h.k_out : h.v_out;
-                if constexpr (APPEND)
-                    p = out + page_at + (kvh << h.page_shift) * size_t(h.head_dim);
-                else
-                    p = out + row * size_t(h.k_out_stride) + kvh * size_t(h.head_dim);
-            }
+            if (kind == 0)
+                p = h.q_out + row * size_t(h.q_out_stride) + number * size_t(h.head_dim);
+            else if constexpr (APPEND)
+                p = (kind == 1 ? h.k_out : h.v_out) + page_at + (number << h.page_shift) * size_t(h.head_dim);
+            else
+                p = h.k_out + row * size_t(h.k_out_stride) + number * size_t(h.head_dim);
             store<O, WIDE>(p, at, a, b);
         }
+        r = r_next;
+        chunk = chunk_next;
     }
 }
 
 template <typename I, typename O, bool WIDE>
-__global__ __launch_bounds__(256) void rotate_heads_kernel(const HeadsArgs h) {
+__global__ __launch_bounds__(256, sizeof(typename StoredAs<I>::Type) == 2 ? 4 : 3) void rotate_heads_kernel(const HeadsArgs h) {
     const int row0 = int(blockIdx.x) * h.rows_each;
-    const AppendItem it{uint32_t(row0), uint32_t(min(h.rows_each, h.rows - row0)), 0, 0};
+    const AppendItem it{uint32_t(row0), uint32_t(min(h.rows_each, h.rows - row0)), 0, 0, 0};
     heads_body<I, O, WIDE, false>(h, it);
 }
 
 template <typename I, typename O, bool WIDE>
-__global__ __launch_bounds__(256) void append_kernel(const HeadsArgs h, const AppendInline in) {
-    const AppendItem* const p = h.items ? h.items + blockIdx.x : in.items + blockIdx.x;
-    const AppendItem it = *p;
+__global__ __launch_bounds__(256, sizeof(typename StoredAs<I>::Type) == 2 ? 4 : 3) void append_kernel(const HeadsArgs h, const AppendInline in) {
+    auto scalar = [](uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); };
+    AppendItem it;
+    if (h.items) {
+        const AppendItem* const p = h.items + blockIdx.x;
+        it = AppendItem{scalar(p->row0), scalar(p->n), scalar(p->slot), scalar(p->first), blockIdx.x};
+    } else {
+        // the last item that begins at or before this workgroup
+        const bool each = h.workgroups == h.n_items;
+        int at = each ? int(blockIdx.x) : 0;
+        for (int n = each ? 1 : h.n_items; n > 1;) {
+            const int half = n / 2;
+            if (in.items[at + half].group0 <= blockIdx.x) {
+                at += half;
+                n -= half;
+            } else {
+                n = half;
+            }
+        }
+        const uint32_t skip = (blockIdx.x - in.items[at].group0) * uint32_t(h.rows_each);
+        it = AppendItem{in.items[at].row0 + skip, min(in.items[at].n - skip, uint32_t(h.rows_each)), in.items[at].slot, in.items[at].first + skip, blockIdx.x};
+    }
     heads_body<I, O, WIDE, true>(h, it);
 }
 
@@ -366,9 +420,9 @@ hipError_t run_rotate(hipStream_t s, const HeadsArgs& a, bool wide) {
 template <typename I, typename O>
 hipError_t run_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool wide) {
     if (wide)
-        launch_kernel(append_kernel<I, O, true>, dim3(uint32_t(a.n_items)), dim3(256), 0, s, a, in);
+        launch_kernel(append_kernel<I, O, true>, dim3(uint32_t(a.workgroups)), dim3(256), 0, s, a, in);
     else
-        launch_kernel(append_kernel<I, O, false>, dim3(uint32_t(a.n_items)), dim3(256), 0, s, a, in);
+        launch_kernel(append_kernel<I, O, false>, dim3(uint32_t(a.workgroups)), dim3(256), 0, s, a, in);
     return hipGetLastError();
 }
 
@@ -382,7 +436,8 @@ hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, b
 }
 
 hipError_t launch_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool in_f32, bool bf16, bool wide) {
-    if (!heads_ok(a) || a.n_items < 0 || (!a.items && a.n_items > kAppendInlineItems)) return hipErrorInvalidValue;
+    if (!heads_ok(a) || a.n_items < 0 || a.workgroups < a.n_items || a.rows_each <= 0 || (a.items ? a.workgroups != a.n_items : a.n_items > kAppendInlineItems))
+        return hipErrorInvalidValue;
     if (a.n_items == 0) return hipSuccess;
     if (in_f32) return bf16 ? run_append<F32, BF16>(s, a, in, wide) : run_append<F32, F16>(s, a, in, wide);
     return bf16 ? run_append<BF16, BF16>(s, a, in, wide) : run_append<F16, F16>(s, a, in, wide);

@@ -7,11 +7,12 @@
 
 namespace ge {
 
-// Rows [row0, row0 + n) of one sequence, cached at rows first, first + 1, ... of table slot `slot`.
+// Rows [row0, row0 + n) of one sequence, cached at rows first, first + 1, ... of table slot `slot`; workgroups from
+// group0 on take rows_each of them each.
 struct AppendItem {
-    uint32_t row0, n, slot, first;
+    uint32_t row0, n, slot, first, group0;
 };
-constexpr int kAppendInlineItems = 200;
+constexpr int kAppendInlineItems = 160;
 // The list of a call that has few, among the kernel's arguments.
 struct AppendInline {
     AppendItem items[kAppendInlineItems];
@@ -26,7 +27,7 @@ struct HeadsArgs {
     const int32_t* positions;        // [rows], null: the cache row (appending only)
     const double* turns;             // [half]: turns of a full circle a position
     const int32_t* table;            // [slots][slot_pages]
-    const AppendItem* items;         // null: in AppendInline when appending
+    const AppendItem* items;         // appending: an item a workgroup; null: in AppendInline, to be searched
     int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;  // elements from one row to the next
     int64_t page_stride;             // elements from one page to the next
     int heads, kv_heads, head_dim, rows;
@@ -34,13 +35,14 @@ struct HeadsArgs {
     int pairs;                       // 1: neighbours are a pair, 0: elements half apart
     int normed;                      // kNorm bits
     float eps, fade, gain;           // fade gain: the magnitude, fade <= 1 <= |gain|
-    int rows_each;                   // rows of a workgroup (not appending)
+    int rows_each, workgroups;       // rows of a workgroup
     int n_items, slot_pages, page_shift;
 };
 static_assert(sizeof(HeadsArgs) + sizeof(AppendInline) <= 4096, "kernel arguments");
 
-// Rows of a workgroup: about 2048 workgroups in long calls, a row a wave in short ones.
-inline int heads_rows_each(int rows) { return rows <= 8192 ? 4 : (rows / 2048 + 3) / 4 * 4; }
+// Rows of a workgroup: a row a wave, up to 4096 workgroups. (16384 rows of 32 + 8 heads of 128 in 4096, 2048, 1024 and
+// 512: 66.7, 70.9, 73.5 and 83.0 us.)
+inline int heads_rows_each(int rows) { return rows <= 4 * 4096 ? 4 : (rows / 4096 + 3) / 4 * 4; }
 
 // wide: everything is in whole 16-byte pieces (heads_wide).
 hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, bool bf16, bool wide);

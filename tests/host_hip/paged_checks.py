@@ -52,7 +52,7 @@ class JoinInline(C.Structure):
 
 class Append(C.Structure):
     """AppendItem, rotary.hpp"""
-    _fields_ = [(n, U) for n in ("row0", "n", "slot", "first")]
+    _fields_ = [(n, U) for n in ("row0", "n", "slot", "first", "group0")]
 
 
 class Heads(C.Structure):
@@ -61,7 +61,7 @@ class Heads(C.Structure):
         [("items", C.POINTER(Append))] + [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride",
                                                                  "k_out_stride", "page_stride")] + \
         [(n, I) for n in ("heads", "kv_heads", "head_dim", "rows", "half", "pairs", "normed")] + \
-        [(n, C.c_float) for n in ("eps", "fade", "gain")] + [(n, I) for n in ("rows_each", "n_items", "slot_pages", "page_shift")]
+        [(n, C.c_float) for n in ("eps", "fade", "gain")] + [(n, I) for n in ("rows_each", "workgroups", "n_items", "slot_pages", "page_shift")]
 
 
 class Launches:
@@ -75,9 +75,15 @@ class Launches:
                 name = name.decode()
                 self.names.append(name)
                 if "append_kernel" in name:
-                    a, few = C.cast(args[0], C.POINTER(Heads))[0], C.cast(args[1], C.POINTER(Append * 200))[0]
+                    a, few = C.cast(args[0], C.POINTER(Heads))[0], C.cast(args[1], C.POINTER(Append * 160))[0]
                     self.args = {f: getattr(a, f) for f, _ in Heads._fields_ if f != "items"}
-                    self.appended = [Append.from_buffer_copy((a.items or few)[i]) for i in range(a.n_items)]
+                    items, self.appended = [Append.from_buffer_copy((a.items or few)[i]) for i in range(a.n_items)], []
+                    assert bool(a.items) == (a.n_items > 160) and (not a.items or a.workgroups == a.n_items)
+                    for g in range(a.workgroups):  # what each takes
+                        i = items[g] if a.items else [x for x in items if x.group0 <= g][-1]
+                        skip = (g - i.group0) * a.rows_each
+                        assert g >= i.group0 and skip < i.n
+                        self.appended.append(Append(i.row0 + skip, min(i.n - skip, a.rows_each), i.slot, i.first + skip, g))
                 elif "rotate_heads_kernel" in name:
                     a = C.cast(args[0], C.POINTER(Heads))[0]
                     self.args = {f: getattr(a, f) for f, _ in Heads._fields_ if f != "items"}
