@@ -419,7 +419,7 @@ void attend(ge_ctx* c, const ge_paged_shape* shape, const void* q, const ge_page
         c->paged_ready = true;
     }
     const PagedPlan p = plan_paged(s, seqs, n_seqs);
-    if (p.workgroups * uint64_t(s.kv_heads) > kCausalMaxGroups || p.joins.size() * uint64_t(s.kv_heads) > kCausalMaxGroups ||
+    if (p.workgroups * uint64_t(s.kv_heads) > kCausalMaxGroups || p.joins.size() * uint64_t(s.kv_heads) > kCausalMaxGroups / 4 ||
         p.items.size() >= kDirect || p.part_rows >= kDirect)
         fail(GE_ERR_INVALID, "%s: the call's rows and keys are too many for one call", kAttend);
     OpTemps temps(c);
@@ -469,7 +469,12 @@ void attend(ge_ctx* c, const ge_paged_shape* shape, const void* q, const ge_page
     }
     launch(c, kAttend, [&] { return launch_paged(c->stream, a, in, s.head_dim, s.type == GE_TYPE_BF16, p.kinds); });
     if (a.n_joins)
-        launch(c, "attention_join", [&] { return launch_causal_join(c->stream, a, join_in, s.head_dim, s.type == GE_TYPE_BF16); });
+        launch(c, "attention_join", [&] {
+            // four parts a group of lanes: few rows of many parts
+            int split = 1;
+            while (split < 16 && p.join_parts > 4 * split) split *= 2;
+            return launch_paged_join(c->stream, a, join_in, s.head_dim, s.type == GE_TYPE_BF16, split);
+        });
     hip_check(hipStreamSynchronize(c->stream), "hipStreamSynchronize");
 }
 

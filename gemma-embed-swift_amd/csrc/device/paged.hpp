@@ -36,8 +36,10 @@ constexpr int paged_workgroups(int hd) {
 }
 constexpr int kPagedAlign = 8;  // copies are of 8 keys, which are in one page
 
-// Head dims as causal_head_dim_ok; kinds: the CausalKind of the items. Joins: launch_causal_join.
+// Head dims as causal_head_dim_ok; kinds: the CausalKind of the items.
 hipError_t launch_paged(hipStream_t s, const PagedArgs& a, const PagedInline& in, int hd, bool bf16, int kinds);
+// The joins' rows (splits[0] parts each; splits[1] is 0), `split` groups of lanes to a row: a power of two.
+hipError_t launch_paged_join(hipStream_t s, const CausalArgs& a, const CausalInline& in, int hd, bool bf16, int split);
 // Dynamic LDS limits; once per device, before launching.
 hipError_t paged_configure();
 

@@ -91,6 +91,7 @@ void add_join(PagedPlan& p, const Tile& t, const ge_paged_seq& e, size_t first_p
     j.splits[0] = splits;
     p.joins.push_back(j);
     p.join_rows = std::max(p.join_rows, int(t.n_rows));
+    p.join_parts = std::max(p.join_parts, int(splits));
 }
 
 // Raises the parts of the group with the longest ones while the items stay within `most`; returns the longest part.

@@ -14,7 +14,7 @@ struct PagedPlan {
     std::vector<CausalJoin> joins;
     size_t workgroups = 0;  // a KV head
     size_t part_rows = 0;
-    int kinds = 0, join_rows = 0;
+    int kinds = 0, join_rows = 0, join_parts = 0;  // the most rows and parts of a join
 };
 
 // The call's sequences are checked: rows ascend, counts are under 2^30.

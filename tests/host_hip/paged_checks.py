@@ -100,7 +100,7 @@ class Launches:
                                 break
                             assert at >= a.n_items
                     self.items = [i for chain in self.chains for i in chain]
-                elif "causal_join_kernel" in name:
+                elif "paged_join_kernel" in name:
                     a, few = C.cast(args[0], C.POINTER(JoinArgs))[0], C.cast(args[1], C.POINTER(JoinInline))[0]
                     self.joins = [Join.from_buffer_copy((a.joins or few.joins)[i]) for i in range(a.n_joins)]
                 elif "table_set_kernel" in name:
@@ -432,7 +432,7 @@ def test_rows_of_a_long_append(ctx, memory):
             append(ctx, memory, None, h, seqs, dict(rows=1 << 17) if len(seqs) != 10 else dict(rows=80000))
         rows = [(i.row0 + r, i.slot, i.first + r) for i in got.appended for r in range(i.n)]
         assert sorted(rows) == sorted((q + r, s, m - n + r) for q, n, s, m in seqs for r in range(n))
-        assert len(got.appended) <= 2048 + len(seqs)
+        assert len(got.appended) <= 5120 + len(seqs)
     ctx.page_table_destroy(h)
 
 
@@ -537,7 +537,7 @@ def test_caps(ctx, memory, table):
     assert np.isfinite(a["cap_z"]) and a["cap_top"] > 0
 
 
-@pytest.mark.parametrize("what", [b"kernel:paged_kernel", b"kernel:causal_join", b"hipStreamSynchronize", b"hipMalloc"])
+@pytest.mark.parametrize("what", [b"kernel:paged_kernel", b"kernel:paged_join", b"hipStreamSynchronize", b"hipMalloc"])
 def test_a_call_that_fails_leaves_nothing_in_flight(ctx, memory, what):
     h = ctx.page_table_create(1, 5000, 16, 5000)
     ctx.page_table_set(h, [(0, i, i) for i in range(5000)])
