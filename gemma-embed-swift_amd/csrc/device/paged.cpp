@@ -202,6 +202,13 @@ void check_operands(const char* op, std::initializer_list<Operand> list, bool* w
     }
 }
 
+// Results may take their operand's place row by row and head by head, where both are of one type.
+void check_in_place(const char* op, const char* what, const ge_heads_shape& s, const void* in, int64_t in_stride, const void* out,
+                    int64_t out_stride) {
+    if (in && in == out && (s.in_type != s.type || (s.rows > 1 && in_stride != out_stride)))
+        fail(GE_ERR_INVALID, "%s: %s in its own place, of another type or row stride", op, what);
+}
+
 void rotate(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const void* q, const void* k, const void* q_norm,
             const void* k_norm, const void* positions, void* q_out, void* k_out) {
     ge_heads_shape s;
@@ -211,6 +218,8 @@ void rotate(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const vo
     const size_t in = s.in_type == GE_TYPE_F32 ? 4 : 2;
     check_operands(kRotate, {{"q", q, s.heads > 0, in}, {"k", k, s.kv_heads > 0, in}, {"q_out", q_out, s.heads > 0, 2},
                              {"k_out", k_out, s.kv_heads > 0, 2}, {"q_norm", q_norm, false, 4}, {"k_norm", k_norm, false, 4}}, &wide);
+    check_in_place(kRotate, "q", s, q, s.q_stride, q_out, s.q_out_stride);
+    check_in_place(kRotate, "k", s, k, s.k_stride, k_out, s.k_out_stride);
     if (r && !positions) fail(GE_ERR_INVALID, "%s: null positions", kRotate);
     if (!aligned(positions, 4)) fail(GE_ERR_INVALID, "%s: positions are not aligned to their elements", kRotate);
     a.q = q;
@@ -272,6 +281,7 @@ void append(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const vo
     check_operands(kAppend, {{"q", q, s.heads > 0, in}, {"k", k, true, in}, {"v", v, true, in}, {"q_out", q_out, s.heads > 0, 2},
                              {"k_pages", k_pages, true, 2}, {"v_pages", v_pages, true, 2}, {"q_norm", q_norm, false, 4},
                              {"k_norm", k_norm, false, 4}}, &wide);
+    check_in_place(kAppend, "q", s, q, s.q_stride, q_out, s.q_out_stride);
     if (!aligned(positions, 4)) fail(GE_ERR_INVALID, "%s: positions are not aligned to their elements", kAppend);
     claim_pages(t, seqs, n_seqs);
 
@@ -345,6 +355,8 @@ void set_pages(ge_ctx* c, ge_page_table* t, const ge_page_entry* entries, int n)
     if (size_t(highest) + 1 > t->writer.size()) t->writer.resize(size_t(highest) + 1, 0u);
     auto place = [&](const ge_page_entry& e) { return size_t(e.slot) * size_t(t->slot_pages) + e.index; };
     std::vector<int32_t> before(static_cast<size_t>(n));
+    std::vector<uint32_t> again;
+    again.reserve(static_cast<size_t>(n));  // nothing can fail once the pages are set
     OpTemps temps(c);
     uint2* const list = reinterpret_cast<uint2*>(op_lists(c, size_t(n) * sizeof(uint2)));
     for (int i = 0; i < n; i++) {
@@ -362,7 +374,6 @@ void set_pages(ge_ctx* c, ge_page_table* t, const ge_page_entry* entries, int n)
     }
     // A page behind a slot's last one, the common case, lengthens its run; the runs of slots with any other entry
     // are found again.
-    std::vector<uint32_t> again;
     for (int i = 0; i < n; i++) {
         ge_page_table::Run& r = t->runs[entries[i].slot];
         if (entries[i].page >= 0 && int(entries[i].index) == r.end && r.end > 0 && t->pages[place(entries[i])] >= 0)
@@ -512,9 +523,11 @@ int ge_op_rotary_create(ge_ctx* c, const ge_rotary_desc* desc, ge_rotary** out) 
 
 int ge_op_rotary_destroy(ge_ctx* c, ge_rotary* r) {
     if (!r) return GE_OK;
-    const int rc = guarded(c, [&] { ge::hip_check(hipFree(r->turns), "hipFree"); });
-    delete r;
-    return rc;
+    return guarded(c, [&] {
+        if (r->ctx != c) fail(GE_ERR_INVALID, "rotary: the rotary positions are another context's");
+        ge::hip_check(hipFree(r->turns), "hipFree");
+        delete r;
+    });
 }
 
 int ge_op_rotate_heads(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* rotary, const void* q, const void* k,
@@ -557,9 +570,11 @@ int ge_op_page_table_set(ge_ctx* c, ge_page_table* t, const ge_page_entry* entri
 
 int ge_op_page_table_destroy(ge_ctx* c, ge_page_table* t) {
     if (!t) return GE_OK;
-    const int rc = guarded(c, [&] { ge::hip_check(hipFree(t->dev), "hipFree"); });
-    delete t;
-    return rc;
+    return guarded(c, [&] {
+        ge::check_table("page table", c, t);
+        ge::hip_check(hipFree(t->dev), "hipFree");
+        delete t;
+    });
 }
 
 int ge_op_paged_append(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* rotary, const void* q, const void* k,

@@ -292,7 +292,8 @@ __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem&
                         turn(pair, c, s);
                         mine[pair] = float2{c, s};
                     }
-                    __builtin_amdgcn_wave_barrier();
+                    // (a wave's own LDS operations are in order: only the compiler has to keep it)
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                     const int first = at.pair[0] < 0 ? 0 : at.pair[0];
 #pragma unroll
                     for (int i = 0; i < N; i++) {
@@ -300,7 +301,7 @@ __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem&
                         cs[i] = x.x;
                         sn[i] = x.y;
                     }
-                    __builtin_amdgcn_wave_barrier();
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 } else {
 #pragma unroll
                     for (int j = 0; j < N; j++) turn(at.pair[j] < 0 ? 0 : at.pair[j], cs[j], sn[j]);

@@ -336,7 +336,7 @@ int ge_op_attention_prefix(ge_ctx* ctx, const ge_attention_shape* shape, const v
  * position f_i, to (a cos - b sin, a sin + b cos) magnitude. f_i = base^(-2 i / dims), and for positions past those a
  * model was trained on: LINEAR f_i / factor; BY_TURNS f_i (w + (1 - w) / factor), w = the part, from 0 to 1, of the way
  * from low_turns to high_turns that the pair's trained f_i / 2 pi turns are. The angle is reduced in fp64. The
- * handle belongs to the context that made it, as a page table does; destroy both before the context. */
+ * handle belongs to the context that made it, as a page table does, and is destroyed in it, before it. */
 enum { GE_ROTARY_HALVES = 0, GE_ROTARY_PAIRS = 1 };
 enum { GE_ROTARY_PLAIN = 0, GE_ROTARY_LINEAR = 1, GE_ROTARY_BY_TURNS = 2 };
 typedef struct ge_rotary_desc {
@@ -413,9 +413,10 @@ int ge_op_paged_append(ge_ctx* ctx, const ge_heads_shape* shape, const ge_rotary
 /* ge_op_attention_causal over pages: out_i = sum_j softmax_j(s_ij) v_j over the keys j <= i + kv_len - q_len of the
  * sequence's slot and, with a window, j > i + kv_len - q_len - window; s_ij = scale q_i . k_j, or with a cap
  * cap tanh(scale q_i . k_j / cap). q and out are rows of heads x head_dim (q_stride, out_stride), pools as
- * ge_op_paged_append has them; what ge_op_attention_causal says of types, limits, precision, rows that see no key, hidden, infinite and
- * NaN values, and rows outside the sequences holds here too; a cap
- * moves a weight by 2^-21 cap of itself at most. page_stride is a multiple of 8. The pages of every key that a row sees must be in the slot; earlier ones may have been taken out. */
+ * ge_op_paged_append has them, page_stride a multiple of 8. What ge_op_attention_causal says of types, limits,
+ * precision, rows that see no key, hidden, infinite and NaN values, and rows outside the sequences holds here too; a
+ * cap moves a weight by 2^-21 cap of itself at most. The pages of every key that a row sees must be in the slot;
+ * earlier ones may have been taken out. */
 typedef struct ge_paged_shape {
     int32_t type;
     int32_t heads, kv_heads, head_dim;

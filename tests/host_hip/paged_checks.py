@@ -283,7 +283,7 @@ ROTATE = dict(in_type=F16, type=F16, heads=4, kv_heads=2, head_dim=64, rows=3)
 
 
 def rotate(ctx, memory, rotary, shape=None, **kw):
-    a = dict(rotary=rotary, q=memory, k=memory, q_norm=None, k_norm=None, positions=memory, q_out=memory, k_out=memory)
+    a = dict(rotary=rotary, q=memory, k=memory, q_norm=None, k_norm=None, positions=memory, q_out=memory + 4096, k_out=memory + 4096)
     a.update(kw)
     ctx.rotate_heads(ge.heads_shape(**dict(ROTATE, **(shape or {}))), a["rotary"], a["q"], a["k"], a["q_norm"], a["k_norm"],
                      a["positions"], a["q_out"], a["k_out"])
@@ -316,6 +316,32 @@ def test_refused_operands(ctx, memory, rotary):
         rotate(ctx, memory, rotary, dict(rows=0), q=None, k=None, q_out=None, k_out=None, positions=None)
     assert not got.names
     assert lib.ge_op_rotate_heads(ctx.handle, None, rotary, *[memory] * 7) == ge.GE_ERR_INVALID
+
+
+def test_results_in_their_operands_place(ctx, memory, rotary, table):
+    place = dict(q_out=memory, k_out=memory)
+    seqs = [(0, 3, 0, 50)]
+    rotate(ctx, memory, rotary, dict(q_stride=264, q_out_stride=264), **place)
+    rotate(ctx, memory, rotary, dict(q_stride=264, rows=1), **place)
+    append(ctx, memory, rotary, table, seqs, q_out=memory)
+    for bad in (dict(q_stride=264), dict(k_stride=136), dict(k_out_stride=136), dict(in_type=F32), dict(in_type=F32, rows=1)):
+        refused(rotate, ctx, memory, rotary, bad, **place)
+    for bad in (dict(q_stride=264), dict(in_type=F32)):
+        refused(append, ctx, memory, rotary, table, seqs, bad, q_out=memory)
+
+
+def test_handles_end_in_their_context(ctx):
+    rotary, table = ctx.rotary_create(64, 1e4), ctx.page_table_create(1, 1, 8, 1)
+    other = ge.Context.create(0)
+    refused(other.rotary_destroy, rotary)
+    refused(other.page_table_destroy, table)
+    assert lib.ge_op_rotary_destroy(None, rotary) == lib.ge_op_page_table_destroy(None, table) == ge.GE_ERR_INVALID
+    other.close()
+    ctx.page_table_set(table, [(0, 0, 0)])  # still there
+    ctx.rotary_destroy(rotary)
+    ctx.page_table_destroy(table)
+    ctx.rotary_destroy(None)
+    ctx.page_table_destroy(None)
 
 
 @pytest.mark.parametrize("shape,kw,wide", [
@@ -367,7 +393,7 @@ def test_frequencies(ctx, memory, dims, scaling, trained, factor):
 
 
 def append(ctx, memory, rotary, table, seqs, shape=None, **kw):
-    a = dict(rotary=rotary, q=memory, k=memory, v=memory, q_norm=None, k_norm=None, positions=None, q_out=memory, k_pages=memory,
+    a = dict(rotary=rotary, q=memory, k=memory, v=memory, q_norm=None, k_norm=None, positions=None, q_out=memory + 4096, k_pages=memory,
              v_pages=memory)
     a.update(kw)
     ctx.paged_append(ge.heads_shape(**dict(dict(ROTATE, rows=500), **(shape or {}))), a["rotary"], a["q"], a["k"], a["v"], a["q_norm"], a["k_norm"],
