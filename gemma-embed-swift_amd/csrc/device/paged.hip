@@ -132,12 +132,23 @@ struct Wide {
         };
         // The blocks of which the wave's rows see a key, in a loop of their own: accumulators that only some turns
         // change cost registers at every join.
+        // Of four workgroups a CU the oldest would end when the youngest has done half, and the CU run out of waves: an
+        // item's priority falls as it gets on. Head dim 64, 8192 tokens over 16192 keys: 485 us without, 465 with; 5 x 301 to
+        // 700 over 2000 to 9700 in parts: 95 and 89. (With two workgroups a CU it gains 1% or loses 4.)
+        constexpr bool kFalls = paged_workgroups(HD) > 2;
+        const int quarter = blocks / 4 + 1;
+        auto fall = [&](int b) {
+            if (kFalls && b == quarter) __builtin_amdgcn_s_setprio(2);
+            if (kFalls && b == 2 * quarter) __builtin_amdgcn_s_setprio(1);
+            if (kFalls && b == 3 * quarter) __builtin_amdgcn_s_setprio(0);
+        };
         const int first = min(max((w.lo_any - span.lo) / BK, 0), blocks);
         const int end = n <= 0 || w.hi_any < span.lo ? first : max(first, min(blocks, (w.hi_any - span.lo) / BK + 1));
         int b = 0;
         for (; b < first; b++) turn(b);
         for (; b < end; b++) {
             turn(b);
+            fall(b);
             unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
             typename Rows<T, HD, DW>::template Block<BK> blk;
             u32x4 p[BK / 16];
@@ -278,6 +289,7 @@ __global__ __launch_bounds__(256, paged_workgroups(HD)) void paged_kernel(const 
     for (;;) {
         int lane = int(threadIdx.x & 63);
         asm volatile("" : "+v"(lane));  // what an item makes of it is not kept over the loop, in registers that it needs
+        if (paged_workgroups(HD) > 2) __builtin_amdgcn_s_setprio(3);  // Wide lets it fall
         const PagedItem it = uniform_entry<PagedItem>(a.paged_items, in.items, at);
         if (KINDS == kCausalNarrow || ((KINDS & kCausalNarrow) && it.narrow))
             Narrow<T, HD, CURVE>::run(a, it, kvh, lane, paged_lds_mem);

@@ -34,7 +34,7 @@ struct StoredAs<F32> {
 // addresses that are not in such pieces: single elements, the whole wave on a head.
 template <bool WIDE>
 struct Shape {
-    static constexpr int N = WIDE ? 8 : 4, kIts = 2;  // kIts: groups of heads loaded together
+    static constexpr int N = WIDE ? 8 : 4;
 };
 
 // log2 of the lanes a head takes.
@@ -218,13 +218,15 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) 
 }
 
 // I: the input type; O: the results'. A workgroup has up to rows_each rows. A wave takes a row, or, where there are
-// fewer rows than waves, a part of its heads, kIts groups of heads at a time: with four groups instead of two, at
-// half the waves a SIMD, 8192 tokens of 32 + 8 + 8 heads of 128 took 59 us to append and not 52. The norms' weights are in LDS, a row for each kind of head: in registers, picked by each lane's kind, they took
-// 10% of that time.
+// fewer rows than waves, a part of its heads, kIts groups of heads at a time, which with four workgroups a CU is what
+// the registers hold. 8192 tokens of 32 + 8 + 8 heads of 128 to append, 16-bit: four groups at half the waves 59 us, two 47,
+// one 48 (at five workgroups 49, at six, which spill, 103); fp32: two at three workgroups 64 us, one at four 62 (5000
+// tokens of 5 heads of 256: 16.6 and 15.3). The norms' weights are in LDS, a row for each kind of head: in
+// registers, picked by each lane's kind, they took 10% of that time.
 template <typename I, typename O, bool WIDE, bool APPEND>
 __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem& it) {
-    constexpr int N = Shape<WIDE>::N, kIts = Shape<WIDE>::kIts, kMaxDim = 512;
     typedef typename StoredAs<I>::Type Stored;
+    constexpr int N = Shape<WIDE>::N, kIts = 4 / int(sizeof(Stored)), kMaxDim = 512;
     __shared__ float2 angles[WIDE ? 4 * kMaxDim / 2 : 1];
     __shared__ __attribute__((aligned(16))) float weights[3][kMaxDim];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
@@ -366,14 +368,14 @@ __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem&
 }
 
 template <typename I, typename O, bool WIDE>
-__global__ __launch_bounds__(256, sizeof(typename StoredAs<I>::Type) == 2 ? 4 : 3) void rotate_heads_kernel(const HeadsArgs h) {
+__global__ __launch_bounds__(256, 4) void rotate_heads_kernel(const HeadsArgs h) {
     const int row0 = int(blockIdx.x) * h.rows_each;
     const AppendItem it{uint32_t(row0), uint32_t(min(h.rows_each, h.rows - row0)), 0, 0, 0};
     heads_body<I, O, WIDE, false>(h, it);
 }
 
 template <typename I, typename O, bool WIDE>
-__global__ __launch_bounds__(256, sizeof(typename StoredAs<I>::Type) == 2 ? 4 : 3) void append_kernel(const HeadsArgs h, const AppendInline in) {
+__global__ __launch_bounds__(256, 4) void append_kernel(const HeadsArgs h, const AppendInline in) {
     auto scalar = [](uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); };
     AppendItem it;
     if (h.items) {

@@ -40,9 +40,11 @@ struct HeadsArgs {
 };
 static_assert(sizeof(HeadsArgs) + sizeof(AppendInline) <= 4096, "kernel arguments");
 
-// Rows of a workgroup: a row a wave, up to 4096 workgroups. (16384 rows of 32 + 8 heads of 128 in 4096, 2048, 1024 and
-// 512: 66.7, 70.9, 73.5 and 83.0 us.)
-inline int heads_rows_each(int rows) { return rows <= 4 * 4096 ? 4 : (rows / 4096 + 3) / 4 * 4; }
+// Rows of a workgroup. Few rows: one, its heads shared out to the waves, which then are one step long (to append 60,
+// 300, 1000, 2048 and 4000 tokens of 32 + 8 + 8 heads of 128: 6.0, 6.7, 9.8, 18.5 and 35 us, with a row a wave 10.7, 10.7, 12.5, 18.0
+// and 26). Else a row a wave, up to 4096 workgroups (16384 rows of 32 + 8 heads of 128 in 4096, 2048, 1024 and 512: 66.7, 70.9,
+// 73.5 and 83.0 us).
+inline int heads_rows_each(int rows) { return rows <= 1024 ? 1 : rows <= 4 * 4096 ? 4 : (rows / 4096 + 3) / 4 * 4; }
 
 // wide: everything is in whole 16-byte pieces (heads_wide).
 hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, bool bf16, bool wide);
