@@ -157,13 +157,13 @@ struct Wide {
             blk.product(w, at + Kv::kBytes, lane, p);
         }
         for (; b < blocks; b++) turn(b);
-        __syncthreads();  // no one reads K and V any more
+        // No one reads K and V any more. (With its barriers after the rows' stores a wave waited 1.7 us for those to arrive.)
+        held.share(lds);
         if (n > 0) {
             constexpr int kSlice = kLds / NW;
             w.l = sum_over_halves(w.l);
             w.template finish_rows<kSlice>(a, it, kvh, r0, n, lane, lds + wave * kSlice);
         }
-        held.share(lds);
         if (n > 0 && held.any) held.add(a, it, span, kvh, r0, n, w.d0 * 32, w.DT * 32);
     }
 };
@@ -297,7 +297,8 @@ __global__ __launch_bounds__(256, paged_workgroups(HD)) void paged_kernel(const 
             Wide<T, HD, CURVE>::run(a, it, kvh, lane, paged_lds_mem);
         at = it.next;
         if (at == 0) break;
-        __syncthreads();  // no one reads the item's LDS any more
+        wait_lgkmcnt0();
+        workgroup_barrier();  // no one reads the item's LDS any more
     }
 }
 
@@ -306,16 +307,18 @@ __global__ __launch_bounds__(256, paged_workgroups(HD)) void paged_kernel(const 
 // Rows of few tiles that end in many parts (a token over a long cache: 64). causal.hip's join has a group of HD / 4
 // lanes (64 at most) take a row's parts one after another, which then is the launch's time; here `split` groups of
 // the workgroup take a row's parts in turn and add up through LDS, in one order. 4 rows a KV head of 64 parts
-// (head dim 128, 8 KV heads): 9.7 us there, 4.1 here.
+// (head dim 128, 8 KV heads): 9.7 us there, 4.0 here. From head dim 256 on, where a wave is a group, rows of more than four
+// take 1024 threads; others, and smaller head dims, 256 (128 rows of 41 tiles in 3 parts at head dim 256: 8.7 us, with
+// 1024 10.0; 64 parts at head dim 128 4.0 and 4.4).
 template <int HD>
 constexpr int kJoinLanes = HD < 256 ? HD / 4 : 64;
 template <int HD>
-constexpr int kJoinThreads = HD < 256 ? 256 : 1024;
-template <int HD>
-constexpr int kJoinGroups = kJoinThreads<HD> / kJoinLanes<HD>;
-template <typename T, int HD>
-__global__ __launch_bounds__(kJoinThreads<HD>) void paged_join_kernel(const CausalArgs a, const CausalInline in, int split) {
-    constexpr int L = kJoinLanes<HD>, G = kJoinGroups<HD>, E = HD / (4 * L);  // lanes of a group, groups, 16-byte loads a lane of a row
+constexpr int kJoinGroups(int threads) {
+    return threads / kJoinLanes<HD>;
+}
+template <typename T, int HD, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_join_kernel(const CausalArgs a, const CausalInline in, int split) {
+    constexpr int L = kJoinLanes<HD>, G = kJoinGroups<HD>(THREADS), E = HD / (4 * L);  // lanes of a group, groups, 16-byte loads a lane of a row
     __shared__ float4_t lds_o[G][E][L];
     __shared__ float2 lds_ml[G];
     const int lane = int(threadIdx.x) & (L - 1), group = int(threadIdx.x) / L, turn = group & (split - 1);
@@ -387,13 +390,20 @@ __global__ __launch_bounds__(kJoinThreads<HD>) void paged_join_kernel(const Caus
             u32x2{T::pack(o[e][0] * inv, o[e][1] * inv), T::pack(o[e][2] * inv, o[e][3] * inv)};
 }
 
+template <typename T, int HD, int THREADS>
+hipError_t run_join_of(hipStream_t s, const CausalArgs& a, const CausalInline& in, int split) {
+    const int rows = kJoinGroups<HD>(THREADS) / split;
+    launch_kernel(paged_join_kernel<T, HD, THREADS>, dim3(uint32_t(a.n_joins) * uint32_t(a.kv_heads), uint32_t(a.join_rows + rows - 1) / uint32_t(rows)),
+                  dim3(THREADS), 0, s, a, in, split);
+    return hipGetLastError();
+}
+
 template <typename T, int HD>
 hipError_t run_join(hipStream_t s, const CausalArgs& a, const CausalInline& in, int split) {
-    split = split < kJoinGroups<HD> ? split : kJoinGroups<HD>;
-    const int rows = kJoinGroups<HD> / split;
-    launch_kernel(paged_join_kernel<T, HD>, dim3(uint32_t(a.n_joins) * uint32_t(a.kv_heads), uint32_t(a.join_rows + rows - 1) / uint32_t(rows)),
-                  dim3(kJoinThreads<HD>), 0, s, a, in, split);
-    return hipGetLastError();
+    constexpr int groups = kJoinGroups<HD>(256);
+    if constexpr (HD >= 256)
+        if (split > groups) return run_join_of<T, HD, 1024>(s, a, in, split);
+    return run_join_of<T, HD, 256>(s, a, in, split < groups ? split : groups);
 }
 
 template <typename T, int HD, typename CURVE, int KINDS>
