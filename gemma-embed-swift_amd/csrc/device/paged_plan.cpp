@@ -9,10 +9,10 @@
 //   shares: where most sequences are one tile (single tokens), workgroups take equal shares of all keys, tile after tile,
 //     and a share's border cuts a tile.
 // Rows that end in parts are joined by a second launch.
-// us of both launches, whole / parts / shares: 8192 tokens over 16192 keys (32 heads of 128 over 8) 1502 / - / 1630, 4 x 512
-// over 5500 to 9500 263 / - / 298, 5 x 301 to 700 over 2000 to 9700 (16 heads of 64 over 8) 132 / 101 / 108, 3 x 500 to 1500
-// over 1500 to 5500 with a window of 1024 (4 heads of 256 over 2) 61 / 42 / 57, 64 tokens over 100 to 8000 (32 heads of 128
-// over 8) 199 / - / 186. Finer shares gain nothing (2, 3 and 4 times as many: 190, 191 and 192).
+// us of both launches, whole / parts / shares: 8192 tokens over 16192 keys (32 heads of 128 over 8) 1515 / - / 1635, 4 x 512
+// over 5500 to 9500 275 / 294 / 324, 5 x 301 to 700 over 2000 to 9700 (16 heads of 64 over 8) 142 / 98 / 110, 3 x 500 to 1500
+// over 1500 to 5500 with a window of 1024 (4 heads of 256 over 2) 64 / 43 / 56, 64 tokens over 100 to 8000 (32 heads of 128
+// over 8) 200 / - / 186. Finer shares gain nothing (2, 3 and 4 times as many: 190, 191 and 192).
 #include "paged_plan.hpp"
 
 #include <algorithm>
