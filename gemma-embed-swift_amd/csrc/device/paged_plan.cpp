@@ -23,8 +23,10 @@ namespace {
 
 constexpr int kCus = 256;
 // Keys are counted in units of 64. What an item takes besides its keys (its queries, the first keys, its rows' way
-// out), the least keys of a part, and the longest tile that is not worth a second launch.
-constexpr int kUnit = 64, kItemUnits = 2, kLeastPart = 2, kWhole = 4;
+// out), the least keys of a part (a token over 512 keys, head dims 256 / 512, us a call: parts of one unit 22.0 / 25.8, of two
+// 23.9 / 30.0), and the longest tile that no estimate is made for (over 256 keys whole 22.7 / 31.0, in parts 21.2 / 25.0; over
+// 128 20.0 / 24.9 and 20.1 / 24.9).
+constexpr int kUnit = 64, kItemUnits = 2, kLeastPart = 1, kWhole = 2;
 // Tiles that a plan's estimate follows one by one; more are even enough.
 constexpr size_t kManyTiles = 1024;
 
