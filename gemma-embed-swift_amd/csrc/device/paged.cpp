@@ -132,9 +132,9 @@ void check_rotary(const ge_rotary_desc& d) {
 constexpr const char* kRotate = "rotate_heads";
 constexpr const char* kAppend = "paged_append";
 
-// The checks and arguments of both entries over rows of heads; whether everything is in 16-byte pieces, in *wide.
+// The checks and arguments of both entries over rows of heads, and the unit that shape and strides come in (rotary.hpp).
 HeadsArgs heads_args(const char* op, ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, bool append, ge_heads_shape* checked,
-                     bool* wide) {
+                     int* unit) {
     if (!shape) fail(GE_ERR_INVALID, "%s: null shape", op);
     ge_heads_shape s = *shape;
     if (s.type != GE_TYPE_F16 && s.type != GE_TYPE_BF16) fail(GE_ERR_INVALID, "%s: results of type %d (F16 or BF16)", op, s.type);
@@ -178,10 +178,13 @@ HeadsArgs heads_args(const char* op, ge_ctx* c, const ge_heads_shape* shape, con
         a.fade = r->fade;
         a.gain = r->gain;
     }
-    const int in8 = s.in_type == GE_TYPE_F32 ? 4 : 8;  // elements of 16 bytes
-    const bool strides = s.q_stride % in8 == 0 && s.k_stride % in8 == 0 && s.q_out_stride % 8 == 0 &&
-                         (append ? s.v_stride % in8 == 0 : s.k_out_stride % 8 == 0);
-    *wide = strides && s.head_dim % 16 == 0 && a.half % 8 == 0;
+    // (units of fp32 rows: 16 bytes at most; wave lanes: up to 64 units a half)
+    const auto rows_in = [&](int u) {
+        const int in = std::min(u, s.in_type == GE_TYPE_F32 ? 4 : 8);
+        return s.q_stride % in == 0 && s.k_stride % in == 0 && s.q_out_stride % u == 0 && (append ? s.v_stride % in == 0 : s.k_out_stride % u == 0);
+    };
+    *unit = 8;
+    while (*unit > 1 && !(s.head_dim % (2 * *unit) == 0 && s.head_dim <= 128 * *unit && a.half % *unit == 0 && rows_in(*unit))) *unit /= 2;
     *checked = s;
     return a;
 }
@@ -191,14 +194,15 @@ struct Operand {
     const char* name;
     const void* p;
     bool needed;
-    size_t size;  // of an element
+    int size;   // of an element
+    bool rows;  // read or written a unit at a time
 };
 
-void check_operands(const char* op, std::initializer_list<Operand> list, bool* wide) {
+void check_operands(const char* op, std::initializer_list<Operand> list, int* unit) {
     for (const Operand& o : list) {
         if (o.needed && !o.p) fail(GE_ERR_INVALID, "%s: null %s", op, o.name);
-        if (!aligned(o.p, o.size)) fail(GE_ERR_INVALID, "%s: %s is not aligned to its elements", op, o.name);
-        *wide = *wide && aligned(o.p, 16);
+        if (!aligned(o.p, size_t(o.size))) fail(GE_ERR_INVALID, "%s: %s is not aligned to its elements", op, o.name);
+        while (o.rows && *unit > 1 && !aligned(o.p, size_t(std::min(16, *unit * o.size)))) *unit /= 2;
     }
 }
 
@@ -212,12 +216,12 @@ void check_in_place(const char* op, const char* what, const ge_heads_shape& s, c
 void rotate(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const void* q, const void* k, const void* q_norm,
             const void* k_norm, const void* positions, void* q_out, void* k_out) {
     ge_heads_shape s;
-    bool wide = false;
-    HeadsArgs a = heads_args(kRotate, c, shape, r, false, &s, &wide);
+    int unit = 1;
+    HeadsArgs a = heads_args(kRotate, c, shape, r, false, &s, &unit);
     if (s.rows == 0) return;
-    const size_t in = s.in_type == GE_TYPE_F32 ? 4 : 2;
-    check_operands(kRotate, {{"q", q, s.heads > 0, in}, {"k", k, s.kv_heads > 0, in}, {"q_out", q_out, s.heads > 0, 2},
-                             {"k_out", k_out, s.kv_heads > 0, 2}, {"q_norm", q_norm, false, 4}, {"k_norm", k_norm, false, 4}}, &wide);
+    const int in = s.in_type == GE_TYPE_F32 ? 4 : 2;
+    check_operands(kRotate, {{"q", q, s.heads > 0, in, true}, {"k", k, s.kv_heads > 0, in, true}, {"q_out", q_out, s.heads > 0, 2, true},
+                             {"k_out", k_out, s.kv_heads > 0, 2, true}, {"q_norm", q_norm, false, 4, false}, {"k_norm", k_norm, false, 4, false}}, &unit);
     check_in_place(kRotate, "q", s, q, s.q_stride, q_out, s.q_out_stride);
     check_in_place(kRotate, "k", s, k, s.k_stride, k_out, s.k_out_stride);
     if (r && !positions) fail(GE_ERR_INVALID, "%s: null positions", kRotate);
@@ -230,7 +234,7 @@ void rotate(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const vo
     a.k_norm = static_cast<const float*>(k_norm);
     a.positions = static_cast<const int32_t*>(positions);
     a.rows_each = heads_rows_each(s.rows);
-    launch(c, kRotate, [&] { return launch_rotate_heads(c->stream, a, s.in_type == GE_TYPE_F32, s.type == GE_TYPE_BF16, wide); });
+    launch(c, kRotate, [&] { return launch_rotate_heads(c->stream, a, s.in_type == GE_TYPE_F32, s.type == GE_TYPE_BF16, unit); });
     hip_check(hipStreamSynchronize(c->stream), "hipStreamSynchronize");
 }
 
@@ -259,8 +263,8 @@ void append(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const vo
             const void* q_norm, const void* k_norm, const void* positions, const ge_page_table* t, const ge_paged_seq* seqs,
             int n_seqs, void* q_out, void* k_pages, void* v_pages) {
     ge_heads_shape s;
-    bool wide = false;
-    HeadsArgs a = heads_args(kAppend, c, shape, r, true, &s, &wide);
+    int unit = 1;
+    HeadsArgs a = heads_args(kAppend, c, shape, r, true, &s, &unit);
     check_table(kAppend, c, t);
     if (s.kv_heads == 0) fail(GE_ERR_INVALID, "%s: no KV heads", kAppend);
     if (n_seqs < 0) fail(GE_ERR_INVALID, "%s: %d sequences", kAppend, n_seqs);
@@ -277,10 +281,10 @@ void append(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const vo
             fail(GE_ERR_INVALID, "%s: sequence %d: slot %u lacks a page of keys [%u, %u)", kAppend, i, e.slot, e.kv_len - e.q_len, e.kv_len);
         rows += e.q_len;
     }
-    const size_t in = s.in_type == GE_TYPE_F32 ? 4 : 2;
-    check_operands(kAppend, {{"q", q, s.heads > 0, in}, {"k", k, true, in}, {"v", v, true, in}, {"q_out", q_out, s.heads > 0, 2},
-                             {"k_pages", k_pages, true, 2}, {"v_pages", v_pages, true, 2}, {"q_norm", q_norm, false, 4},
-                             {"k_norm", k_norm, false, 4}}, &wide);
+    const int in = s.in_type == GE_TYPE_F32 ? 4 : 2;
+    check_operands(kAppend, {{"q", q, s.heads > 0, in, true}, {"k", k, true, in, true}, {"v", v, true, in, true}, {"q_out", q_out, s.heads > 0, 2, true},
+                             {"k_pages", k_pages, true, 2, true}, {"v_pages", v_pages, true, 2, true}, {"q_norm", q_norm, false, 4, false},
+                             {"k_norm", k_norm, false, 4, false}}, &unit);
     check_in_place(kAppend, "q", s, q, s.q_stride, q_out, s.q_out_stride);
     if (!aligned(positions, 4)) fail(GE_ERR_INVALID, "%s: positions are not aligned to their elements", kAppend);
     claim_pages(t, seqs, n_seqs);
@@ -324,7 +328,7 @@ void append(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const vo
     a.slot_pages = t->slot_pages;
     a.page_shift = t->page_shift;
     a.page_stride = s.page_stride;
-    launch(c, kAppend, [&] { return launch_append(c->stream, a, few, s.in_type == GE_TYPE_F32, s.type == GE_TYPE_BF16, wide); });
+    launch(c, kAppend, [&] { return launch_append(c->stream, a, few, s.in_type == GE_TYPE_F32, s.type == GE_TYPE_BF16, unit); });
     hip_check(hipStreamSynchronize(c->stream), "hipStreamSynchronize");
 }
 

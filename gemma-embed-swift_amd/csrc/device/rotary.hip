@@ -30,19 +30,20 @@ struct StoredAs<F32> {
 };
 
 // The pieces of a head that a lane holds: N elements of `a` and as many of `b`, the pairs' two sides where
-// they turn.
-// Wide: one 16-byte-aligned unit of 8 + 8 elements a lane, head_dim / 16 lanes a head (a power of two of
-// lanes, so that several heads stand side by side in a wave). Narrow, for head dims, parts, strides and
-// addresses that are not in such pieces: single elements, the whole wave on a head.
-template <bool WIDE>
+// they turn. UNIT: elements that lie together.
+// 8, 4, 2: one unit of each a lane, loaded and stored whole, head_dim / (2 UNIT) lanes a head (a power of two of
+// lanes, so that several heads stand side by side in a wave). 1, for whatever does not come in larger ones: four of
+// each a lane, the whole wave on a head. 16384 rows of 32 + 8 heads of 128 of which 128, 72, 36 and 34 elements turn: 66, U4, U2
+// and 190 us.
+template <int UNIT>
 struct Shape {
-    static constexpr int N = WIDE ? 8 : 4;
+    static constexpr int N = UNIT == 1 ? 4 : UNIT, kUnits = N / UNIT;
 };
 
 // log2 of the lanes a head takes.
-template <bool WIDE>
+template <int UNIT>
 __device__ __forceinline__ int lanes_log(int head_dim) {
-    return WIDE ? (head_dim <= 16 ? 0 : 32 - __builtin_clz(uint32_t(head_dim / 16 - 1))) : 6;
+    return UNIT == 1 ? 6 : head_dim <= 2 * UNIT ? 0 : 32 - __builtin_clz(uint32_t(head_dim / (2 * UNIT) - 1));
 }
 
 // The sum over groups of 2^log lanes: halves of a group hold equal sums, so that a mirrored move is as
@@ -63,71 +64,90 @@ __device__ __forceinline__ float group_sum(float v, int log) {
     return v;
 }
 
-// Where a lane's elements lie in a head: a's first element and, `step` apart, its others (step 1 wide, 0
-// past the head's end); b likewise; the first pair, or -1 where they do not turn.
-template <bool WIDE>
+// Where a lane's units lie in a head: their first elements, -1 past the head's end (b likewise), and first pairs, -1
+// where they do not turn.
+template <int UNIT>
 struct Place {
-    static constexpr int N = Shape<WIDE>::N;
-    int a[WIDE ? 1 : N], b[WIDE ? 1 : N], pair[WIDE ? 1 : N];
-    bool any;  // wide: the lane has a unit; narrow: a unit has index < head_dim / 2
+    static constexpr int U = Shape<UNIT>::kUnits;
+    int a[U], b[U], pair[U];
+    bool any;  // a unit lies in the head
 
     __device__ __forceinline__ void init(const HeadsArgs& h, int lane_of_head) {
-        constexpr int E = WIDE ? 8 : 1;
         any = false;
 #pragma unroll
-        for (int j = 0; j < (WIDE ? 1 : N); j++) {
-            const int u = (lane_of_head + 64 * j) * E;  // the unit's first pair
+        for (int j = 0; j < U; j++) {
+            const int u = (lane_of_head + 64 * j) * UNIT;  // the unit's first pair
             const bool in = u < h.head_dim / 2, turns = u < h.half;
             any = any || in;
             pair[j] = in && turns ? u : -1;
             a[j] = !in ? -1 : turns && !h.pairs ? u : 2 * u;
-            b[j] = !in ? -1 : turns && !h.pairs ? h.half + u : 2 * u + E;
+            b[j] = !in ? -1 : turns && !h.pairs ? h.half + u : 2 * u + UNIT;
         }
     }
 };
 
-// A lane's elements of one head as they lie in memory, loaded ahead. (Vectors and single members: arrays that
-// are loaded under a condition went through scratch memory.)
-template <typename T, bool WIDE>
-struct Raw;
-template <typename T>
-struct Raw<T, true> {
-    u32x4 a{}, b{};
-    __device__ __forceinline__ void load(const uint16_t* p, const Place<true>& at) {
-        a = *reinterpret_cast<const u32x4*>(p + at.a[0]);
-        b = *reinterpret_cast<const u32x4*>(p + at.b[0]);
-    }
-    __device__ __forceinline__ void values(float (&x)[8], float (&y)[8]) const {
+// N elements as they lie in memory. (Vectors and single members: arrays that are loaded under a condition went
+// through scratch memory.)
+template <typename T, int N>
+struct Elements {
+    typedef uint32_t Words __attribute__((ext_vector_type(N / 2)));
+    Words w{};
+    __device__ __forceinline__ void load(const uint16_t* p) { w = *reinterpret_cast<const Words*>(p); }
+    __device__ __forceinline__ void values(float (&x)[N]) const {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            x[i] = T::value(uint16_t(a[i / 2] >> (16 * (i % 2))));
-            y[i] = T::value(uint16_t(b[i / 2] >> (16 * (i % 2))));
-        }
+        for (int i = 0; i < N; i++) x[i] = T::value(uint16_t(w[i / 2] >> (16 * (i % 2))));
+    }
+};
+template <typename T>
+struct Elements<T, 2> {
+    uint32_t w = 0;
+    __device__ __forceinline__ void load(const uint16_t* p) { w = *reinterpret_cast<const uint32_t*>(p); }
+    __device__ __forceinline__ void values(float (&x)[2]) const {
+        x[0] = T::value(uint16_t(w));
+        x[1] = T::value(uint16_t(w >> 16));
+    }
+};
+template <int N>
+struct Elements<F32, N> {
+    typedef float Words __attribute__((ext_vector_type(N < 4 ? N : 4)));
+    Words w{}, more{};  // more: of 8
+    __device__ __forceinline__ void load(const float* p) {
+        w = *reinterpret_cast<const Words*>(p);
+        if constexpr (N == 8) more = *reinterpret_cast<const Words*>(p + 4);
+    }
+    __device__ __forceinline__ void values(float (&x)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = i < 4 ? w[i] : more[i - 4];
     }
 };
 template <>
-struct Raw<F32, true> {
-    float4_t a0{}, a1{}, b0{}, b1{};
-    __device__ __forceinline__ void load(const float* p, const Place<true>& at) {
-        a0 = *reinterpret_cast<const float4_t*>(p + at.a[0]);
-        a1 = *reinterpret_cast<const float4_t*>(p + at.a[0] + 4);
-        b0 = *reinterpret_cast<const float4_t*>(p + at.b[0]);
-        b1 = *reinterpret_cast<const float4_t*>(p + at.b[0] + 4);
+struct Elements<F32, 2> {
+    typedef float Words __attribute__((ext_vector_type(2)));
+    Words w{};
+    __device__ __forceinline__ void load(const float* p) { w = *reinterpret_cast<const Words*>(p); }
+    __device__ __forceinline__ void values(float (&x)[2]) const {
+        x[0] = w[0];
+        x[1] = w[1];
     }
-    __device__ __forceinline__ void values(float (&x)[8], float (&y)[8]) const {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[i] = a0[i];
-            x[4 + i] = a1[i];
-            y[i] = b0[i];
-            y[4 + i] = b1[i];
-        }
+};
+
+// A lane's elements of one head, loaded ahead.
+template <typename T, int UNIT>
+struct Raw {
+    Elements<T, UNIT> a, b;
+    __device__ __forceinline__ void load(const typename StoredAs<T>::Type* p, const Place<UNIT>& at) {
+        a.load(p + at.a[0]);
+        b.load(p + at.b[0]);
+    }
+    __device__ __forceinline__ void values(float (&x)[UNIT], float (&y)[UNIT]) const {
+        a.values(x);
+        b.values(y);
     }
 };
 template <typename T>
-struct Raw<T, false> {
+struct Raw<T, 1> {
     float4_t a{}, b{};
-    __device__ __forceinline__ void load(const typename StoredAs<T>::Type* p, const Place<false>& at) {
+    __device__ __forceinline__ void load(const typename StoredAs<T>::Type* p, const Place<1>& at) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {  // a unit past the head's end takes the head's first element, and is not used
             a[j] = T::value(p[max(at.a[j], 0)]);
@@ -145,36 +165,36 @@ struct Raw<T, false> {
 };
 
 // A lane's weights, from the LDS row of its head's kind.
-template <bool WIDE>
-__device__ __forceinline__ void weigh(const float* w, const Place<WIDE>& at, float (&a)[Shape<WIDE>::N], float (&b)[Shape<WIDE>::N]) {
-    constexpr int N = Shape<WIDE>::N;
-    if constexpr (WIDE) {
+template <int UNIT>
+__device__ __forceinline__ void weigh(const float* w, const Place<UNIT>& at, float (&a)[Shape<UNIT>::N], float (&b)[Shape<UNIT>::N]) {
+    constexpr int V = UNIT < 4 ? UNIT : 4;
+    typedef float Vector __attribute__((ext_vector_type(V)));
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            const float4_t x = *reinterpret_cast<const float4_t*>(w + at.a[0] + i), y = *reinterpret_cast<const float4_t*>(w + at.b[0] + i);
+    for (int j = 0; j < Shape<UNIT>::N; j += V) {
+        const int unit = j / UNIT, within = j % UNIT;
+        const Vector x = *reinterpret_cast<const Vector*>(w + max(at.a[unit], 0) + within), y = *reinterpret_cast<const Vector*>(w + max(at.b[unit], 0) + within);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                a[i + j] *= x[j];
-                b[i + j] *= y[j];
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-            a[j] *= w[at.a[j] < 0 ? 0 : at.a[j]];
-            b[j] *= w[at.b[j] < 0 ? 0 : at.b[j]];
+        for (int i = 0; i < V; i++) {
+            a[j + i] *= x[i];
+            b[j + i] *= y[i];
         }
     }
 }
 
-template <typename O, bool WIDE>
-__device__ __forceinline__ void store(uint16_t* p, const Place<WIDE>& at, const float (&a)[Shape<WIDE>::N], const float (&b)[Shape<WIDE>::N]) {
-    if constexpr (WIDE) {
+template <typename O, int UNIT>
+__device__ __forceinline__ void store(uint16_t* p, const Place<UNIT>& at, const float (&a)[Shape<UNIT>::N], const float (&b)[Shape<UNIT>::N]) {
+    if constexpr (UNIT == 8) {
         *reinterpret_cast<u32x4*>(p + at.a[0]) = u32x4{O::pack(a[0], a[1]), O::pack(a[2], a[3]), O::pack(a[4], a[5]), O::pack(a[6], a[7])};
         *reinterpret_cast<u32x4*>(p + at.b[0]) = u32x4{O::pack(b[0], b[1]), O::pack(b[2], b[3]), O::pack(b[4], b[5]), O::pack(b[6], b[7])};
+    } else if constexpr (UNIT == 4) {
+        *reinterpret_cast<u32x2*>(p + at.a[0]) = u32x2{O::pack(a[0], a[1]), O::pack(a[2], a[3])};
+        *reinterpret_cast<u32x2*>(p + at.b[0]) = u32x2{O::pack(b[0], b[1]), O::pack(b[2], b[3])};
+    } else if constexpr (UNIT == 2) {
+        *reinterpret_cast<uint32_t*>(p + at.a[0]) = O::pack(a[0], a[1]);
+        *reinterpret_cast<uint32_t*>(p + at.b[0]) = O::pack(b[0], b[1]);
     } else {
 #pragma unroll
-        for (int j = 0; j < Shape<WIDE>::N; j++)
+        for (int j = 0; j < 4; j++)
             if (at.a[j] >= 0) {
                 p[at.a[j]] = uint16_t(O::pack(a[j], 0.0f));
                 p[at.b[j]] = uint16_t(O::pack(b[j], 0.0f));
@@ -225,31 +245,31 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) 
 // one 48 (at five workgroups 49, at six, which spill, 103); fp32: two at three workgroups 64 us, one at four 62 (5000
 // tokens of 5 heads of 256: 16.6 and 15.3). The norms' weights are in LDS, a row for each kind of head: in
 // registers, picked by each lane's kind, they took 10% of that time.
-template <typename I, typename O, bool WIDE, bool APPEND>
+template <typename I, typename O, int UNIT, bool APPEND>
 __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem& it) {
     typedef typename StoredAs<I>::Type Stored;
-    constexpr int N = Shape<WIDE>::N, kIts = 4 / int(sizeof(Stored)), kMaxDim = 512;
-    __shared__ float2 angles[WIDE ? 4 * kMaxDim / 2 : 1];
+    constexpr int N = Shape<UNIT>::N, kIts = 4 / int(sizeof(Stored)), kMaxDim = 512;
+    __shared__ float2 angles[UNIT > 1 ? 4 * kMaxDim / 2 : 1];
     __shared__ __attribute__((aligned(16))) float weights[3][kMaxDim];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-    const int log = lanes_log<WIDE>(h.head_dim), at_once = 64 >> log;
+    const int log = lanes_log<UNIT>(h.head_dim), at_once = 64 >> log;
     const int all = h.heads + (APPEND ? 2 : 1) * h.kv_heads;
     const int groups = (all + at_once - 1) / at_once, chunks = (groups + kIts - 1) / kIts;
-    Place<WIDE> at;
+    Place<UNIT> at;
     at.init(h, lane & ((1 << log) - 1));
     const float inv_dim = 1.0f / float(h.head_dim);
-    float2* const mine = angles + (WIDE ? wave * (kMaxDim / 2) : 0);
+    float2* const mine = angles + (UNIT > 1 ? wave * (kMaxDim / 2) : 0);
     // a head's kind: 0 q, 1 k, 2 v; its number among them
     auto kind_of = [&](int head) { return head < h.heads ? 0 : head < h.heads + h.kv_heads ? 1 : 2; };
     auto number_of = [&](int head, int kind) { return kind == 0 ? head : kind == 1 ? head - h.heads : head - h.heads - h.kv_heads; };
-    auto load = [&](Raw<I, WIDE>& raw, int r, int group) {
+    auto load = [&](Raw<I, UNIT>& raw, int r, int group) {
         const int head = group * at_once + (lane >> log), kind = kind_of(head);
         if (group < groups && head < all && at.any) {
             const void* const base = kind == 0 ? h.q : kind == 1 ? h.k : h.v;
             const int64_t stride = kind == 0 ? h.q_stride : kind == 1 ? h.k_stride : h.v_stride;
             raw.load(static_cast<const Stored*>(base) + (size_t(it.row0) + uint32_t(r)) * size_t(stride) + size_t(number_of(head, kind)) * size_t(h.head_dim), at);
         } else {
-            raw = Raw<I, WIDE>{};
+            raw = Raw<I, UNIT>{};
         }
     };
     // A wave's steps: chunks [chunk0, chunk1) of its rows r, r + stride, ..., each loaded a step ahead.
@@ -258,7 +278,7 @@ __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem&
     const int stride = split ? int(it.n) : 4;
     int r = split ? wave % int(it.n) : wave, chunk = chunk0;
     if (chunk >= chunks) r = int(it.n);
-    Raw<I, WIDE> raw[kIts];
+    Raw<I, UNIT> raw[kIts];
     if (r < int(it.n)) {
 #pragma unroll
         for (int i = 0; i < kIts; i++) load(raw[i], r, chunk * kIts + i);
@@ -290,7 +310,7 @@ __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem&
                     c *= h.fade;
                     s *= h.fade;
                 };
-                if constexpr (WIDE) {
+                if constexpr (UNIT > 1) {
                     for (int pair = lane; pair < h.half; pair += 64) {
                         float c, s;
                         turn(pair, c, s);
@@ -323,17 +343,17 @@ __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem&
             if (r_next < int(it.n)) load(raw[i], r_next, chunk_next * kIts + i);
             if (h.normed) {
                 norm(a, b, here && (h.normed >> kind & 1), log, inv_dim, h.eps);
-                if (here && at.any) weigh<WIDE>(weights[kind], at, a, b);
+                if (here && at.any) weigh<UNIT>(weights[kind], at, a, b);
             }
             if (!here || !at.any) continue;
             if (h.half && kind < 2) {
-                if constexpr (WIDE) {
+                if constexpr (UNIT > 1) {
                     if (at.pair[0] >= 0) {
-                        if (h.pairs) {  // neighbours: pairs i of a and 4 + i of b
+                        if (h.pairs) {  // neighbours: pairs i of a and N / 2 + i of b
 #pragma unroll
                             for (int j = 0; j < N; j += 2) {
                                 turn_pair(a[j], a[j + 1], cs[j / 2], sn[j / 2]);
-                                turn_pair(b[j], b[j + 1], cs[4 + j / 2], sn[4 + j / 2]);
+                                turn_pair(b[j], b[j + 1], cs[N / 2 + j / 2], sn[N / 2 + j / 2]);
                             }
                         } else {
 #pragma unroll
@@ -348,7 +368,7 @@ __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem&
                 if (h.gain != 1.0f) {
 #pragma unroll
                     for (int j = 0; j < N; j++)
-                        if (at.pair[WIDE ? 0 : j] >= 0) {
+                        if (at.pair[UNIT > 1 ? 0 : j] >= 0) {
                             a[j] *= h.gain;
                             b[j] *= h.gain;
                         }
@@ -362,21 +382,21 @@ __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem&
                 p = (kind == 1 ? h.k_out : h.v_out) + page_at + (number << h.page_shift) * size_t(h.head_dim);
             else
                 p = h.k_out + row * size_t(h.k_out_stride) + number * size_t(h.head_dim);
-            store<O, WIDE>(p, at, a, b);
+            store<O, UNIT>(p, at, a, b);
         }
         r = r_next;
         chunk = chunk_next;
     }
 }
 
-template <typename I, typename O, bool WIDE>
+template <typename I, typename O, int UNIT>
 __global__ __launch_bounds__(256, 4) void rotate_heads_kernel(const HeadsArgs h) {
     const int row0 = int(blockIdx.x) * h.rows_each;
     const AppendItem it{uint32_t(row0), uint32_t(min(h.rows_each, h.rows - row0)), 0, 0, 0};
-    heads_body<I, O, WIDE, false>(h, it);
+    heads_body<I, O, UNIT, false>(h, it);
 }
 
-template <typename I, typename O, bool WIDE>
+template <typename I, typename O, int UNIT>
 __global__ __launch_bounds__(256, 4) void append_kernel(const HeadsArgs h, const AppendInline in) {
     auto scalar = [](uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); };
     AppendItem it;
@@ -399,7 +419,7 @@ __global__ __launch_bounds__(256, 4) void append_kernel(const HeadsArgs h, const
         const uint32_t skip = (blockIdx.x - in.items[at].group0) * uint32_t(h.rows_each);
         it = AppendItem{in.items[at].row0 + skip, min(in.items[at].n - skip, uint32_t(h.rows_each)), in.items[at].slot, in.items[at].first + skip, blockIdx.x};
     }
-    heads_body<I, O, WIDE, true>(h, it);
+    heads_body<I, O, UNIT, true>(h, it);
 }
 
 __global__ __launch_bounds__(256) void table_set_kernel(int32_t* table, const uint2* entries, int n) {
@@ -412,40 +432,59 @@ bool heads_ok(const HeadsArgs& a) {
            a.half >= 0 && a.half <= a.head_dim / 2 && a.rows >= 0;
 }
 
-template <typename I, typename O>
-hipError_t run_rotate(hipStream_t s, const HeadsArgs& a, bool wide) {
-    const dim3 grid(uint32_t((int64_t(a.rows) + a.rows_each - 1) / a.rows_each));
-    if (wide)
-        launch_kernel(rotate_heads_kernel<I, O, true>, grid, dim3(256), 0, s, a);
-    else
-        launch_kernel(rotate_heads_kernel<I, O, false>, grid, dim3(256), 0, s, a);
+template <typename I, typename O, int UNIT>
+hipError_t run_rotate(hipStream_t s, const HeadsArgs& a) {
+    launch_kernel(rotate_heads_kernel<I, O, UNIT>, dim3(uint32_t((int64_t(a.rows) + a.rows_each - 1) / a.rows_each)), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
 template <typename I, typename O>
-hipError_t run_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool wide) {
-    if (wide)
-        launch_kernel(append_kernel<I, O, true>, dim3(uint32_t(a.workgroups)), dim3(256), 0, s, a, in);
-    else
-        launch_kernel(append_kernel<I, O, false>, dim3(uint32_t(a.workgroups)), dim3(256), 0, s, a, in);
+hipError_t run_rotate(hipStream_t s, const HeadsArgs& a, int unit) {
+    switch (unit) {
+        case 8: return run_rotate<I, O, 8>(s, a);
+        case 4: return run_rotate<I, O, 4>(s, a);
+        case 2: return run_rotate<I, O, 2>(s, a);
+        default: return run_rotate<I, O, 1>(s, a);
+    }
+}
+
+template <typename I, typename O, int UNIT>
+hipError_t run_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in) {
+    launch_kernel(append_kernel<I, O, UNIT>, dim3(uint32_t(a.workgroups)), dim3(256), 0, s, a, in);
     return hipGetLastError();
+}
+
+template <typename I, typename O>
+hipError_t run_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, int unit) {
+    switch (unit) {
+        case 8: return run_append<I, O, 8>(s, a, in);
+        case 4: return run_append<I, O, 4>(s, a, in);
+        case 2: return run_append<I, O, 2>(s, a, in);
+        default: return run_append<I, O, 1>(s, a, in);
+    }
+}
+
+// What the kernels assume of a unit.
+bool unit_ok(const HeadsArgs& a, int unit) {
+    return unit == 1 || ((unit == 2 || unit == 4 || unit == 8) && a.head_dim % (2 * unit) == 0 && a.head_dim <= 128 * unit && a.half % unit == 0);
 }
 
 }  // namespace
 
-hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, bool bf16, bool wide) {
-    if (!heads_ok(a) || a.rows_each <= 0 || (a.half && !a.positions)) return hipErrorInvalidValue;
+hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, bool bf16, int unit) {
+    if (!heads_ok(a) || !unit_ok(a, unit) || a.rows_each <= 0 || (a.half && !a.positions)) return hipErrorInvalidValue;
     if (a.rows == 0) return hipSuccess;
-    if (in_f32) return bf16 ? run_rotate<F32, BF16>(s, a, wide) : run_rotate<F32, F16>(s, a, wide);
-    return bf16 ? run_rotate<BF16, BF16>(s, a, wide) : run_rotate<F16, F16>(s, a, wide);
+    if (in_f32) return bf16 ? run_rotate<F32, BF16>(s, a, unit) : run_rotate<F32, F16>(s, a, unit);
+    return bf16 ? run_rotate<BF16, BF16>(s, a, unit) : run_rotate<F16, F16>(s, a, unit);
 }
 
-hipError_t launch_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool in_f32, bool bf16, bool wide) {
-    if (!heads_ok(a) || a.n_items < 0 || a.workgroups < a.n_items || a.rows_each <= 0 || (a.items ? a.workgroups != a.n_items : a.n_items > kAppendInlineItems))
+hipError_t launch_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool in_f32, bool bf16, int unit) {
+    if (!heads_ok(a) || !unit_ok(a, unit) || a.n_items < 0 || a.workgroups < a.n_items || a.rows_each <= 0 ||
+        (a.items ? a.workgroups != a.n_items : a.n_items > kAppendInlineItems))
         return hipErrorInvalidValue;
     if (a.n_items == 0) return hipSuccess;
-    if (in_f32) return bf16 ? run_append<F32, BF16>(s, a, in, wide) : run_append<F32, F16>(s, a, in, wide);
-    return bf16 ? run_append<BF16, BF16>(s, a, in, wide) : run_append<F16, F16>(s, a, in, wide);
+    if (in_f32) return bf16 ? run_append<F32, BF16>(s, a, in, unit) : run_append<F32, F16>(s, a, in, unit);
+    return bf16 ? run_append<BF16, BF16>(s, a, in, unit) : run_append<F16, F16>(s, a, in, unit);
 }
 
 hipError_t launch_table_set(hipStream_t s, int32_t* table, const uint2* entries, int n) {

@@ -46,9 +46,9 @@ static_assert(sizeof(HeadsArgs) + sizeof(AppendInline) <= 4096, "kernel argument
 // 73.5 and 83.0 us).
 inline int heads_rows_each(int rows) { return rows <= 1024 ? 1 : rows <= 4 * 4096 ? 4 : (rows / 4096 + 3) / 4 * 4; }
 
-// wide: everything is in whole 16-byte pieces (heads_wide).
-hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, bool bf16, bool wide);
-hipError_t launch_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool in_f32, bool bf16, bool wide);
+// unit: 8, 4, 2 or 1 elements, in which head_dim / 2, half, every stride and every address come (fp32 rows: 16 bytes at most).
+hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, bool bf16, int unit);
+hipError_t launch_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool in_f32, bool bf16, int unit);
 // Page numbers into a table: entries of (place in the table, page) pairs.
 hipError_t launch_table_set(hipStream_t s, int32_t* table, const uint2* entries, int n);
 

@@ -3,6 +3,7 @@ a call's launches are given. Run by tests/test_paged_host.py in a process of its
 library's objects over that runtime."""
 import ctypes as C
 import random
+import re
 
 import numpy as np
 import pytest
@@ -344,25 +345,37 @@ def test_handles_end_in_their_context(ctx):
     ctx.page_table_destroy(None)
 
 
-@pytest.mark.parametrize("shape,kw,wide", [
-    ({}, {}, True), (dict(head_dim=80), {}, True), (dict(in_type=F32), {}, True), (dict(q_stride=264), {}, True), (dict(q_stride=260), {}, False),
-    (dict(in_type=F32, q_stride=260), {}, True), (dict(in_type=F32, k_stride=130), {}, False), (dict(k_out_stride=132), {}, False),
-    (dict(head_dim=72), {}, False), (dict(head_dim=66), {}, False), ({}, dict(q=2), False), ({}, dict(k_out=8), False), ({}, dict(q_norm=4), False),
-    ({}, dict(positions=4), True)])
-def test_whole_pieces_or_not(ctx, memory, rotary, shape, kw, wide):
-    """The 16-byte form only where every address, stride and part allows it."""
+def unit_of(name):
+    return int(re.search(r"Li(\d)EEEv", name).group(1))
+
+
+@pytest.mark.parametrize("shape,kw,unit", [
+    ({}, {}, 8), (dict(head_dim=80), {}, 8), (dict(in_type=F32), {}, 8), (dict(q_stride=264), {}, 8), (dict(q_stride=260), {}, 4),
+    (dict(q_stride=258), {}, 2), (dict(q_stride=257), {}, 1), (dict(in_type=F32, q_stride=260), {}, 8), (dict(in_type=F32, k_stride=130), {}, 2),
+    (dict(in_type=F32, k_stride=129), {}, 1), (dict(k_out_stride=132), {}, 4), (dict(q_out_stride=262), {}, 2),
+    (dict(head_dim=72), {}, 4), (dict(head_dim=68), {}, 2), (dict(head_dim=66), {}, 1), (dict(head_dim=260), {}, 1), (dict(head_dim=264), {}, 4),
+    ({}, dict(q=2), 1), ({}, dict(q=4), 2), ({}, dict(k_out=8), 4), (dict(in_type=F32), dict(k=8), 2), (dict(in_type=F32), dict(k=4), 1),
+    (dict(in_type=F32), dict(k=16), 8), ({}, dict(q_norm=4), 8), ({}, dict(positions=4), 8)])
+def test_units(ctx, memory, rotary, shape, kw, unit):
+    """Elements move in the largest units that every address, stride and part allows."""
     with Launches() as got:
-        rotate(ctx, memory, rotary, shape, **{n: memory + x for n, x in kw.items()})
-    assert len(got.names) == 1 and ("Lb1E" in got.names[0]) == wide
+        rotate(ctx, memory, rotary, shape, **{n: memory + (4096 if n.endswith("out") else 0) + x for n, x in kw.items()})
+    assert len(got.names) == 1 and unit_of(got.names[0]) == unit
 
 
 def test_parts_of_a_head(ctx, memory):
-    for dims, wide in ((16, True), (48, True), (24, False), (2, False), (64, True)):
+    for dims, unit in ((16, 8), (48, 8), (24, 4), (20, 2), (36, 2), (2, 1), (34, 1), (64, 8)):
         h = ctx.rotary_create(dims, 1e4)
         with Launches() as got:
             rotate(ctx, memory, h)
-        assert ("Lb1E" in got.names[0]) == wide and got.args["half"] == dims // 2
+        assert unit_of(got.names[0]) == unit and got.args["half"] == dims // 2
         ctx.rotary_destroy(h)
+    h = ctx.rotary_create(4, 1e4)  # more units of 2 than lanes
+    for hd, unit in ((256, 2), (512, 1)):
+        with Launches() as got:
+            rotate(ctx, memory, h, dict(head_dim=hd))
+        assert unit_of(got.names[0]) == unit
+    ctx.rotary_destroy(h)
 
 
 def test_magnitudes(ctx, memory):

@@ -366,6 +366,13 @@ def test_appending(ctx, heads, kv_heads, hd, dims, in_type, type, page):
     append(ctx, SEQS, heads, kv_heads, hd, in_type, type, page, dims, fused=True, layout=1 if dims else 0, seed=page) if dims else None
 
 
+@pytest.mark.parametrize("in_type,type", [(F32, BF16), (F16, F16)])
+@pytest.mark.parametrize("hd,dims", [(72, 72), (40, 40), (40, 20), (128, 36), (64, 20), (12, 12), (8, 8), (4, 4), (264, 132), (512, 36)])
+def test_appending_in_units_of_four_and_two(ctx, hd, dims, in_type, type):
+    append(ctx, SEQS, 5, 2, hd, in_type, type, 8, dims, normed_heads=7, fused=True, seed=hd)
+    append(ctx, SEQS, 5, 2, hd, in_type, type, 32, dims, layout=1, seed=dims)
+
+
 @pytest.mark.parametrize("normed_heads", range(8))
 def test_norms_of_an_append(ctx, normed_heads):
     append(ctx, SEQS, 4, 2, 128, F32, BF16, dims=64, normed_heads=normed_heads, fused=True, seed=normed_heads)

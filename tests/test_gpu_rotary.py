@@ -124,6 +124,16 @@ def test_layouts(ctx, heads, kv_heads, hd, dims, layout, in_type, type):
     rotate(ctx, 1, heads, kv_heads, hd, in_type, type, dims, layout=layout, seed=hd)
 
 
+@pytest.mark.parametrize("in_type,type", [(F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("hd,dims,pad", [(72, 72, 0), (8, 8, 0), (40, 24, 0), (264, 264, 0), (504, 8, 0), (512, 512, 4), (64, 64, 4), (68, 68, 0), (4, 4, 0),
+                                         (12, 12, 0), (128, 36, 0), (256, 20, 0), (20, 0, 0), (256, 256, 2), (512, 36, 0), (36, 36, 1)])
+def test_units_of_four_and_two(ctx, hd, dims, pad, layout, in_type, type):
+    """Heads, parts and strides that come in fewer than 8 elements, some of more units than a wave has lanes."""
+    rotate(ctx, 9, 5, 2, hd, in_type, type, dims, normed_heads=3, layout=layout, pads=(pad,) * 4, seed=hd + dims)
+    rotate(ctx, 1500, 3, 1, hd, in_type, type, dims, layout=layout, pads=(pad,) * 4, seed=hd)
+
+
 @pytest.mark.parametrize("normed_heads", [0, 1, 2, 3])
 @pytest.mark.parametrize("weights", [True, False])
 @pytest.mark.parametrize("hd,dims", [(128, 0), (128, 64), (40, 40), (40, 0)])
