@@ -33,8 +33,8 @@ struct StoredAs<F32> {
 // they turn. UNIT: elements that lie together.
 // 8, 4, 2: one unit of each a lane, loaded and stored whole, head_dim / (2 UNIT) lanes a head (a power of two of
 // lanes, so that several heads stand side by side in a wave). 1, for whatever does not come in larger ones: four of
-// each a lane, the whole wave on a head. 16384 rows of 32 + 8 heads of 128 of which 128, 72, 36 and 34 elements turn: 66, U4, U2
-// and 190 us.
+// each a lane, the whole wave on a head. 16384 rows of 32 + 8 heads of 128 of which 128, 72, 36 and 34 elements turn: 66, 76, 110
+// and 185 us.
 template <int UNIT>
 struct Shape {
     static constexpr int N = UNIT == 1 ? 4 : UNIT, kUnits = N / UNIT;
@@ -243,12 +243,13 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) 
 // fewer rows than waves, a part of its heads, kIts groups of heads at a time, which with four workgroups a CU is what
 // the registers hold. 8192 tokens of 32 + 8 + 8 heads of 128 to append, 16-bit: four groups at half the waves 59 us, two 47,
 // one 48 (at five workgroups 49, at six, which spill, 103); fp32: two at three workgroups 64 us, one at four 62 (5000
-// tokens of 5 heads of 256: 16.6 and 15.3). The norms' weights are in LDS, a row for each kind of head: in
+// tokens of 5 heads of 256: 16.6 and 15.3). Smaller units have registers for more, which with few heads stay empty: four
+// groups of units of 4 16384 rows of 5 + 1 heads of 72 in 16.0 us, two in 13.6. The norms' weights are in LDS, a row for each kind of head: in
 // registers, picked by each lane's kind, they took 10% of that time.
 template <typename I, typename O, int UNIT, bool APPEND>
 __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem& it) {
     typedef typename StoredAs<I>::Type Stored;
-    constexpr int N = Shape<UNIT>::N, kIts = 4 / int(sizeof(Stored)), kMaxDim = 512;
+    constexpr int N = Shape<UNIT>::N, kIts = UNIT * sizeof(Stored) == 32 ? 1 : 2, kMaxDim = 512;
     __shared__ float2 angles[UNIT > 1 ? 4 * kMaxDim / 2 : 1];
     __shared__ __attribute__((aligned(16))) float weights[3][kMaxDim];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));

@@ -357,8 +357,8 @@ int ge_op_rotary_destroy(ge_ctx* ctx, ge_rotary* rotary);
  * of kv_heads x head_dim; a stride is the elements from one row to the next (0: rows back to back), so that
  * they may be views of one projection's output. Inputs are of in_type (GE_TYPE_F32 or the results' type), results of
  * type (GE_TYPE_F16 or GE_TYPE_BF16). Up to 4096 heads of each kind (0 for none, where an entry allows it), head_dim even
- * up to 512, rows under 2^30, strides up to 2^24. Buffers are aligned to their elements; the fast path needs
- * 16 bytes (addresses and strides), head_dim a multiple of 16 and dims one of 16.
+ * up to 512, rows under 2^30, strides up to 2^24. Buffers are aligned to their elements; rows move in units of 8, 4, 2 or
+ * 1 elements, the largest that head_dim / 2, dims / 2, strides and addresses come in (up to 16 bytes), larger ones faster.
  * normed: which heads are RMS-normed first, x / sqrt(mean x^2 + eps) * w over the head, w fp32 [head_dim] (null: 1);
  * value heads have no weight. All in fp32, rounded once. */
 enum { GE_NORM_Q = 1, GE_NORM_K = 2, GE_NORM_V = 4 };
@@ -372,8 +372,8 @@ typedef struct ge_heads_shape {
 } ge_heads_shape;
 
 /* q_out and k_out = the rows of q and k, normed (Q and K) and turned. positions: device int32 [rows], any values; rotary
- * (and then positions) nullable: not turned. q_out may be q and k_out k, of one type and stride; other overlaps are not
- * allowed. q and q_out may be null with no query heads, k and k_out with no KV heads. */
+ * (and then positions) nullable: not turned. q_out may be q and k_out k, of one type and stride (else refused); other
+ * overlaps are not allowed. q and q_out may be null with no query heads, k and k_out with no KV heads. */
 int ge_op_rotate_heads(ge_ctx* ctx, const ge_heads_shape* shape, const ge_rotary* rotary, const void* q, const void* k,
                        const void* q_norm, const void* k_norm, const void* positions, void* q_out, void* k_out);
 
