@@ -33,8 +33,8 @@ struct StoredAs<F32> {
 // they turn. UNIT: elements that lie together.
 // 8, 4, 2: one unit of each a lane, loaded and stored whole, head_dim / (2 UNIT) lanes a head (a power of two of
 // lanes, so that several heads stand side by side in a wave). 1, for whatever does not come in larger ones: four of
-// each a lane, the whole wave on a head. 16384 rows of 32 + 8 heads of 128 of which 128, 72, 36 and 34 elements turn: 66, 76, 110
-// and 185 us.
+// each a lane, head_dim / 8 lanes. 16384 rows of 32 + 8 heads of 128 of which 128, 72, 36 and 34 elements turn: 66, 76, 110
+// and 118 us (a whole wave to a head in units of 1: 185).
 template <int UNIT>
 struct Shape {
     static constexpr int N = UNIT == 1 ? 4 : UNIT, kUnits = N / UNIT;
@@ -43,7 +43,8 @@ struct Shape {
 // log2 of the lanes a head takes.
 template <int UNIT>
 __device__ __forceinline__ int lanes_log(int head_dim) {
-    return UNIT == 1 ? 6 : head_dim <= 2 * UNIT ? 0 : 32 - __builtin_clz(uint32_t(head_dim / (2 * UNIT) - 1));
+    const int lanes = (head_dim / 2 + Shape<UNIT>::N - 1) / Shape<UNIT>::N;
+    return lanes <= 1 ? 0 : 32 - __builtin_clz(uint32_t(lanes - 1));
 }
 
 // The sum over groups of 2^log lanes: halves of a group hold equal sums, so that a mirrored move is as
@@ -72,11 +73,11 @@ struct Place {
     int a[U], b[U], pair[U];
     bool any;  // a unit lies in the head
 
-    __device__ __forceinline__ void init(const HeadsArgs& h, int lane_of_head) {
+    __device__ __forceinline__ void init(const HeadsArgs& h, int lane_of_head, int lanes) {
         any = false;
 #pragma unroll
         for (int j = 0; j < U; j++) {
-            const int u = (lane_of_head + 64 * j) * UNIT;  // the unit's first pair
+            const int u = (lane_of_head + lanes * j) * UNIT;  // the unit's first pair
             const bool in = u < h.head_dim / 2, turns = u < h.half;
             any = any || in;
             pair[j] = in && turns ? u : -1;
@@ -257,7 +258,7 @@ __device__ __forceinline__ void heads_body(const HeadsArgs& h, const AppendItem&
     const int all = h.heads + (APPEND ? 2 : 1) * h.kv_heads;
     const int groups = (all + at_once - 1) / at_once, chunks = (groups + kIts - 1) / kIts;
     Place<UNIT> at;
-    at.init(h, lane & ((1 << log) - 1));
+    at.init(h, lane & ((1 << log) - 1), 1 << log);
     const float inv_dim = 1.0f / float(h.head_dim);
     float2* const mine = angles + (UNIT > 1 ? wave * (kMaxDim / 2) : 0);
     // a head's kind: 0 q, 1 k, 2 v; its number among them
