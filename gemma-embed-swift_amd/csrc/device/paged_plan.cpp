@@ -33,7 +33,7 @@ constexpr size_t kManyTiles = 1024;
 struct Tile {
     uint32_t seq, row0, n_rows;
     int32_t lo, hi;
-    int units() const { return (hi - lo + kUnit - 1) / kUnit; }
+    int units() const { return int((uint32_t(hi - lo) + kUnit - 1) / kUnit); }
 };
 
 // A sequence's tiles [first, first + n), the longest's units, and the parts they are cut into.
@@ -55,16 +55,35 @@ float items_us(int head_dim, bool narrow, float load, float longest) {
 // The joining launch, with its parts' rows written and read.
 float join_us(float rows, int kv_heads, int head_dim) { return 5.0f + rows * float(kv_heads) * float(head_dim) * 8 / 8e6f; }
 
-// The units on the CU that has most of them, the items taken longest first.
-int64_t heaviest(std::vector<int> items, int64_t cus) {
-    std::sort(items.begin(), items.end(), [](int a, int b) { return a > b; });
-    std::vector<int64_t> load(items.begin(), items.begin() + std::min<int64_t>(cus, int64_t(items.size())));
-    if (int64_t(items.size()) <= cus) return load.front();
+// Where each of `n` counts up to `most` comes when the largest are first, equal ones in order.
+template <typename COUNT>
+std::vector<uint32_t> largest_first(size_t n, int most, COUNT&& count) {
+    std::vector<uint32_t> order(n);
+    if (size_t(most) > 16 * n + 4096) {
+        for (size_t i = 0; i < n; i++) order[i] = uint32_t(i);
+        std::stable_sort(order.begin(), order.end(), [&](uint32_t a, uint32_t b) { return count(a) > count(b); });
+        return order;
+    }
+    std::vector<uint32_t> at(size_t(most) + 2, 0);  // of count c: where those of count most - c begin
+    for (size_t i = 0; i < n; i++) at[size_t(most - count(i)) + 1]++;
+    for (size_t c = 1; c < at.size(); c++) at[c] += at[c - 1];
+    for (size_t i = 0; i < n; i++) order[at[size_t(most - count(i))]++] = uint32_t(i);
+    return order;
+}
+
+// The units on the CU that has most of them, the tiles taken longest first. Of many a CU, their average and one more.
+int64_t heaviest(const std::vector<Tile>& tiles, int longest, int64_t total, int64_t cus) {
+    const size_t n = tiles.size();
+    if (n <= size_t(cus)) return longest + kItemUnits;
+    if (n > 8 * size_t(cus)) return std::max<int64_t>(longest + kItemUnits, total / cus + total / int64_t(n));
+    const std::vector<uint32_t> order = largest_first(n, longest, [&](size_t i) { return tiles[i].units(); });
+    std::vector<int64_t> load(static_cast<size_t>(cus));
+    for (size_t i = 0; i < size_t(cus); i++) load[i] = tiles[order[i]].units() + kItemUnits;
     const auto later = [](int64_t a, int64_t b) { return a > b; };
     std::make_heap(load.begin(), load.end(), later);
-    for (size_t i = size_t(cus); i < items.size(); i++) {
+    for (size_t i = size_t(cus); i < n; i++) {
         std::pop_heap(load.begin(), load.end(), later);
-        load.back() += items[i];
+        load.back() += tiles[order[i]].units() + kItemUnits;
         std::push_heap(load.begin(), load.end(), later);
     }
     return *std::max_element(load.begin(), load.end());
@@ -84,7 +103,7 @@ PagedItem item_of(const Tile& t, const ge_paged_seq& e, int64_t lo, int64_t hi, 
     return i;
 }
 
-int item_units(const PagedItem& i) { return int(i.k_hi - i.k_lo + kUnit - 1) / kUnit; }
+int item_units(const PagedItem& i) { return int((i.k_hi - i.k_lo + kUnit - 1) / kUnit); }
 
 void add_join(PagedPlan& p, const Tile& t, const ge_paged_seq& e, size_t first_part, uint32_t splits) {
     CausalJoin j{e.q_start, t.row0, t.n_rows, {}, {}, {}};
@@ -118,31 +137,45 @@ void plan_parts(PagedPlan& p, const std::vector<Group>& groups, const std::vecto
     // where each tile's parts begin among the partial rows, then the items part by part
     std::vector<uint32_t> part(tiles.size());
     std::vector<int> splits(tiles.size());
-    for (const Group& g : groups)
+    for (const Group& g : groups) {
+        const int step = g.step();
         for (uint32_t i = g.first; i < g.first + g.n; i++) {
             const Tile& t = tiles[i];
-            splits[i] = std::max(1, (t.units() + g.step() - 1) / g.step());
+            splits[i] = g.parts == 1 ? 1 : std::max(1, (t.units() + step - 1) / step);
             part[i] = uint32_t(p.part_rows);
             if (splits[i] == 1) continue;
             p.part_rows += size_t(splits[i]) * t.n_rows;
             add_join(p, t, seqs[t.seq], part[i], uint32_t(splits[i]));
         }
-    for (const Group& g : groups)
+    }
+    size_t n = 0;
+    for (const int x : splits) n += size_t(x);
+    std::vector<PagedItem> items;
+    items.reserve(n);
+    int longest = 0;
+    for (const Group& g : groups) {
+        const int64_t step = int64_t(g.step()) * kUnit;
         for (int s = 0; s < g.parts; s++)
             for (uint32_t i = g.first; i < g.first + g.n; i++) {
                 const Tile& t = tiles[i];
                 if (s >= splits[i]) continue;
-                const int64_t k = t.lo + int64_t(s) * g.step() * kUnit;
-                p.items.push_back(item_of(t, seqs[t.seq], k, std::min<int64_t>(t.hi, k + int64_t(g.step()) * kUnit),
-                                          splits[i] == 1 ? kDirect : part[i] + uint32_t(s) * t.n_rows));
+                const int64_t k = t.lo + s * step;
+                items.push_back(item_of(t, seqs[t.seq], k, std::min<int64_t>(t.hi, k + step), splits[i] == 1 ? kDirect : part[i] + uint32_t(s) * t.n_rows));
+                longest = std::max(longest, item_units(items.back()));
             }
-    std::stable_sort(p.items.begin(), p.items.end(), [](const PagedItem& a, const PagedItem& b) { return item_units(a) > item_units(b); });
+    }
+    p.items.reserve(n);
+    for (const uint32_t i : largest_first(n, longest, [&](size_t x) { return item_units(items[x]); })) p.items.push_back(items[i]);
     p.workgroups = p.items.size();
 }
 
 void plan_shares(PagedPlan& p, const std::vector<Tile>& tiles, const ge_paged_seq* seqs, int64_t total, int64_t shares) {
+    p.items.reserve(size_t(shares) + tiles.size());
+    p.joins.reserve(tiles.size());
     std::vector<PagedItem> rest;     // all but the workgroups' first items
     std::vector<size_t> rest_of;     // their workgroups
+    rest.reserve(tiles.size());
+    rest_of.reserve(tiles.size());
     int64_t left = total, room = 0;  // units not yet given out; of the current workgroup's share
     bool open = false;               // the current workgroup has an item
     auto begin = [&] {
@@ -213,8 +246,8 @@ PagedPlan plan_paged(const ge_paged_shape& s, const ge_paged_seq* seqs, int n_se
         for (int64_t r = 0; r < rows; r += wide) {
             const int64_t n = std::min<int64_t>(wide, rows - r);
             int64_t lo = 0;
-            if (s.window) lo = std::max<int64_t>(0, r / group + shift - s.window + 1) / kPagedAlign * kPagedAlign;
-            int64_t hi = std::min<int64_t>(e.kv_len, (r + n - 1) / group + shift + 1);
+            if (s.window) lo = std::max<int64_t>(0, uint32_t(r) / uint32_t(group) + shift - s.window + 1) / kPagedAlign * kPagedAlign;
+            int64_t hi = std::min<int64_t>(e.kv_len, uint32_t(r + n - 1) / uint32_t(group) + shift + 1);
             if (hi <= lo) lo = hi = 0;
             tiles.push_back(Tile{uint32_t(q), uint32_t(r), uint32_t(n), int32_t(lo), int32_t(hi)});
             const int units = tiles.back().units();
@@ -236,12 +269,10 @@ PagedPlan plan_paged(const ge_paged_shape& s, const ge_paged_seq* seqs, int n_se
     auto joined = [&](int64_t parts) { return join_us(float(parts) * row_avg, s.kv_heads, s.head_dim); };
     int64_t shares = 0, most = 0;  // the way taken: whole where both are 0
     if (longest > kWhole && tiles.size() < std::max(kManyTiles, size_t(at_once))) {
-        std::vector<int> units(tiles.size());
-        for (size_t i = 0; i < units.size(); i++) units[i] = tiles[i].units() + kItemUnits;
         // Estimates are off by what they leave out: whole single tiles of different lengths leave the memory to the few
         // longest at the end, 10%; shares of wide tiles, over different keys at a time, miss the L2, 15%.
         const bool single = 2 * groups.size() > tiles.size();
-        float best = us(float(heaviest(std::move(units), cus)), float(longest + kItemUnits)) * (single ? 1.1f : 1.0f);
+        float best = us(float(heaviest(tiles, longest, total, cus)), float(longest + kItemUnits)) * (single ? 1.1f : 1.0f);
         const int64_t n = std::min(at_once, (total - n_tiles * kItemUnits) / kLeastPart);
         if (n > 1) {
             const float share = float(total) / float(n) + kItemUnits;
