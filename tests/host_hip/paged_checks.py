@@ -565,6 +565,33 @@ def test_the_plan_covers_every_key_once(ctx, memory, heads, kv_heads, hd, window
     ctx.page_table_destroy(h)
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd", [(2, 1, 64), (1024, 1024, 64), (4, 1, 512)])
+@pytest.mark.parametrize("window", [0, 300000])
+def test_the_plan_of_long_caches(ctx, memory, heads, kv_heads, hd, window):
+    h = ctx.page_table_create(3, 600, 1024, 600)
+    ctx.page_table_set(h, [(s, i, i) for s in range(3) for i in range(600)])
+    for seqs in ([(0, 1, 0, 614400)], [(0, 2, 0, 600001), (2, 1, 1, 100), (3, 1, 2, 345678)]):
+        got = attend(ctx, memory, h, seqs, heads, kv_heads, hd, window=window)
+        covered(got, seqs, heads, kv_heads, hd, window)
+        if kv_heads > 1000:  # whole tiles, the longest first
+            units = [-(-(i.k_hi - i.k_lo) // 64) for i in got.items]
+            assert units == sorted(units, reverse=True) and not got.joins
+    ctx.page_table_destroy(h)
+
+
+@pytest.mark.parametrize("n", [33, 300, 1500])
+def test_the_longest_tiles_come_first(ctx, memory, n):
+    """Items of one kind of workgroup each, sorted; equal ones in the sequences' order."""
+    h = ctx.page_table_create(n, 4, 64, 4)
+    ctx.page_table_set(h, [(s, i, i) for s in range(n) for i in range(4)])
+    seqs = [(i, 1, i, 1 + 7 * i % 128) for i in range(n)]
+    got = attend(ctx, memory, h, seqs, q_rows=n)
+    covered(got, seqs, 4, 2, 64, 0)
+    order = [(-(-(i.k_hi - i.k_lo) // 64), i.slot) for i in got.items]
+    assert order == sorted(order, key=lambda x: (-x[0], x[1])) and not got.joins
+    ctx.page_table_destroy(h)
+
+
 def test_caps(ctx, memory, table):
     seqs = [(0, 1, 0, 50)]
     a = attend(ctx, memory, table, seqs, scale=-0.5).args
