@@ -9,10 +9,10 @@
 //   shares: where most sequences are one tile (single tokens), workgroups take equal shares of all keys, tile after tile,
 //     and a share's border cuts a tile.
 // Rows that end in parts are joined by a second launch.
-// us of both launches, whole / parts / shares: 8192 tokens over 16192 keys (32 heads of 128 over 8) 1515 / - / 1635, 4 x 512
-// over 5500 to 9500 275 / 294 / 324, 5 x 301 to 700 over 2000 to 9700 (16 heads of 64 over 8) 142 / 98 / 110, 3 x 500 to 1500
-// over 1500 to 5500 with a window of 1024 (4 heads of 256 over 2) 64 / 43 / 56, 64 tokens over 100 to 8000 (32 heads of 128
-// over 8) 200 / - / 186. Finer shares gain nothing (2, 3 and 4 times as many: 190, 191 and 192).
+// us of both launches, whole / parts / shares: 8192 tokens over 16192 keys (32 heads of 128 over 8) 1515 / - / 1650, 4 x 512
+// over 5500 to 9500 275 / 302 / 334, 5 x 301 to 700 over 2000 to 9700 (16 heads of 64 over 8) 139 / 96 / 102, 3 x 500 to 1500
+// over 1500 to 5500 with a window of 1024 (4 heads of 256 over 2) 63 / 42 / 49, 64 tokens over 100 to 8000 (32 heads of 128
+// over 8) 199 / - / 187. Finer shares gain nothing (2, 3 and 4 times as many: 190, 191 and 192).
 #include "paged_plan.hpp"
 
 #include <algorithm>
@@ -176,7 +176,8 @@ void plan_shares(PagedPlan& p, const std::vector<Tile>& tiles, const ge_paged_se
     std::vector<size_t> rest_of;     // their workgroups
     rest.reserve(tiles.size());
     rest_of.reserve(tiles.size());
-    int64_t left = total, room = 0;  // units not yet given out; of the current workgroup's share
+    // units not yet given out, an item more for each border; of the current workgroup's share
+    int64_t left = total + (shares - 1) * kItemUnits, room = 0;
     bool open = false;               // the current workgroup has an item
     auto begin = [&] {
         const int64_t groups = shares - int64_t(p.workgroups);
@@ -210,10 +211,9 @@ void plan_shares(PagedPlan& p, const std::vector<Tile>& tiles, const ge_paged_se
                 open = true;
             }
             room -= take + kItemUnits;
-            left -= take;
+            left -= take + kItemUnits;
             k = end;
         }
-        left -= kItemUnits;
         if (splits) add_join(p, t, e, first_part, splits);
     }
     // the chains: from a workgroup's first item to its others, in order
@@ -273,7 +273,9 @@ PagedPlan plan_paged(const ge_paged_shape& s, const ge_paged_seq* seqs, int n_se
         // longest at the end, 10%; shares of wide tiles, over different keys at a time, miss the L2, 15%.
         const bool single = 2 * groups.size() > tiles.size();
         float best = us(float(heaviest(tiles, longest, total, cus)), float(longest + kItemUnits)) * (single ? 1.1f : 1.0f);
-        const int64_t n = std::min(at_once, (total - n_tiles * kItemUnits) / kLeastPart);
+        // (a row of more than 128 parts waits for its join: a token over 30000 keys, head dim 256, in 469, 235 and 118 parts 10.7 + 11.2,
+        // 11.0 + 7.4 and 13.4 + 5.4 us, head dim 128 9.3 + 12.3, 8.8 + 8.0 and 9.7 + 5.6)
+        const int64_t n = std::min(at_once, (total - n_tiles * kItemUnits) / std::max(kLeastPart, longest / 128));
         if (n > 1) {
             const float share = float(total) / float(n) + kItemUnits;
             const float t = us(float((n + cus - 1) / cus) * share, share) * (single ? 1.0f : 1.15f) + joined(n + std::min(n, n_tiles));
