@@ -81,10 +81,11 @@ struct Straight {
 };
 
 // 32 rows of one KV head: queries in registers, accumulators, running maximum and sum. DW waves can hold
-// the same rows: they all compute the scores and each takes its share of the head's dims in the product.
-template <typename T, int HD, int DW>
+// the same rows: they all compute the scores, or each its share's sums of them (QW = DW), which they then add up
+// (Block::join), and each takes its share of the head's dims in the product.
+template <typename T, int HD, int DW, int QW = 1>
 struct Rows {
-    static constexpr int KS = HD / 16, DT = HD / 32 / DW;
+    static constexpr int KS = HD / 16 / QW, DT = HD / 32 / DW;
     u32x4 q[KS];
     float16_t o[DT];
     float m, l;
@@ -97,7 +98,7 @@ struct Rows {
     __device__ __forceinline__ void init(const CausalArgs& a, const CausalItem& it, int kvh, int r0, int n, int dims, int lane) {
         const uint32_t r = uint32_t(r0) + uint32_t(min(lane & 31, n - 1)), g = uint32_t(a.group);
         const uint32_t i = r / g, head = uint32_t(kvh) * g + r % g;
-        const uint16_t* p = a.q + (size_t(it.q_token) + i) * size_t(a.q_stride) + size_t(head) * HD + (lane >> 5) * 8;
+        const uint16_t* p = a.q + (size_t(it.q_token) + i) * size_t(a.q_stride) + size_t(head) * HD + (QW > 1 ? dims * (HD / QW) : 0) + (lane >> 5) * 8;
 #pragma unroll
         for (int s = 0; s < KS; s++) q[s] = *reinterpret_cast<const u32x4*>(p + s * 16) ^ a.q_flip;
 #pragma unroll
@@ -125,7 +126,7 @@ struct Rows {
             const int key = lane & 31, f = (key >> 1) & 7;
             const unsigned char* at[4];
 #pragma unroll
-            for (int c = 0; c < 4; c++) at[c] = K + key * 128 + (((2 * c + (lane >> 5)) ^ f) * 16);
+            for (int c = 0; c < 4; c++) at[c] = K + (QW > 1 ? w.d0 / 2 * (BK * 128) : 0) + key * 128 + (((2 * c + (lane >> 5)) ^ f) * 16);
             // fragments read kAhead steps before their product; the barriers keep the scheduler from
             // reading all of them first, which spills
             u32x4 ring[kAhead];
@@ -143,6 +144,26 @@ struct Rows {
                 s[t] = T::mfma(ring[i % kAhead], w.q[k], s[t]);
                 if (i + kAhead < KT * KS) read(i + kAhead);
             }
+        }
+
+        // The shares' sums, through 1024 KT floats of LDS a wave: `mine` and the other wave's of a pair.
+        __device__ __forceinline__ void join(unsigned char* mine, const unsigned char* other, int lane) {
+            static_assert(QW == 1 || QW == 2, "pairs");
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<float4_t*>(mine + (t * 4 + e / 4) * 1024 + lane * 16) = float4_t{s[t][e], s[t][e + 1], s[t][e + 2], s[t][e + 3]};
+            wait_lgkmcnt0();
+            workgroup_barrier();
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float4_t x = *reinterpret_cast<const float4_t*>(other + (t * 4 + e / 4) * 1024 + lane * 16);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[t][e + i] += x[i];
+                }
         }
 
         __device__ __forceinline__ bool sees_all(const Rows& w, int kb, int end) const {

@@ -92,34 +92,36 @@ struct Wide {
     static_assert(NW / DW * 32 == paged_wide_rows(HD), "rows of a wide item");
     static_assert(NG >= 1 && NW % 2 == 0, "every wave copies groups of one key parity");
     using Kv = KvBlock<HD, BK>;
-    static constexpr int kLds = 2 * 2 * Kv::kBytes;
+    using W = Rows<T, HD, DW, DW>;
+    static constexpr int kBlocks = 2 * 2 * Kv::kBytes, kShares = DW > 1 ? BK * 128 : 0;  // a wave's, of the scores
+    static constexpr int kLds = kBlocks + NW * kShares;
 
     static __device__ __forceinline__ void run(const PagedArgs& a, const CausalItem& it, int kvh, int lane, unsigned char* lds) {
         const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
         const uint32_t k_off = Kv::k_lane(lane, wave & 1, HD * 2), v_off = Kv::v_lane(lane, HD * 2);
         const PagedSpan<BK> span(a, it);
         const int blocks = span.blocks;
-        // The pages of 64 groups of 8 keys (kBlocks blocks) at a time, a lane a group, read when the ones before them are
+        // The pages of 64 groups of 8 keys (kAhead blocks) at a time, a lane a group, read when the ones before them are
         // taken. (As scalar loads in every block they cost registers across its branches: at head dim 256 150 spilled.)
-        constexpr int kBlocks = 64 * 8 / BK;
+        constexpr int kAhead = 64 * 8 / BK;
         int ids = 0, ids_next = span.group_page(lane);
         auto issue = [&](int b) {
             unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
-            if (b % kBlocks == 0) {
+            if (b % kAhead == 0) {
                 ids = ids_next;
-                ids_next = span.group_page((b + kBlocks) * (BK / 8) + lane);
+                ids_next = span.group_page((b + kAhead) * (BK / 8) + lane);
             }
 #pragma unroll
             for (int i = 0; i < NG; i++) {
                 const int k8 = wave + i * NW, key = span.first(b) + k8 * 8;
-                const int page = __builtin_amdgcn_readlane(ids, b % kBlocks * (BK / 8) + k8);
+                const int page = __builtin_amdgcn_readlane(ids, b % kAhead * (BK / 8) + k8);
                 copy_group<HD, BK, HD / 64>(span.template rows<HD>(a.k, page, key, kvh), at, k8, k_off);
                 copy_group<HD, BK, HD / 64>(span.template rows<HD>(a.v, page, key, kvh), at + Kv::kBytes, k8, v_off);
             }
         };
         // a wave with no rows repeats the item's last
         const int row = wave / DW * 32, n = min(32, int(it.n_rows) - row), r0 = int(it.row0) + row;
-        Rows<T, HD, DW> w;
+        W w;
         HeldBack<T, HD> held;
         held.init(a, it);
         if (blocks > 0) issue(0);
@@ -152,22 +154,28 @@ struct Wide {
         const int first = min(max((w.lo_any - span.lo) / BK, 0), blocks);
         const int end = n <= 0 || w.hi_any < span.lo ? first : max(first, min(blocks, (w.hi_any - span.lo) / BK + 1));
         int b = 0;
-        for (; b < first; b++) turn(b);
+        auto pass = [&](int b) {
+            turn(b);
+            if constexpr (DW > 1) workgroup_barrier();  // the other pair's, in join
+        };
+        unsigned char* const shares = lds + kBlocks;
+        for (; b < first; b++) pass(b);
         for (; b < end; b++) {
             turn(b);
             fall(b);
             unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
-            typename Rows<T, HD, DW>::template Block<BK> blk;
+            typename W::template Block<BK> blk;
             u32x4 p[BK / 16];
             blk.scores(w, at, lane);
+            if constexpr (DW > 1) blk.join(shares + wave * kShares, shares + (wave ^ 1) * kShares, lane);
             blk.softmax(w, span.first(b), span.end(b), a.c, lane, p, curve);
             blk.product(w, at + Kv::kBytes, lane, p);
         }
-        for (; b < blocks; b++) turn(b);
+        for (; b < blocks; b++) pass(b);
         // No one reads K and V any more. (With its barriers after the rows' stores a wave waited 1.7 us for those to arrive.)
         held.share(lds);
         if (n > 0) {
-            constexpr int kSlice = kLds / NW;
+            constexpr int kSlice = kBlocks / NW;
             w.l = sum_over_halves(w.l);
             w.template finish_rows<kSlice>(a, it, kvh, r0, n, lane, lds + wave * kSlice);
         }
