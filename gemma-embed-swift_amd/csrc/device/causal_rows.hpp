@@ -49,6 +49,10 @@ struct KvBlock {
     // Chunk (PANEL, k8) of a block whose rows start at r's base; off: the lane's offset of row 8 k8. Rows past
     // r's size read as zeros. The panel goes into the instruction's offset, which moves the LDS address as well
     // as the source's, so that a wave's chunks of a row group share one offset register.
+    static __device__ __forceinline__ void copy(__amdgpu_buffer_rsrc_t r, unsigned char* block, int k8, uint32_t off, int panel) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            r, (__attribute__((address_space(3))) void*)(block + (panel * (BK / 8) + k8) * 1024), 16, off, panel * 128, 0, 0);
+    }
     template <int PANEL>
     static __device__ __forceinline__ void copy(__amdgpu_buffer_rsrc_t r, unsigned char* block, int k8, uint32_t off) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -74,6 +78,11 @@ struct KvBlock {
 // Fragments read ahead of their products (four spill at head dim 256).
 template <int HD>
 constexpr int kFragmentsAhead = HD == 256 ? 3 : 4;
+
+// What is done between a score's products: nothing.
+struct Nothing {
+    __device__ __forceinline__ void operator()(int, int) const {}
+};
 
 // What becomes of a score besides its factor: nothing.
 struct Straight {
@@ -122,7 +131,9 @@ struct Rows {
         static constexpr int KT = BK / 32, kAhead = kFragmentsAhead<HD>;
         float16_t s[KT];
 
-        __device__ __forceinline__ void scores(const Rows& w, const unsigned char* K, int lane) {
+        // between(step, steps) stands before each step's product.
+        template <typename BETWEEN = Nothing>
+        __device__ __forceinline__ void scores(const Rows& w, const unsigned char* K, int lane, const BETWEEN& between = {}) {
             const int key = lane & 31, f = (key >> 1) & 7;
             const unsigned char* at[4];
 #pragma unroll
@@ -141,6 +152,7 @@ struct Rows {
                 const int t = i / KS, k = i % KS;
                 if (k == 0) s[t] = float16_t{};
                 __builtin_amdgcn_sched_barrier(0);
+                between(i, KT * KS);
                 s[t] = T::mfma(ring[i % kAhead], w.q[k], s[t]);
                 if (i + kAhead < KT * KS) read(i + kAhead);
             }

@@ -9,11 +9,12 @@
 // as long as its keys, and rows past the sequence's end read as zeros. Page numbers are read into scalar registers.
 //
 // What bounds it, of 1.3 PFLOP/s (a large product) and 7.0 TB/s (reads of one run; 5.9 of 4 KB pieces in no order): long prompts
-// at head dim 128 the card's power, the matrix pipe 56% busy at 1.66 GHz (8192 tokens over 16192 keys, 32 heads over 8: 1465
-// to 1515 us, 1.07 to 1.11 PFLOP/s); at head dim 64 the exponentials (16 heads over 8: 465 us, 0.87 PFLOP/s). Tokens the reads
-// (64 over 100 to 8000 keys, pages of 16: 182 us, 5.5 TB/s). Chunks the few items a CU and the parts they leave (5 x 301 to 700
-// over 2000 to 9700, 16 heads of 64 over 8: 88 and 9 us, 0.65 PFLOP/s; 3 x 500 to 1500, window 1024, 4 capped heads of 256 over
-// 2: 35 and 9 us, of which 15 are keys and 12 the way in and out).
+// at head dim 128 the card's power, the matrix pipe 56% busy at 1.66 GHz (8192 tokens over 16192 keys, 32 heads over 8: 1445
+// to 1605 us on several cards, 1.01 to 1.12 PFLOP/s); at head dim 64 the exponentials (16 heads over 8: 445 to 520 us, 0.78 to
+// 0.91 PFLOP/s); at 512 a workgroup's 64 rows, half of what its reads of LDS could feed (4 heads: 1340 to 1435 us, 0.57 to 0.61).
+// Tokens the reads (64 over 100 to 8000 keys, pages of 16: 182 us, 5.5 TB/s). Chunks the few items a CU and the parts they leave
+// (5 x 301 to 700 over 2000 to 9700, 16 heads of 64 over 8: 87 and 9 us, 0.65 PFLOP/s; 3 x 500 to 1500, window 1024, 4 capped
+// heads of 256 over 2: 34 and 8 us, of which 15 are keys and 12 the way in and out).
 #include "causal_rows.hpp"
 #include "paged.hpp"
 
@@ -105,8 +106,8 @@ struct Wide {
         // taken. (As scalar loads in every block they cost registers across its branches: at head dim 256 150 spilled.)
         constexpr int kAhead = 64 * 8 / BK;
         int ids = 0, ids_next = span.group_page(lane);
-        auto issue = [&](int b) {
-            unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
+        __amdgpu_buffer_rsrc_t rk[NG], rv[NG];
+        auto prepare = [&](int b) {
             if (b % kAhead == 0) {
                 ids = ids_next;
                 ids_next = span.group_page((b + kAhead) * (BK / 8) + lane);
@@ -115,10 +116,23 @@ struct Wide {
             for (int i = 0; i < NG; i++) {
                 const int k8 = wave + i * NW, key = span.first(b) + k8 * 8;
                 const int page = __builtin_amdgcn_readlane(ids, b % kAhead * (BK / 8) + k8);
-                copy_group<HD, BK, HD / 64>(span.template rows<HD>(a.k, page, key, kvh), at, k8, k_off);
-                copy_group<HD, BK, HD / 64>(span.template rows<HD>(a.v, page, key, kvh), at + Kv::kBytes, k8, v_off);
+                rk[i] = span.template rows<HD>(a.k, page, key, kvh);
+                rv[i] = span.template rows<HD>(a.v, page, key, kvh);
             }
         };
+        auto issue = [&](int b) {
+            unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
+            prepare(b);
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                copy_group<HD, BK, HD / 64>(rk[i], at, wave + i * NW, k_off);
+                copy_group<HD, BK, HD / 64>(rv[i], at + Kv::kBytes, wave + i * NW, v_off);
+            }
+        };
+        // Issued together, a block's copies keep its products waiting (16 a wave at head dim 512); from head dim 128 on they
+        // stand between the products of the block before: 8192 tokens over 16192 keys 1435 us instead of 1520 (4 heads of 512),
+        // 466 and 475 (4 of 256 over 2), 1605 and 1614 (32 of 128 over 8), and at 64, with four workgroups a CU, 518 and 516.
+        constexpr bool kBetween = HD >= 128;
         // a wave with no rows repeats the item's last
         const int row = wave / DW * 32, n = min(32, int(it.n_rows) - row), r0 = int(it.row0) + row;
         W w;
@@ -128,7 +142,7 @@ struct Wide {
         w.init(a, it, kvh, n > 0 ? r0 : int(it.row0 + it.n_rows) - 1, max(n, 1), wave % DW, lane);
         const CURVE curve{a.cap_z, a.cap_top};
         // Block b has landed everywhere, block b - 1 has been read, and the next one's copies start.
-        auto turn = [&](int b) {
+        auto turn = [&](int b, bool copies) {
             wait_vmcnt<0>();
             if (held.mixed(span.first(b), BK)) {
 #pragma unroll
@@ -137,7 +151,10 @@ struct Wide {
             }
             wait_lgkmcnt0();
             workgroup_barrier();
-            if (b + 1 < blocks) issue(b + 1);
+            if (!copies)
+                prepare(b + 1);
+            else if (b + 1 < blocks)
+                issue(b + 1);
         };
         // The blocks of which the wave's rows see a key, in a loop of their own: accumulators that only some turns
         // change cost registers at every join.
@@ -155,18 +172,26 @@ struct Wide {
         const int end = n <= 0 || w.hi_any < span.lo ? first : max(first, min(blocks, (w.hi_any - span.lo) / BK + 1));
         int b = 0;
         auto pass = [&](int b) {
-            turn(b);
+            turn(b, true);
             if constexpr (DW > 1) workgroup_barrier();  // the other pair's, in join
         };
         unsigned char* const shares = lds + kBlocks;
         for (; b < first; b++) pass(b);
         for (; b < end; b++) {
-            turn(b);
+            turn(b, !kBetween);
             fall(b);
+            // the next block's copies, one at a time between this one's products (past the last block of no bytes)
+            unsigned char* const next = lds + ((b + 1) & 1) * 2 * Kv::kBytes;
+            auto between = [&](int step, int steps) {
+                constexpr int P = HD / 64, C = NG * 2 * P;
+                if (!kBetween || step % (steps / C)) return;
+                const int c = step / (steps / C), i = c / (2 * P), v = c / P % 2, panel = c % P;
+                Kv::copy(v ? rv[i] : rk[i], next + v * Kv::kBytes, wave + i * NW, v ? v_off : k_off, panel);
+            };
             unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
             typename W::template Block<BK> blk;
             u32x4 p[BK / 16];
-            blk.scores(w, at, lane);
+            blk.scores(w, at, lane, between);
             if constexpr (DW > 1) blk.join(shares + wave * kShares, shares + (wave ^ 1) * kShares, lane);
             blk.softmax(w, span.first(b), span.end(b), a.c, lane, p, curve);
             blk.product(w, at + Kv::kBytes, lane, p);
