@@ -197,6 +197,7 @@ struct Wide {
             blk.product(w, at + Kv::kBytes, lane, p);
         }
         for (; b < blocks; b++) pass(b);
+        wait_vmcnt<0>();  // the copies of no bytes past the last block, which still write LDS
         // No one reads K and V any more. (With its barriers after the rows' stores a wave waited 1.7 us for those to arrive.)
         held.share(lds);
         if (n > 0) {
