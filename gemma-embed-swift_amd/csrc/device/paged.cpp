@@ -132,9 +132,8 @@ void check_rotary(const ge_rotary_desc& d) {
 constexpr const char* kRotate = "rotate_heads";
 constexpr const char* kAppend = "paged_append";
 
-// The checks and arguments of both entries over rows of heads, and the unit that shape and strides come in (rotary.hpp).
-HeadsArgs heads_args(const char* op, ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, bool append, ge_heads_shape* checked,
-                     int* unit) {
+// The checks and arguments of both entries over rows of heads.
+HeadsArgs heads_args(const char* op, ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, bool append, ge_heads_shape* checked) {
     if (!shape) fail(GE_ERR_INVALID, "%s: null shape", op);
     ge_heads_shape s = *shape;
     if (s.type != GE_TYPE_F16 && s.type != GE_TYPE_BF16) fail(GE_ERR_INVALID, "%s: results of type %d (F16 or BF16)", op, s.type);
@@ -178,13 +177,6 @@ HeadsArgs heads_args(const char* op, ge_ctx* c, const ge_heads_shape* shape, con
         a.fade = r->fade;
         a.gain = r->gain;
     }
-    // (units of fp32 rows: 16 bytes at most; wave lanes: up to 64 units a half)
-    const auto rows_in = [&](int u) {
-        const int in = std::min(u, s.in_type == GE_TYPE_F32 ? 4 : 8);
-        return s.q_stride % in == 0 && s.k_stride % in == 0 && s.q_out_stride % u == 0 && (append ? s.v_stride % in == 0 : s.k_out_stride % u == 0);
-    };
-    *unit = 8;
-    while (*unit > 1 && !(s.head_dim % (2 * *unit) == 0 && s.head_dim <= 128 * *unit && a.half % *unit == 0 && rows_in(*unit))) *unit /= 2;
     *checked = s;
     return a;
 }
@@ -198,12 +190,23 @@ struct Operand {
     bool rows;  // read or written a unit at a time
 };
 
-void check_operands(const char* op, std::initializer_list<Operand> list, int* unit) {
+// Checks them and returns the unit of a call: the largest that its heads, the part that turns, its strides and its
+// addresses come in together, accesses being of 16 bytes at most. (One rule: a unit that one of them refuses may leave
+// only a smaller one than the next, as heads past 256 elements do, which come in units of 4 and 1 but not of 2.)
+int operands_unit(const char* op, const ge_heads_shape& s, int half, bool append, std::initializer_list<Operand> list) {
     for (const Operand& o : list) {
         if (o.needed && !o.p) fail(GE_ERR_INVALID, "%s: null %s", op, o.name);
         if (!aligned(o.p, size_t(o.size))) fail(GE_ERR_INVALID, "%s: %s is not aligned to its elements", op, o.name);
-        while (o.rows && *unit > 1 && !aligned(o.p, size_t(std::min(16, *unit * o.size)))) *unit /= 2;
     }
+    const auto moves_in = [&](int u) {
+        const int in = std::min(u, s.in_type == GE_TYPE_F32 ? 4 : 8);
+        return heads_unit_ok(s.head_dim, half, u) && s.q_stride % in == 0 && s.k_stride % in == 0 && s.q_out_stride % u == 0 &&
+               (append ? s.v_stride % in == 0 : s.k_out_stride % u == 0) &&
+               std::all_of(list.begin(), list.end(), [&](const Operand& o) { return !o.rows || aligned(o.p, size_t(std::min(16, u * o.size))); });
+    };
+    int unit = 8;
+    while (!moves_in(unit)) unit /= 2;  // in units of 1 it does
+    return unit;
 }
 
 // Results may take their operand's place row by row and head by head, where both are of one type.
@@ -216,12 +219,12 @@ void check_in_place(const char* op, const char* what, const ge_heads_shape& s, c
 void rotate(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const void* q, const void* k, const void* q_norm,
             const void* k_norm, const void* positions, void* q_out, void* k_out) {
     ge_heads_shape s;
-    int unit = 1;
-    HeadsArgs a = heads_args(kRotate, c, shape, r, false, &s, &unit);
+    HeadsArgs a = heads_args(kRotate, c, shape, r, false, &s);
     if (s.rows == 0) return;
     const int in = s.in_type == GE_TYPE_F32 ? 4 : 2;
-    check_operands(kRotate, {{"q", q, s.heads > 0, in, true}, {"k", k, s.kv_heads > 0, in, true}, {"q_out", q_out, s.heads > 0, 2, true},
-                             {"k_out", k_out, s.kv_heads > 0, 2, true}, {"q_norm", q_norm, false, 4, false}, {"k_norm", k_norm, false, 4, false}}, &unit);
+    const int unit = operands_unit(kRotate, s, a.half, false,
+                                   {{"q", q, s.heads > 0, in, true}, {"k", k, s.kv_heads > 0, in, true}, {"q_out", q_out, s.heads > 0, 2, true},
+                                    {"k_out", k_out, s.kv_heads > 0, 2, true}, {"q_norm", q_norm, false, 4, false}, {"k_norm", k_norm, false, 4, false}});
     check_in_place(kRotate, "q", s, q, s.q_stride, q_out, s.q_out_stride);
     check_in_place(kRotate, "k", s, k, s.k_stride, k_out, s.k_out_stride);
     if (r && !positions) fail(GE_ERR_INVALID, "%s: null positions", kRotate);
@@ -263,8 +266,7 @@ void append(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const vo
             const void* q_norm, const void* k_norm, const void* positions, const ge_page_table* t, const ge_paged_seq* seqs,
             int n_seqs, void* q_out, void* k_pages, void* v_pages) {
     ge_heads_shape s;
-    int unit = 1;
-    HeadsArgs a = heads_args(kAppend, c, shape, r, true, &s, &unit);
+    HeadsArgs a = heads_args(kAppend, c, shape, r, true, &s);
     check_table(kAppend, c, t);
     if (s.kv_heads == 0) fail(GE_ERR_INVALID, "%s: no KV heads", kAppend);
     if (n_seqs < 0) fail(GE_ERR_INVALID, "%s: %d sequences", kAppend, n_seqs);
@@ -282,9 +284,10 @@ void append(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const vo
         rows += e.q_len;
     }
     const int in = s.in_type == GE_TYPE_F32 ? 4 : 2;
-    check_operands(kAppend, {{"q", q, s.heads > 0, in, true}, {"k", k, true, in, true}, {"v", v, true, in, true}, {"q_out", q_out, s.heads > 0, 2, true},
-                             {"k_pages", k_pages, true, 2, true}, {"v_pages", v_pages, true, 2, true}, {"q_norm", q_norm, false, 4, false},
-                             {"k_norm", k_norm, false, 4, false}}, &unit);
+    const int unit = operands_unit(kAppend, s, a.half, true,
+                                   {{"q", q, s.heads > 0, in, true}, {"k", k, true, in, true}, {"v", v, true, in, true}, {"q_out", q_out, s.heads > 0, 2, true},
+                                    {"k_pages", k_pages, true, 2, true}, {"v_pages", v_pages, true, 2, true}, {"q_norm", q_norm, false, 4, false},
+                                    {"k_norm", k_norm, false, 4, false}});
     check_in_place(kAppend, "q", s, q, s.q_stride, q_out, s.q_out_stride);
     if (!aligned(positions, 4)) fail(GE_ERR_INVALID, "%s: positions are not aligned to their elements", kAppend);
     claim_pages(t, seqs, n_seqs);

@@ -466,22 +466,17 @@ hipError_t run_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in,
     }
 }
 
-// What the kernels assume of a unit.
-bool unit_ok(const HeadsArgs& a, int unit) {
-    return unit == 1 || ((unit == 2 || unit == 4 || unit == 8) && a.head_dim % (2 * unit) == 0 && a.head_dim <= 128 * unit && a.half % unit == 0);
-}
-
 }  // namespace
 
 hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, bool bf16, int unit) {
-    if (!heads_ok(a) || !unit_ok(a, unit) || a.rows_each <= 0 || (a.half && !a.positions)) return hipErrorInvalidValue;
+    if (!heads_ok(a) || !heads_unit_ok(a.head_dim, a.half, unit) || a.rows_each <= 0 || (a.half && !a.positions)) return hipErrorInvalidValue;
     if (a.rows == 0) return hipSuccess;
     if (in_f32) return bf16 ? run_rotate<F32, BF16>(s, a, unit) : run_rotate<F32, F16>(s, a, unit);
     return bf16 ? run_rotate<BF16, BF16>(s, a, unit) : run_rotate<F16, F16>(s, a, unit);
 }
 
 hipError_t launch_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool in_f32, bool bf16, int unit) {
-    if (!heads_ok(a) || !unit_ok(a, unit) || a.n_items < 0 || a.workgroups < a.n_items || a.rows_each <= 0 ||
+    if (!heads_ok(a) || !heads_unit_ok(a.head_dim, a.half, unit) || a.n_items < 0 || a.workgroups < a.n_items || a.rows_each <= 0 ||
         (a.items ? a.workgroups != a.n_items : a.n_items > kAppendInlineItems))
         return hipErrorInvalidValue;
     if (a.n_items == 0) return hipSuccess;

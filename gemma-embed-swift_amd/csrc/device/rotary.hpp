@@ -46,7 +46,13 @@ static_assert(sizeof(HeadsArgs) + sizeof(AppendInline) <= 4096, "kernel argument
 // 73.5 and 83.0 us).
 inline int heads_rows_each(int rows) { return rows <= 1024 ? 1 : rows <= 4 * 4096 ? 4 : (rows / 4096 + 3) / 4 * 4; }
 
-// unit: 8, 4, 2 or 1 elements, in which head_dim / 2, half, every stride and every address come (fp32 rows: 16 bytes at most).
+// Whether heads and the pairs that turn come in units of 8, 4, 2 or 1 elements, of which a wave holds 64 of each half of a
+// head (units of 1: four a lane).
+inline bool heads_unit_ok(int head_dim, int half, int unit) {
+    return unit == 1 || ((unit == 2 || unit == 4 || unit == 8) && head_dim % (2 * unit) == 0 && head_dim <= 128 * unit && half % unit == 0);
+}
+
+// unit: one for which heads_unit_ok holds and in which every stride and every address come (fp32 rows: 16 bytes at most).
 hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, bool bf16, int unit);
 hipError_t launch_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool in_f32, bool bf16, int unit);
 // Page numbers into a table: entries of (place in the table, page) pairs.
