@@ -48,15 +48,20 @@ struct KvBlock {
     }
     // Chunk (PANEL, k8) of a block whose rows start at r's base; off: the lane's offset of row 8 k8. Rows past
     // r's size read as zeros. The panel goes into the instruction's offset, which moves the LDS address as well
-    // as the source's, so that a wave's chunks of a row group share one offset register.
-    static __device__ __forceinline__ void copy(__amdgpu_buffer_rsrc_t r, unsigned char* block, int k8, uint32_t off, int panel) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            r, (__attribute__((address_space(3))) void*)(block + (panel * (BK / 8) + k8) * 1024), 16, off, panel * 128, 0, 0);
-    }
+    // as the source's, so that a wave's chunks of a row group share one offset register. (Not into the scalar offset: that
+    // one is no part of what is compared with r's size, and taken off it the size of a resource of no rows would be negative.)
     template <int PANEL>
     static __device__ __forceinline__ void copy(__amdgpu_buffer_rsrc_t r, unsigned char* block, int k8, uint32_t off) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             r, (__attribute__((address_space(3))) void*)(block + (PANEL * (BK / 8) + k8) * 1024 - PANEL * 128), 16, off, 0, PANEL * 128, 0);
+    }
+    // The same for a panel that is a constant once its loop is unrolled.
+    template <int PANEL = 0>
+    static __device__ __forceinline__ void copy_panel(__amdgpu_buffer_rsrc_t r, unsigned char* block, int k8, uint32_t off, int panel) {
+        if (panel == PANEL)
+            copy<PANEL>(r, block, k8, off);
+        else if constexpr (PANEL + 1 < HD / 64)
+            copy_panel<PANEL + 1>(r, block, k8, off, panel);
     }
     // The wave's chunks of panels [0, PANELS) and row groups k8, k8 + STEP, ... in this order.
     template <int PANELS, int STEP, int I = 0>

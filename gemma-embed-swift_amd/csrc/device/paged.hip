@@ -186,7 +186,7 @@ struct Wide {
                 constexpr int P = HD / 64, C = NG * 2 * P;
                 if (!kBetween || step % (steps / C)) return;
                 const int c = step / (steps / C), i = c / (2 * P), v = c / P % 2, panel = c % P;
-                Kv::copy(v ? rv[i] : rk[i], next + v * Kv::kBytes, wave + i * NW, v ? v_off : k_off, panel);
+                Kv::copy_panel(v ? rv[i] : rk[i], next + v * Kv::kBytes, wave + i * NW, v ? v_off : k_off, panel);
             };
             unsigned char* const at = lds + (b & 1) * 2 * Kv::kBytes;
             typename W::template Block<BK> blk;
