@@ -273,8 +273,11 @@ PagedPlan plan_paged(const ge_paged_shape& s, const ge_paged_seq* seqs, int n_se
         // longest at the end, 10%; shares of wide tiles, over different keys at a time, miss the L2, 15%.
         const bool single = 2 * groups.size() > tiles.size();
         float best = us(float(heaviest(tiles, longest, total, cus)), float(longest + kItemUnits)) * (single ? 1.1f : 1.0f);
-        // (a row of more than 128 parts waits for its join: a token over 30000 keys, head dim 256, in 469, 235 and 118 parts 10.7 + 11.2,
-        // 11.0 + 7.4 and 13.4 + 5.4 us, head dim 128 9.3 + 12.3, 8.8 + 8.0 and 9.7 + 5.6)
+        // A row of many parts waits for its join: shares have as many whole units as bring the longest tile to 128 to 255 parts. A
+        // token over 30000 keys, head dim 256, in 469, 235 and 118 parts 10.7 + 11.2, 11.0 + 7.4 and 13.4 + 5.4 us, head dim 128
+        // 9.3 + 12.3, 8.8 + 8.0 and 9.7 + 5.6; over 16319 keys in 255 and 127 parts (one KV head of 64, 128, 256 and 512) 12.6 and
+        // 11.1, 15.6 and 13.1, 16.4 and 16.4, 23.6 and 24.7, over 32000 in 166 and 125 12.3 and 11.8, 15.4 and 14.4, 17.9 and 19.3,
+        // 30.2 and 31.7.
         const int64_t n = std::min(at_once, (total - n_tiles * kItemUnits) / std::max(kLeastPart, longest / 128));
         if (n > 1) {
             const float share = float(total) / float(n) + kItemUnits;
