@@ -299,6 +299,7 @@ void append(ge_ctx* c, const ge_heads_shape* shape, const ge_rotary* r, const vo
         groups += (size_t(seqs[i].q_len) + each - 1) / each;
         some += seqs[i].q_len > 0;
     }
+    if (groups > kCausalMaxGroups) fail(GE_ERR_INVALID, "%s: %zu sequences with rows are too many for one call", kAppend, some);
     const bool inlined = some <= size_t(kAppendInlineItems);
     OpTemps temps(c);
     AppendInline few;

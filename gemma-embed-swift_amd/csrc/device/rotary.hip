@@ -476,7 +476,7 @@ hipError_t launch_rotate_heads(hipStream_t s, const HeadsArgs& a, bool in_f32, b
 }
 
 hipError_t launch_append(hipStream_t s, const HeadsArgs& a, const AppendInline& in, bool in_f32, bool bf16, int unit) {
-    if (!heads_ok(a) || !heads_unit_ok(a.head_dim, a.half, unit) || a.n_items < 0 || a.workgroups < a.n_items || a.rows_each <= 0 ||
+    if (!heads_ok(a) || !heads_unit_ok(a.head_dim, a.half, unit) || a.n_items < 0 || a.workgroups < a.n_items || uint64_t(a.workgroups) * 256 >> 32 || a.rows_each <= 0 ||
         (a.items ? a.workgroups != a.n_items : a.n_items > kAppendInlineItems))
         return hipErrorInvalidValue;
     if (a.n_items == 0) return hipSuccess;

@@ -404,7 +404,7 @@ typedef struct ge_paged_seq {
  * back; both may interleave in one buffer), [kv_heads][page_rows][head_dim]. Every page written must be in its slot, and a page
  * is written by one sequence of a call at one place: else nothing is written and the call refused. Other rows of pages,
  * and rows of q_out outside the sequences, stay as they were. q_out may be q, of one type and stride; no query heads: q
- * and q_out may be null. */
+ * and q_out may be null. Around 2^24 sequences with rows are too many for one call. */
 int ge_op_paged_append(ge_ctx* ctx, const ge_heads_shape* shape, const ge_rotary* rotary, const void* q, const void* k,
                        const void* v, const void* q_norm, const void* k_norm, const void* positions,
                        const ge_page_table* table, const ge_paged_seq* seqs, int32_t n_seqs, void* q_out, void* k_pages,
