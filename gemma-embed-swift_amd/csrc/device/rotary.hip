@@ -204,7 +204,8 @@ __device__ __forceinline__ void store(uint16_t* p, const Place<UNIT>& at, const 
 }
 
 // x / sqrt(mean(x^2) + eps). Squares that leave fp32's range, or get lost below it where eps does not
-// outweigh them, are taken of x times a power of two.
+// outweigh them, are taken of x times a power of two: 2^90 brings the smallest element's square over 512 to 2^-127, which has
+// 22 bits, and a sum below 2^-60 to 2^120.
 template <int N>
 __device__ __forceinline__ void norm(float (&a)[N], float (&b)[N], bool on, int log, float inv_dim, float eps) {
     auto squares = [&] {
@@ -216,7 +217,7 @@ __device__ __forceinline__ void norm(float (&a)[N], float (&b)[N], bool on, int 
     float ss = squares(), e = eps;
     const bool large = on && !(ss <= 1e37f), small = on && ss < 0x1p-60f && eps < 0x1p-100f;
     if (__builtin_amdgcn_ballot_w64(large || small)) {
-        const float f = large ? 0x1p-100f : small ? 0x1p80f : 1.0f;
+        const float f = large ? 0x1p-100f : small ? 0x1p90f : 1.0f;
 #pragma unroll
         for (int i = 0; i < N; i++) {
             a[i] *= f;
