@@ -120,6 +120,8 @@ void check_rotary(const ge_rotary_desc& d) {
     if (d.scaling < GE_ROTARY_PLAIN || d.scaling > GE_ROTARY_BY_TURNS) fail(GE_ERR_INVALID, "rotary: scaling %d", d.scaling);
     if (!(d.base > 0.0f) || !std::isfinite(d.base)) fail(GE_ERR_INVALID, "rotary: base must be positive and finite");
     if (!std::isfinite(d.magnitude)) fail(GE_ERR_INVALID, "rotary: magnitude is not finite");
+    // (sines and cosines times it are fp32 values)
+    if (d.magnitude != 0.0f && std::fabs(d.magnitude) < FLT_MIN) fail(GE_ERR_INVALID, "rotary: magnitude below 2^-126 and not 0");
     if (d.scaling != GE_ROTARY_PLAIN && (!(d.factor > 0.0f) || !std::isfinite(d.factor)))
         fail(GE_ERR_INVALID, "rotary: factor must be positive and finite");
     if (d.scaling == GE_ROTARY_BY_TURNS &&

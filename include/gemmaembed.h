@@ -347,7 +347,7 @@ typedef struct ge_rotary_desc {
     float base;
     float factor;      /* LINEAR and BY_TURNS */
     float low_turns, high_turns; /* BY_TURNS: low_turns < high_turns */
-    float magnitude;   /* 0: 1 */
+    float magnitude;   /* 0: 1; else from 2^-126 on, either sign */
 } ge_rotary_desc;
 typedef struct ge_rotary ge_rotary;
 int ge_op_rotary_create(ge_ctx* ctx, const ge_rotary_desc* desc, ge_rotary** out);

@@ -29,3 +29,11 @@ def test_sequences_of_an_append(ctx, memory, n):
         lib.host_hip_on_launch(LAUNCH())
     assert len(names) == (n < 1 << 24)
     ctx.page_table_destroy(h)
+
+
+def test_magnitudes_below_normal_numbers(ctx):
+    """A sine or cosine times such a magnitude has few bits: at 2^-147 the products are off by an eighth."""
+    for m in (2.0 ** -126, -2.0 ** -126, 0.0, -0.0, 1e-30):
+        ctx.rotary_destroy(ctx.rotary_create(64, 1e4, magnitude=m))
+    for m in (2.0 ** -127, -2.0 ** -127, 2.0 ** -149):
+        refused(ctx.rotary_create, 64, 1e4, magnitude=m)
