@@ -358,7 +358,8 @@ int ge_op_rotary_destroy(ge_ctx* ctx, ge_rotary* rotary);
  * they may be views of one projection's output. Inputs are of in_type (GE_TYPE_F32 or the results' type), results of
  * type (GE_TYPE_F16 or GE_TYPE_BF16). Up to 4096 heads of each kind (0 for none, where an entry allows it), head_dim even
  * up to 512, rows under 2^30, strides up to 2^24. Buffers are aligned to their elements; rows move in units of 8, 4, 2 or
- * 1 elements, the largest that head_dim / 2, dims / 2, strides and addresses come in (up to 16 bytes), larger ones faster.
+ * 1 elements, the largest that head_dim / 2, dims / 2, strides and addresses come in (up to 16 bytes; of 2 only up to
+ * head_dim 256), larger ones faster.
  * normed: which heads are RMS-normed first, x / sqrt(mean x^2 + eps) * w over the head, w fp32 [head_dim] (null: 1);
  * value heads have no weight. All in fp32, rounded once. */
 enum { GE_NORM_Q = 1, GE_NORM_K = 2, GE_NORM_V = 4 };
@@ -368,7 +369,7 @@ typedef struct ge_heads_shape {
     int32_t normed;
     float eps;
     int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
-    int64_t page_stride; /* ge_op_paged_append: elements from one page to the next, 0: back to back */
+    int64_t page_stride; /* ge_op_paged_append: elements from one page to the next, a multiple of 8; 0: back to back */
 } ge_heads_shape;
 
 /* q_out and k_out = the rows of q and k, normed (Q and K) and turned. positions: device int32 [rows], any values; rotary
@@ -400,8 +401,8 @@ typedef struct ge_paged_seq {
 
 /* Appends the call's tokens: row i of a sequence is at position and cache row kv_len - q_len + i (positions, device int32
  * [rows], nullable: other positions to turn by). q_out = q normed and turned; k normed and turned and v (normed with
- * GE_NORM_V) go to their pages. Pools k_pages and v_pages: page p from element p page_stride on (0: pages back to
- * back; both may interleave in one buffer), [kv_heads][page_rows][head_dim]. Every page written must be in its slot, and a page
+ * GE_NORM_V) go to their pages. Pools k_pages and v_pages: page p from element p page_stride on (a multiple of 8 up to
+ * 2^40; 0: pages back to back; both may interleave in one buffer), [kv_heads][page_rows][head_dim]. Every page written must be in its slot, and a page
  * is written by one sequence of a call at one place: else nothing is written and the call refused. Other rows of pages,
  * and rows of q_out outside the sequences, stay as they were. q_out may be q, of one type and stride; no query heads: q
  * and q_out may be null. Around 2^24 sequences with rows are too many for one call. */
