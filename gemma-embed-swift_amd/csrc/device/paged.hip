@@ -10,10 +10,11 @@
 //
 // What bounds it, of 1.3 PFLOP/s (a large product) and 7.0 TB/s (reads of one run; 5.9 of 4 KB pieces in no order): long prompts
 // at head dim 128 the card's power, the matrix pipe 56% busy at 1.66 GHz (8192 tokens over 16192 keys, 32 heads over 8: 1445
-// to 1605 us on several cards, 1.01 to 1.12 PFLOP/s); at head dim 64 the exponentials (16 heads over 8: 445 to 520 us, 0.78 to
-// 0.91 PFLOP/s); at 512 a workgroup's 64 rows, half of what its reads of LDS could feed (4 heads: 1340 to 1435 us, 0.57 to 0.61).
+// to 1605 us on several cards, 1.01 to 1.12 PFLOP/s); at head dim 64 exponentials and sums beside the products, the VALU 62%
+// and the matrix pipe 41% busy (16 heads over 8: 445 to 520 us, 0.78 to 0.91 PFLOP/s); at 256 the same with 35 and 48% (4 heads
+// over 2: 400 and 22 us, 0.97); at 512 one wave a SIMD, beside which nothing runs while it waits: 33 and 25% (4 heads: 1290 us, 0.63).
 // Tokens the reads (64 over 100 to 8000 keys, pages of 16: 182 us, 5.5 TB/s). Chunks the few items a CU and the parts they leave
-// (5 x 301 to 700 over 2000 to 9700, 16 heads of 64 over 8: 87 and 9 us, 0.65 PFLOP/s; 3 x 500 to 1500, window 1024, 4 capped
+// (5 x 301 to 700 over 2000 to 9700, 16 heads of 64 over 8: 87 to 94 and 9 us, 0.60 to 0.65 PFLOP/s; 3 x 500 to 1500, window 1024, 4 capped
 // heads of 256 over 2: 34 and 8 us, of which 15 are keys and 12 the way in and out).
 #include "causal_rows.hpp"
 #include "paged.hpp"
