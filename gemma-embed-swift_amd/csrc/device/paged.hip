@@ -385,15 +385,15 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(const CausalArgs a,
         }
         float top = m;
 #pragma unroll
-        for (int i = 0; i < 4; i++) top = fmaxf(top, ml[i].y == 0.0f ? -INFINITY : ml[i].x);
+        for (int i = 0; i < 4; i++) top = fmaxf(top, ml[i].x);
         const float fade = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
         l *= fade;
 #pragma unroll
         for (int e = 0; e < E; e++) o[e] *= fade;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            // a part that saw no key has nothing to add, whatever its rows hold
-            if (ml[i].y == 0.0f) continue;
+            // (a part without a weight adds zeros, or the NaN of an infinite value whose key weighs nothing)
+            if (s0 + uint32_t(i * split) >= parts) continue;
             const float f = ml[i].x == top ? 1.0f : __builtin_amdgcn_exp2f(ml[i].x - top);
             l = __builtin_fmaf(ml[i].y, f, l);
 #pragma unroll
@@ -415,7 +415,6 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(const CausalArgs a,
     for (int e = 0; e < E; e++) o[e] = float4_t{};
     for (int i = 0; i < split; i++) {
         const float2 ml = lds_ml[group + i];
-        if (ml.y == 0.0f) continue;
         const float f = ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
         sum = __builtin_fmaf(ml.y, f, sum);
 #pragma unroll

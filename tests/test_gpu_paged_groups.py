@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import gemma_embed as ge
-from test_gpu_causal import BF16, F16
+from test_gpu_causal import BF16, F16, to_bits, to_float
 from test_gpu_paged import INF, NAN, attend
 
 pytestmark = pytest.mark.gpu
@@ -59,3 +59,20 @@ def test_windows_and_caps_of_many_heads(ctx, heads, kv_heads, hd, kind):
 def test_chunks_of_many_heads(ctx, heads, kv_heads, hd, kind, window):
     """Stacked rows of a token in several tiles, and tiles that begin within a token."""
     attend(ctx, [(0, 3, 200), (3, 7, 7), (11, 2, 77), (13, 5, 2)], heads, kv_heads, hd, kind, 16, window=window, seed=5, edit=nan_in_page_0)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(2, 1, 64), (4, 4, 128), (3, 1, 256), (2, 1, 512), (48, 1, 128)])
+def test_infinite_values_of_keys_that_weigh_nothing(ctx, heads, kv_heads, hd):
+    """A value that a row sees reaches it however little its key weighs, also where a whole part's scores fall past fp32's
+    lowest: an infinity there is 0 times infinity in the definition."""
+    def edit(q, cache):
+        q[:] = to_bits(np.full(q.shape, 2.0 ** 40), BF16)
+        for j in range(192):
+            cache.row(cache.k, 0, j)[:] = to_bits(np.full((kv_heads, hd), -(2.0 ** 100)), BF16)
+        cache.row(cache.v, 0, 5)[0, 3] = INF[BF16]
+        cache.row(cache.v, 0, 70)[-1, hd - 1] = NAN[BF16]
+        cache.row(cache.v, 0, 1500)[0, 9] = INF[BF16]
+
+    got = attend(ctx, [(0, 1, 2000)], heads, kv_heads, hd, BF16, scale=2.0 ** -44, edit=edit, seed=hd)
+    f = to_float(got[0], BF16).reshape(heads, hd)
+    assert np.isnan(f[0, 3]) and np.isnan(f[-1, hd - 1]) and f[0, 9] == np.inf and np.isfinite(f[0, 4:9]).all()
