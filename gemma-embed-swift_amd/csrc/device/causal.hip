@@ -280,9 +280,9 @@ __global__ __launch_bounds__(256) void causal_join_kernel(const CausalArgs a, co
     float4_t o[E] = {};
     for (uint32_t s0 = 0; s0 < parts; s0 += L) {
         const float2 ml = load(s0 + lane);
-        // a part that saw no key has nothing to add, whatever its rows hold
-        const float f = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
-        sum += ml.y == 0.0f ? 0.0f : ml.y * f;
+        // (a part without a weight adds zeros, or the NaN of an infinite value whose key weighs nothing)
+        const float f = ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
+        sum += ml.y * f;
         const int n = int(min(uint32_t(L), parts - s0));
         for (int i0 = 0; i0 < n; i0 += 4) {  // four parts' loads in flight
             float4_t x[4][E];
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(256) void causal_join_kernel(const CausalArgs a, co
             for (int i = 0; i < 4; i++) {
                 const int k = group0 + min(i0 + i, n - 1);
                 const float w = __shfl(f, k, 64);
-                const bool none = i0 + i >= n || __shfl(ml.y, k, 64) == 0.0f;
+                const bool none = i0 + i >= n;
 #pragma unroll
                 for (int e = 0; e < E; e++)
 #pragma unroll
